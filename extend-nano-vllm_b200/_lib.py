@@ -86,7 +86,18 @@ SIGNATURES: dict[str, tuple] = {
     "b200moe_nvl_return": (_I, [_P, _I, _P, _P, _P, _L, _L, _I, _I, _P, _P, _P]),
     "b200moe_nvl_wait_return": (_I, [_I, _I, _P, _P, _P]),
     "b200moe_nvl_return_signal": (_I, [_I, _I, _P, _P, _P]),
+    "b200moe_route_scored_topk": (_I, [_P, _I, _L, _I, _I, _I, _P, _I, _I, _I, _I,
+                                       ctypes.c_float, _P, _P, _P]),
+    "b200moe_w4_bytes": (_L, [_L, _L, _L, _I, _I]),
+    "b200moe_w4_pack": (_I, [_P, _P, _P, _L, _L, _L, _I, _I, _P, _P]),
+    "b200moe_w4_linear": (_I, [_P, _L, _I, _I, _P, _I, _I, _P, _P]),
+    "b200moe_w4_experts_workspace": (_L, [_L, _I, _I, _I, _I]),
+    "b200moe_w4_experts": (_I, [_P, _L, _I, _I, _P, _P, _I, _I, _P, _I, _I, _P, _I, _I, _P, _L,
+                                _P, _P]),
 }
+SCORE_CODES = {"softmax": 0, "sigmoid": 1}
+GROUP_SCORE_CODES = {"max": 0, "top2": 1}
+W4_ZEROS, W4_F16_SCALES, W4_GATE_UP = 1, 2, 4
 NVL_LAYOUT_WORDS = 10
 NVL_ROUTE_CAP = 8  # layout word: route records per source region
 

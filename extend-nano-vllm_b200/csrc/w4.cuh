@@ -1,0 +1,72 @@
+// 4-bit weights with group scales: the layout that the kernels read, and the
+// conversion of codes to operands.
+//
+//   W[n, k] = scale[n, k / g] * (q[n, k] - zero[n, k / g]),  q in 0..15,
+//   g in {32, 64, 128}, zero = 8 where no zero points are given.
+//
+// A matrix [rows, k] is laid out once as tiles of 128 rows; a tile is a run of
+// blocks of 128 k, each one contiguous piece of memory:
+//   codes  4 chunks x 128 rows x 16 bytes: chunk c holds 32 k of every row, so
+//          32 lanes that own 32 rows read 512 consecutive bytes;
+//   scales [128 / g][128 rows] of 16 bits (bf16 or fp16);
+//   zeros  [128 / g][128 rows] of 8 bits, only with zero points.
+// In each 32-bit word of a chunk, k = 8 j + 2 i sits at bit 4 i and
+// k = 8 j + 2 i + 1 at bit 16 + 4 i: (word >> 4 i) & 0x000f000f is a pair of
+// neighbouring k in the halves of a register, which is how the matrix
+// instruction wants them.  Rows and k beyond the matrix have scale 0.
+//
+// "gate_up" order: a tile holds 64 features of a SwiGLU pair [2 I, k] (gate
+// rows first); each quarter of 32 rows is 16 gate rows, then the 16 up rows of
+// the same features, so one warp owns both factors of its products.
+#pragma once
+
+#include "common.cuh"
+
+namespace b200moe {
+namespace w4 {
+
+constexpr int kTileRows = 128;
+constexpr int kBlockK = 128;
+constexpr int kCodeBytes = kTileRows * kBlockK / 2;  // 8192 per block
+
+struct Shape {
+  int group;       // k per scale: 32, 64 or 128
+  int has_zero;    // zero points follow the scales
+  int half_scale;  // scales are fp16 (else bf16)
+  __host__ __device__ int groups_per_block() const { return kBlockK / group; }
+  __host__ __device__ int scale_off() const { return kCodeBytes; }
+  __host__ __device__ int zero_off() const { return kCodeBytes + groups_per_block() * 256; }
+  __host__ __device__ int block_bytes() const {
+    return kCodeBytes + groups_per_block() * (has_zero ? 384 : 256);
+  }
+};
+
+inline Shape shape_of(int group, int flags) {
+  return Shape{group, (flags & B200MOE_W4_ZEROS) != 0, (flags & B200MOE_W4_F16_SCALES) != 0};
+}
+inline bool group_ok(int group) { return group == 32 || group == 64 || group == 128; }
+__host__ __device__ inline int64_t blocks_of(int64_t k) { return (k + kBlockK - 1) / kBlockK; }
+
+__device__ __forceinline__ float scale_f32(uint16_t bits, int half_scale) {
+  return half_scale ? __half2float(__ushort_as_half(bits))
+                    : __uint_as_float(static_cast<uint32_t>(bits) << 16);
+}
+
+// (128 + z) in both halves, as bf16 (exact: bf16 has steps of 1 from 128 to 256).
+__device__ __forceinline__ uint32_t zero_pair(uint32_t z) { return 0x43004300u | z | (z << 16); }
+
+// Eight codes -> four pairs q - z in bf16.  The code goes into the low bits
+// of 128.0 (0x4300), which reads as 128 + q; subtracting 128 + z leaves the
+// integer q - z, exact in bf16.
+__device__ __forceinline__ void decode8(uint32_t word, uint32_t zpair, uint32_t (&out)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t v = ((word >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&v),
+                                     *reinterpret_cast<const __nv_bfloat162 *>(&zpair));
+    out[i] = *reinterpret_cast<const uint32_t *>(&d);
+  }
+}
+
+}  // namespace w4
+}  // namespace b200moe

@@ -9,6 +9,7 @@ graphs (no host synchronisation happens inside them).
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from dataclasses import dataclass
 
@@ -475,3 +476,198 @@ def expert_down_scatter(engine: int, act: torch.Tensor, w2: torch.Tensor, packed
 def nvl_wait_return(rank: int, bufs) -> None:
     call("b200moe_nvl_wait_return", rank, bufs.ep_size, bufs.peer_bases, bufs.layout_ptr,
          bufs.stream_ptr())
+
+
+# ---------------------------------------------------------------------------
+# Scored routing.
+# ---------------------------------------------------------------------------
+def route_scored_topk(logits: torch.Tensor, top_k: int, *, score: str = "softmax",
+                      bias: torch.Tensor | None = None, num_groups: int = 1,
+                      topk_groups: int = 1, group_score: str = "top2", renormalize: bool = True,
+                      scale: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """Scored top-k routing of [T, E] logits -> (bf16 weights, int64 ids) [T, k].
+
+    ``score``: "softmax" or "sigmoid" of the logits.  ``bias`` (fp32 [E]) is
+    added to the scores for the choice only; the weights are the scores
+    themselves, renormalised over the k chosen (``renormalize``) and multiplied
+    by ``scale``.  With ``num_groups`` > 1 the experts form that many equal
+    groups and only the ``topk_groups`` best ones are on offer; a group's
+    score is its largest biased score ("max") or the sum of its two largest
+    ("top2").  Equal values go to the lowest index."""
+    _require_cuda(logits, bias)
+    if logits.dim() != 2:
+        raise ValueError("router logits must be [tokens, experts]")
+    if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError(f"router logits must be fp32/bf16/fp16, got {logits.dtype}")
+    if score not in _lib.SCORE_CODES:
+        raise ValueError(f"unknown score function {score!r}")
+    if group_score not in _lib.GROUP_SCORE_CODES:
+        raise ValueError(f"unknown group score {group_score!r}")
+    tokens, experts = logits.shape
+    if bias is not None:
+        if bias.dtype != torch.float32 or bias.shape != (experts,):
+            raise TypeError("bias must be fp32 with one value per expert")
+        if bias.device != logits.device:
+            raise ValueError("bias must be on the logits' device")
+        bias = bias.contiguous()
+    logits = logits.contiguous()
+    weights = torch.empty((tokens, top_k), device=logits.device, dtype=torch.bfloat16)
+    ids = torch.empty((tokens, top_k), device=logits.device, dtype=torch.int64)
+    call("b200moe_route_scored_topk", _p(logits), _DTYPE_CODES[logits.dtype], tokens, experts,
+         top_k, _lib.SCORE_CODES[score], _p(bias), num_groups, topk_groups,
+         _lib.GROUP_SCORE_CODES[group_score], int(bool(renormalize)), scale, _p(weights), _p(ids),
+         _stream(logits))
+    return weights, ids
+
+
+# ---------------------------------------------------------------------------
+# 4-bit weights with group scales.
+# ---------------------------------------------------------------------------
+@dataclass
+class W4Weight:
+    """4-bit weights laid out for the kernels (pack_w4): one matrix [rows, k]
+    or a stack of them, W = scale * (code - zero) by groups of ``group`` k."""
+
+    data: torch.Tensor  # uint8
+    matrices: int
+    rows: int
+    k: int
+    group: int
+    flags: int
+
+    @property
+    def device(self) -> torch.device:
+        return self.data.device
+
+
+def quantize_w4(weight: torch.Tensor, group: int = 128, zeros: bool = False
+                ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """Round a weight [..., rows, k] to 4 bits by groups of ``group`` k.
+
+    -> (codes uint8 [..., rows, k], bf16 scales [..., rows, k / group], zero
+    points uint8 of the scales' shape or None).  Without ``zeros`` a group is
+    symmetric (scale = largest magnitude / 7, zero 8); with it the codes span
+    the group's range, 0 included."""
+    if group not in (32, 64, 128):
+        raise ValueError(f"group size {group} must be 32, 64 or 128")
+    if weight.size(-1) % group:
+        raise ValueError("k must be a multiple of the group size")
+    w = weight.float().unflatten(-1, (-1, group))
+    if zeros:
+        low, high = w.amin(-1, keepdim=True).clamp_(max=0), w.amax(-1, keepdim=True).clamp_(min=0)
+        scale = ((high - low) / 15).bfloat16()
+        zero = (-low / scale.float()).round_().nan_to_num_(0.0).clamp_(0, 15)
+    else:
+        scale = (w.abs().amax(-1, keepdim=True) / 7).bfloat16()
+        zero = torch.full_like(scale, 8, dtype=torch.float32)
+    # A group of zeros has scale 0: every code stands for 0 then.
+    codes = (w / scale.float()).nan_to_num_(0.0).round_().add_(zero).clamp_(0, 15)
+    return (codes.to(torch.uint8).flatten(-2), scale.squeeze(-1),
+            zero.squeeze(-1).to(torch.uint8) if zeros else None)
+
+
+def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None, *,
+            layout: str = "rows") -> W4Weight:
+    """Lay codes [rows, k] or [matrices, rows, k] (uint8 0..15), scales (bf16 or
+    fp16) and optional zero points (uint8) [..., rows, k / group] out for the
+    kernels, once.  ``layout="gate_up"``: the rows are a SwiGLU pair [2 I, k],
+    gate rows first (the first weight of ``experts_w4``)."""
+    _require_cuda(codes, scales, zeros)
+    if layout not in ("rows", "gate_up"):
+        raise ValueError(f"unknown layout {layout!r}")
+    if codes.dim() not in (2, 3) or codes.dtype != torch.uint8:
+        raise TypeError("codes must be uint8 [rows, k] or [matrices, rows, k]")
+    if scales.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"scales must be bf16 or fp16, got {scales.dtype}")
+    rows, k = codes.shape[-2:]
+    groups = scales.size(-1)
+    if scales.shape[:-1] != codes.shape[:-1] or groups == 0 or k % groups:
+        raise ValueError("scales must be [..., rows, k / group]")
+    if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != scales.shape):
+        raise TypeError("zeros must be uint8 of the scales' shape")
+    if any(t is not None and t.device != codes.device for t in (scales, zeros)):
+        raise ValueError("codes, scales and zeros must be on one device")
+    matrices = codes.size(0) if codes.dim() == 3 else 1
+    flags = ((_lib.W4_ZEROS if zeros is not None else 0)
+             | (_lib.W4_F16_SCALES if scales.dtype == torch.float16 else 0)
+             | (_lib.W4_GATE_UP if layout == "gate_up" else 0))
+    group = k // groups
+    size = int(_lib.LIB.b200moe_w4_bytes(matrices, rows, k, group, flags))
+    if size < 0:
+        raise ValueError(f"no 4-bit layout for {matrices} x [{rows}, {k}] in groups of {group} "
+                         "(32, 64 or 128; a gate_up weight has an even number of rows)")
+    codes, scales = _aligned(codes), scales.contiguous()
+    zeros = None if zeros is None else zeros.contiguous()
+    data = torch.empty(size, device=codes.device, dtype=torch.uint8)
+    call("b200moe_w4_pack", _p(codes), _p(scales), _p(zeros), matrices, rows, k, group, flags,
+         _p(data), _stream(codes))
+    return W4Weight(data, matrices, rows, k, group, flags)
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous and at a 16-byte address, by a copy where it is not."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _check_w4(x: torch.Tensor, weight: W4Weight, k: int) -> None:
+    if x.dtype != torch.bfloat16:
+        raise TypeError(f"the 4-bit products take bf16 activations, got {x.dtype}")
+    if weight.device != x.device:
+        raise ValueError("weights and activations must be on one device")
+    if weight.k != k:
+        raise ValueError(f"the weight has k = {weight.k}, the activations {k}")
+
+
+def linear_w4(x: torch.Tensor, weight: W4Weight) -> torch.Tensor:
+    """x [..., k] W^T with a 4-bit weight [rows, k] -> bf16 [..., rows]."""
+    _require_cuda(x)
+    _check_w4(x, weight, x.size(-1))
+    if weight.matrices != 1 or weight.flags & _lib.W4_GATE_UP:
+        raise ValueError("linear_w4 takes one weight in the \"rows\" layout")
+    rows = x.numel() // weight.k
+    out = torch.empty((*x.shape[:-1], weight.rows), device=x.device, dtype=torch.bfloat16)
+    x = _aligned(x)
+    call("b200moe_w4_linear", _p(x), rows, weight.rows, weight.k, _p(weight.data), weight.group,
+         weight.flags, _p(out), _stream(x))
+    return out
+
+
+def experts_w4(x: torch.Tensor, expert_ids: torch.Tensor, route_weights: torch.Tensor,
+               w13: W4Weight, w2: W4Weight) -> torch.Tensor:
+    """Routed SwiGLU experts with 4-bit weights -> bf16 [T, H].
+
+    x bf16 [T, H]; expert_ids int64 and route_weights bf16 [T, k] (as the
+    routers return them); w13: every expert's gate and up rows [E, 2 I, H]
+    packed with ``layout="gate_up"``; w2 [E, H, I].  A route whose id is outside
+    [0, E) (a dropped one) contributes nothing."""
+    _require_cuda(x, expert_ids, route_weights)
+    if x.dim() != 2:
+        raise ValueError("x must be [tokens, hidden]")
+    tokens, hidden = x.shape
+    _check_w4(x, w13, hidden)
+    if expert_ids.dtype != torch.int64 or expert_ids.dim() != 2 or expert_ids.size(0) != tokens:
+        raise TypeError("expert_ids must be int64 [tokens, k]")
+    if route_weights.dtype != torch.bfloat16 or route_weights.shape != expert_ids.shape:
+        raise TypeError("route_weights must be bf16 of the ids' shape")
+    if not w13.flags & _lib.W4_GATE_UP or w2.flags & _lib.W4_GATE_UP:
+        raise ValueError("w13 needs the \"gate_up\" layout and w2 the \"rows\" layout")
+    inter = w13.rows // 2
+    if w2.matrices != w13.matrices or w2.rows != hidden or w2.k != inter:
+        raise ValueError(f"w2 must be {w13.matrices} x [{hidden}, {inter}]")
+    if any(t.device != x.device for t in (expert_ids, route_weights, w2.data)):
+        raise ValueError("weights, routes and activations must be on one device")
+    top_k, experts = expert_ids.size(1), w13.matrices
+    out = torch.empty((tokens, hidden), device=x.device, dtype=torch.bfloat16)
+    size = _w4_workspace(tokens, hidden, inter, top_k, experts)
+    workspace = torch.empty(size, device=x.device, dtype=torch.uint8)
+    x, expert_ids, route_weights = _aligned(x), expert_ids.contiguous(), route_weights.contiguous()
+    call("b200moe_w4_experts", _p(x), tokens, hidden, inter, _p(expert_ids), _p(route_weights),
+         top_k, experts, _p(w13.data), w13.group, w13.flags, _p(w2.data), w2.group, w2.flags,
+         _p(workspace), size, _p(out), _stream(x))
+    return out
+
+
+@functools.lru_cache(maxsize=256)
+def _w4_workspace(tokens: int, hidden: int, inter: int, top_k: int, experts: int) -> int:
+    return int(_lib.LIB.b200moe_w4_experts_workspace(tokens, hidden, inter, top_k, experts))

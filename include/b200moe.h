@@ -78,6 +78,18 @@ extern "C" {
 #define B200MOE_CNT_CHUNKS 4      /* number of row chunks (0 when `chunks` is NULL) */
 #define B200MOE_NUM_COUNTERS 5
 
+/* ---- scored routing ----------------------------------------------------- */
+#define B200MOE_SCORE_SOFTMAX 0
+#define B200MOE_SCORE_SIGMOID 1
+#define B200MOE_GROUP_MAX 0  /* a group's score: its largest choice value */
+#define B200MOE_GROUP_TOP2 1 /* the sum of its two largest */
+
+/* ---- 4-bit weights: flags of a laid-out matrix --------------------------- */
+#define B200MOE_W4_ZEROS 1      /* integer zero points per group (else 8) */
+#define B200MOE_W4_F16_SCALES 2 /* scales are fp16 (else bf16) */
+#define B200MOE_W4_GATE_UP 4    /* a SwiGLU pair [2 I, k], gate rows first: its rows are
+                                   interleaved so that one warp holds both factors */
+
 B200MOE_API const char *b200moe_last_error(void);
 B200MOE_API int b200moe_abi_version(void);
 
@@ -583,6 +595,75 @@ B200MOE_API int b200moe_nvl_return_signal(int rank, int ep_size, const uint64_t 
 /* Source: waits until every destination returned its rows. */
 B200MOE_API int b200moe_nvl_wait_return(int rank, int ep_size, const uint64_t *peer_bases,
                                         const int64_t *layout, void *stream);
+
+/*
+ * Scored routing, for layers whose router is not a plain softmax top-k:
+ *   s_e = sigmoid(l_e) or softmax(l)_e,  c_e = s_e + bias_e,
+ *   the topk_groups of num_groups equal expert groups with the largest group
+ *   score (largest c, or sum of the two largest c) stay on offer, the top_k
+ *   experts with the largest c among them are chosen (equal values: lowest
+ *   index first), and
+ *   weight = s_id [/ sum of the chosen s] * scale, rounded to bf16.
+ * fp32 throughout.  A NaN logit or choice value counts as -inf; chosen scores
+ * that sum to 0 give weights 0 when renormalising.
+ *   logits     [num_tokens, num_experts] of logits_dtype (BF16/F16/F32)
+ *   bias       [num_experts] fp32 or NULL
+ *   weights    [num_tokens, top_k] bf16 out
+ *   expert_ids [num_tokens, top_k] int64 out, by descending c
+ * Limits: num_experts <= 1024, top_k <= 32, num_groups <= 32,
+ * top_k <= topk_groups * num_experts / num_groups.
+ */
+B200MOE_API int b200moe_route_scored_topk(const void *logits, int logits_dtype,
+                                          int64_t num_tokens, int num_experts, int top_k,
+                                          int score, const float *bias, int num_groups,
+                                          int topk_groups, int group_score, int renormalize,
+                                          float scale, void *weights, int64_t *expert_ids,
+                                          void *stream);
+
+/*
+ * 4-bit weights with group scales,
+ *   W[n, k] = scale[n, k / group] * (code[n, k] - zero[n, k / group]),
+ * code and zero in 0..15 (zero = 8 without B200MOE_W4_ZEROS), group 32, 64 or
+ * 128.  b200moe_w4_pack lays `matrices` matrices [rows, k] out for the kernels
+ * below, once: tiles of 128 rows, blocks of 128 k, each block's codes, scales
+ * and zero points contiguous.  b200moe_w4_bytes is the size of the result
+ * (-1: no such layout).
+ *   codes  [matrices, rows, k] uint8, one code per byte (16-byte aligned)
+ *   scales [matrices, rows, k / group] bf16 or fp16 (B200MOE_W4_F16_SCALES)
+ *   zeros  [matrices, rows, k / group] uint8, with B200MOE_W4_ZEROS
+ */
+B200MOE_API int64_t b200moe_w4_bytes(int64_t matrices, int64_t rows, int64_t k, int group,
+                                     int flags);
+B200MOE_API int b200moe_w4_pack(const uint8_t *codes, const void *scales, const uint8_t *zeros,
+                                int64_t matrices, int64_t rows, int64_t k, int group, int flags,
+                                void *out, void *stream);
+
+/*
+ * Dense product out[m, n] = sum_k x[m, k] W[n, k], fp32 sums, bf16 out.
+ *   x [m, k] bf16, w one laid-out matrix [n, k], out [m, n] bf16; 16-byte aligned.
+ */
+B200MOE_API int b200moe_w4_linear(const void *x, int64_t m, int n, int k, const void *w, int group,
+                                  int flags, void *out, void *stream);
+
+/*
+ * The routed experts of one layer with 4-bit weights:
+ *   act[r] = silu(x_t G_e^T) * (x_t U_e^T) for every route r = (t, s), e = id[r],
+ *   out[t] = sum_s weight[t, s] * (act[t, s] D_e^T), in slot order,
+ * with fp32 sums and bf16 out.  Routes whose id is outside [0, num_experts)
+ * contribute nothing.
+ *   x [tokens, hidden] bf16, expert_ids [tokens, top_k] int64, weights
+ *   [tokens, top_k] bf16, w13 [num_experts] laid-out SwiGLU pairs [2 inter,
+ *   hidden] (B200MOE_W4_GATE_UP), w2 [num_experts] matrices [hidden, inter],
+ *   out [tokens, hidden] bf16; pointers 16-byte aligned.
+ *   workspace: b200moe_w4_experts_workspace bytes, 256-byte aligned.
+ */
+B200MOE_API int64_t b200moe_w4_experts_workspace(int64_t tokens, int hidden, int inter, int top_k,
+                                                 int num_experts);
+B200MOE_API int b200moe_w4_experts(const void *x, int64_t tokens, int hidden, int inter,
+                                   const int64_t *expert_ids, const void *weights, int top_k,
+                                   int num_experts, const void *w13, int group13, int flags13,
+                                   const void *w2, int group2, int flags2, void *workspace,
+                                   int64_t workspace_bytes, void *out, void *stream);
 
 #ifdef __cplusplus
 }
