@@ -1,5 +1,7 @@
 // C entry points of the products with 4-bit weights: argument checks, workspace
 // layout and the choice of kernel.
+#include <math.h>
+
 #include "w4.cuh"
 
 namespace b200moe {
@@ -10,8 +12,118 @@ int w4_route_experts(const void *x, int64_t tokens, int hidden, int inter, const
                      const w4::Shape &sh13, const void *w2, const w4::Shape &sh2, float *act,
                      void *out, cudaStream_t s);
 
+int w4_linear_tc(const void *x, int64_t m, int n, int k, const void *w, const w4::Shape &sh,
+                 void *out, cudaStream_t s);
+int w4_gate_up_tc(const RowSource &src, int hidden, int inter, const void *w13,
+                  const w4::Shape &sh, int64_t row_capacity, const int32_t *mtiles,
+                  int64_t max_mtiles, const int32_t *counters, double tiles, int64_t rows,
+                  void *act, cudaStream_t s);
+int w4_down_tc(const void *act, int hidden, int inter, const void *w2, const w4::Shape &sh,
+               const int32_t *row_route, const void *route_weights, int64_t num_routes,
+               int64_t row_capacity, const int32_t *mtiles, int64_t max_mtiles,
+               const int32_t *counters, double tiles, int64_t rows, float *y, cudaStream_t s);
+
 namespace {
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Rows up to which the dense product and routes up to which the experts run
+// on the CUDA cores.
+constexpr int64_t kGemvRows = 4;
+constexpr int64_t kGemvRoutes = 16;
+// Routes up to which the gate/up product gathers its rows in its own loads
+// instead of reading a packed copy.
+constexpr int64_t kGatherRoutes = 512;
+
+// Pieces of the workspace, each on a 256-byte boundary.
+struct Workspace {
+  int64_t bytes = 0;
+  char *base = nullptr;
+  template <typename T>
+  T *take(int64_t count) {
+    T *p = reinterpret_cast<T *>(base + bytes);
+    bytes += (count * static_cast<int64_t>(sizeof(T)) + 255) / 256 * 256;
+    return p;
+  }
+};
+
+struct ExpertBuffers {
+  int64_t row_capacity = 0, max_mtiles = 0, scratch_bytes = 0;
+  float *act_f32 = nullptr;  // CUDA-core path: [routes, inter]
+  int32_t *row_route = nullptr, *route_row = nullptr, *combine_rows = nullptr,
+          *tile_expert = nullptr, *offsets = nullptr, *counts = nullptr, *mtiles = nullptr,
+          *counters = nullptr, *scratch = nullptr;
+  __nv_bfloat16 *x_packed = nullptr;  // above kGatherRoutes routes
+  __nv_bfloat16 *act = nullptr;       // [row_capacity, inter], packed order
+  float *y = nullptr;                 // [routes, hidden], route order
+};
+
+ExpertBuffers expert_buffers(Workspace &ws, int64_t tokens, int hidden, int inter, int top_k,
+                             int num_experts) {
+  ExpertBuffers b;
+  const int64_t routes = tokens * top_k;
+  if (routes <= kGemvRoutes) {
+    b.act_f32 = ws.take<float>(routes * inter);
+    return b;
+  }
+  b.row_capacity = b200moe_pack_row_capacity(routes, num_experts);
+  b.max_mtiles = b200moe_pack_max_mtiles(routes, num_experts);
+  b.scratch_bytes = static_cast<int64_t>(b200moe_pack_scratch_bytes(routes, num_experts));
+  b.row_route = ws.take<int32_t>(b.row_capacity);
+  b.route_row = ws.take<int32_t>(routes);
+  b.combine_rows = ws.take<int32_t>(routes);
+  b.tile_expert = ws.take<int32_t>(b.row_capacity / B200MOE_BLOCK_ROWS);
+  b.offsets = ws.take<int32_t>(num_experts + 1);
+  b.counts = ws.take<int32_t>(num_experts);
+  b.mtiles = ws.take<int32_t>(b.max_mtiles * B200MOE_MTILE_WORDS);
+  b.counters = ws.take<int32_t>(B200MOE_NUM_COUNTERS);
+  b.scratch = ws.take<int32_t>(b.scratch_bytes / 4);
+  if (routes > kGatherRoutes) b.x_packed = ws.take<__nv_bfloat16>(b.row_capacity * hidden);
+  b.act = ws.take<__nv_bfloat16>(b.row_capacity * inter);
+  b.y = ws.take<float>(routes * hidden);
+  return b;
+}
+
+// out[t, :] = sum over slots, in slot order, of the fp32 route rows y (rows
+// that combine_rows does not name are not read).  One thread per 4 columns.
+__global__ void __launch_bounds__(256) w4_combine_kernel(const float *y, int64_t num_routes,
+                                                         const int32_t *combine_rows,
+                                                         int64_t tokens, int top_k, int hidden,
+                                                         __nv_bfloat16 *__restrict__ out) {
+  pdl_trigger();
+  pdl_wait();
+  const int vecs = hidden / 4;
+  const int64_t idx = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  const int64_t token = idx / vecs;
+  const int col = static_cast<int>(idx - token * vecs) * 4;
+  if (token >= tokens) return;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = 0; s0 < top_k; s0 += 4) {
+    // Four slots' row numbers, then their rows, are in flight together.
+    int64_t row[4];
+    float4 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      row[j] = s0 + j < top_k ? combine_rows[token * top_k + s0 + j] : num_routes;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (row[j] >= 0 && row[j] < num_routes)
+        v[j] = *reinterpret_cast<const float4 *>(y + row[j] * hidden + col);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (row[j] >= 0 && row[j] < num_routes) {
+        acc.x += v[j].x;
+        acc.y += v[j].y;
+        acc.z += v[j].z;
+        acc.w += v[j].w;
+      }
+  }
+  uint2 o;
+  __nv_bfloat162 *op = reinterpret_cast<__nv_bfloat162 *>(&o);
+  op[0] = __floats2bfloat162_rn(acc.x, acc.y);
+  op[1] = __floats2bfloat162_rn(acc.z, acc.w);
+  *reinterpret_cast<uint2 *>(out + token * hidden + col) = o;
+}
+
 }  // namespace
 }  // namespace b200moe
 
@@ -29,20 +141,17 @@ int b200moe_w4_linear(const void *x, int64_t m, int n, int k, const void *w, int
   B200_ARG(aligned16(x) && aligned16(w), "x and w must be 16-byte aligned");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const w4::Shape sh = w4::shape_of(group, flags);
-  constexpr int64_t kRows = 65535 * 4;
-  for (int64_t m0 = 0; m0 < m; m0 += kRows) {
-    const int rc = w4_linear_gemv(static_cast<const char *>(x) + m0 * k * 2,
-                                  min64(kRows, m - m0), n, k, w, sh,
-                                  static_cast<char *>(out) + m0 * n * 2, s);
-    if (rc) return rc;
-  }
-  return B200MOE_OK;
+  B200_UNSUPPORTED(m < (int64_t)0x7fffffff, "too many rows");
+  return m <= kGemvRows ? w4_linear_gemv(x, m, n, k, w, sh, out, s)
+                        : w4_linear_tc(x, m, n, k, w, sh, out, s);
 }
 
 int64_t b200moe_w4_experts_workspace(int64_t tokens, int hidden, int inter, int top_k,
                                      int num_experts) {
   if (tokens < 0 || hidden < 1 || inter < 1 || top_k < 1 || num_experts < 1) return -1;
-  return tokens * top_k * inter * 4;
+  b200moe::Workspace ws;
+  b200moe::expert_buffers(ws, tokens, hidden, inter, top_k, num_experts);
+  return ws.bytes;
 }
 
 int b200moe_w4_experts(const void *x, int64_t tokens, int hidden, int inter,
@@ -69,16 +178,47 @@ int b200moe_w4_experts(const void *x, int64_t tokens, int hidden, int inter,
   B200_ARG(workspace_bytes >= need, "workspace needs %lld bytes", (long long)need);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const w4::Shape sh13 = w4::shape_of(group13, flags13), sh2 = w4::shape_of(group2, flags2);
-  const int64_t most = 65535 / top_k;
-  B200_UNSUPPORTED(most >= 1, "top_k too large");
-  for (int64_t t = 0; t < tokens; t += most) {
-    const int rc = w4_route_experts(
-        static_cast<const char *>(x) + t * hidden * 2, min64(most, tokens - t), hidden, inter,
-        expert_ids + t * top_k, static_cast<const char *>(weights) + t * top_k * 2, top_k,
-        num_experts, w13, sh13, w2, sh2, static_cast<float *>(workspace) + t * top_k * inter,
-        static_cast<char *>(out) + t * hidden * 2, s);
+  const int64_t routes = tokens * top_k;
+  Workspace ws;
+  ws.base = static_cast<char *>(workspace);
+  const ExpertBuffers b = expert_buffers(ws, tokens, hidden, inter, top_k, num_experts);
+  if (routes <= kGemvRoutes)
+    return w4_route_experts(x, tokens, hidden, inter, expert_ids, weights, top_k, num_experts, w13,
+                            sh13, w2, sh2, b.act_f32, out, s);
+  // Without a capacity the packing call writes neither ids nor weights.
+  int rc = b200moe_pack_routes(const_cast<int64_t *>(expert_ids), nullptr, routes, num_experts,
+                               nullptr, 0, num_experts, nullptr, -1, b.row_capacity, b.row_route,
+                               b.route_row, b.combine_rows, b.tile_expert, b.offsets, b.counts,
+                               b.mtiles, b.max_mtiles, nullptr, b.counters, nullptr, b.scratch,
+                               static_cast<size_t>(b.scratch_bytes), stream);
+  if (rc) return rc;
+  RowSource src = {};
+  src.x = x;
+  src.x_rows = tokens;
+  src.x_packed = b.x_packed;
+  src.row_route = b.row_route;
+  src.top_k = top_k;
+  src.num_routes = routes;
+  if (b.x_packed) {
+    rc = b200moe_gather_rows(x, tokens, hidden, b.row_route, nullptr, top_k, routes,
+                             b.row_capacity, b.counters, b.x_packed, stream);
     if (rc) return rc;
   }
+  // Row tiles to expect when routes fall evenly, and rows of a full one.
+  const double mean = static_cast<double>(routes) / num_experts;
+  const double tiles = num_experts * (1.0 - exp(-mean)) + static_cast<double>(routes) / 128;
+  const int64_t rows = min64(tokens, static_cast<int64_t>(2.5 * mean) + 16);
+  rc = w4_gate_up_tc(src, hidden, inter, w13, sh13, b.row_capacity, b.mtiles, b.max_mtiles,
+                     b.counters, tiles, rows, b.act, s);
+  if (rc) return rc;
+  rc = w4_down_tc(b.act, hidden, inter, w2, sh2, b.row_route, weights, routes, b.row_capacity,
+                  b.mtiles, b.max_mtiles, b.counters, tiles, rows, b.y, s);
+  if (rc) return rc;
+  const int64_t threads = tokens * (hidden / 4);
+  B200_LAUNCH_PDL(kPdlCombine, w4_combine_kernel,
+                  dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, s, b.y, routes,
+                  b.combine_rows, tokens, top_k, hidden, static_cast<__nv_bfloat16 *>(out));
+  B200_LAUNCHED();
   return B200MOE_OK;
 }
 
