@@ -23,6 +23,8 @@
 // Every wait is bounded; on expiry the CTA records a status bit and leaves.
 #include <cudaTypedefs.h>
 
+#include <type_traits>
+
 #include "w4.cuh"
 
 namespace b200moe {
@@ -37,17 +39,19 @@ using w4::Shape;
 
 enum Kind { kLinear = 0, kGateUp = 1, kDown = 2 };
 
-constexpr int A_STAGES = 4;   // of 64 TMEM columns: 128 k in bf16 pairs
-constexpr int A_COL0 = 256;   // accumulators below, operand stages above
 constexpr int MAX_WS = 16;
 constexpr int SMEM_LIMIT = 226 * 1024;
 constexpr int TAIL_BYTES = 1024;  // barriers
 
 template <int NT>
 struct Cfg {
-  static constexpr int BS = NT == 128 ? 4 : NT == 64 ? 6 : 8;  // stages of x rows
-  static constexpr int B_BYTES = NT * 256;                     // 128 k of NT rows
-  static constexpr int ND = 256 / NT > 8 ? 8 : 256 / NT;       // accumulators
+  // TMEM: accumulators first, then operand stages of 64 columns (128 k in bf16
+  // pairs).  The operand stages and those of the x rows advance together, so
+  // one completion frees both.
+  static constexpr int D_COLS = NT == 128 ? 256 : 128;
+  static constexpr int ND = D_COLS / NT;             // accumulators
+  static constexpr int BS = (512 - D_COLS) / 64;     // operand stages
+  static constexpr int B_BYTES = NT * 256;           // 128 k of NT rows
   static constexpr int C = NT == 16 ? 8 : 16;                  // columns per chunk
   static constexpr int NCH = NT / C / 2;                       // chunks per promoting group
   // Decoding groups: one keeps up with 128-row tiles (512 cycles of matrix
@@ -167,27 +171,57 @@ __device__ __forceinline__ void arrive_cluster(uint32_t addr) {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
-__device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, volatile int *abort) {
-  const uint64_t start = global_timer_ns();
-  for (uint32_t spins = 0;; ++spins) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    if (ok) return true;
-    if ((spins & 63u) == 63u) {
+__device__ __forceinline__ bool try_wait_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// The rest of a wait that the first try did not satisfy.  No timer is read on
+// the way; gives up after about two seconds of cycles, or when another role did.
+template <bool kCluster>
+__device__ __forceinline__ bool wait_more(uint32_t bar, uint32_t parity, volatile int *abort) {
+  int64_t start = 0;
+  for (uint32_t tries = 1;; ++tries) {
+    if (kCluster ? try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)) return true;
+    if ((tries & 1023u) == 0) {
       if (*abort) return false;
-      if (global_timer_ns() - start > 2000000000ull) {
+      const int64_t now = clock64();
+      if (start == 0) {
+        start = now;
+      } else if (now - start > 4000000000ll) {
         *abort = 1;
         atomicOr(&g_status, kStatusTimeout);
         return false;
       }
     }
   }
+}
+
+// One try in line, the loop out of the way: a taken branch costs a lone warp
+// about 70-140 cycles here (measured), as much as a whole step of a role.
+template <bool kCluster = false>
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int *abort) {
+  const bool now = kCluster ? try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity);
+  if (__builtin_expect(now, 1)) return true;
+  return wait_more<kCluster>(bar, parity, abort);
+}
+
+// One lane of the warp, in a form that tells the compiler so: matrix
+// instructions issued under it take uniform registers (37 cycles each at
+// N = 16); under a test of the lane number they took 128.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(p));
+  return p != 0;
 }
 
 // x * sigmoid(x); the fast exp and division are good to a few units in 2^-23,
@@ -198,68 +232,434 @@ __device__ __forceinline__ float silu_fast(float x) { return __fdividef(x, 1.0f 
 struct Ring {
   int stage = 0;
   uint32_t phase = 0;
-  __device__ __forceinline__ void next(int n) {
-    if (++stage == n) {
-      stage = 0;
-      phase ^= 1;
-    }
+  __device__ __forceinline__ void next(int n, int by = 1) {
+    stage += by;
+    const bool wrap = stage >= n;
+    stage -= wrap ? n : 0;
+    phase ^= wrap ? 1u : 0u;
   }
 };
 
+// What every role of a CTA knows (shared-memory addresses, this CTA's share).
+struct Ctx {
+  uint32_t s_b, s_w, s_red;
+  uint32_t w_full, w_empty, b_full, a_full, ab_empty, d_full, d_empty, red_full, red_empty;
+  uint32_t tmem;
+  volatile int *abort;
+  int wbytes, scale_off, zero_off;
+  int items, first, step, kb0, kb1;
+  int rank, split;
+};
+
+// Codes: one bulk copy per block of 128 k.  One lane.
 template <int NT>
+__device__ __forceinline__ void load_codes(const Args &args, const Ctx &c) {
+  Ring w;
+  for (int it = c.first; it < c.items; it += c.step) {
+    const Tile t = tile_of<NT>(args, it / args.n_blocks);
+    const uint8_t *src = args.w + (static_cast<int64_t>(t.e) * args.n_blocks + it % args.n_blocks) *
+                                      args.num_kb * c.wbytes;
+    for (int r0 = 0; r0 < t.rows; r0 += NT)
+      for (int kb = c.kb0; kb < c.kb1; ++kb) {
+        if (!wait(c.w_empty + 8 * w.stage, w.phase ^ 1, c.abort)) return;
+        const uint32_t bar = c.w_full + 8 * w.stage;
+        mbar_arrive_expect_tx(bar, c.wbytes);
+        bulk_load(c.s_w + w.stage * c.wbytes, src + static_cast<int64_t>(kb) * c.wbytes, c.wbytes,
+                  bar);
+        w.next(args.ws);
+      }
+  }
+}
+
+// Rows of x.  Dense rows and full tiles come as one box of NT rows per 64 k,
+// the rows of other tiles as boxes of 16 (lane b loads the b-th), gathered
+// rows four at a time (lane l loads the l-th four).  A whole warp.
+template <int NT>
+__device__ __forceinline__ void load_rows(const Args &args, const Ctx &c, const CUtensorMap *tm,
+                                          const CUtensorMap *tm_whole) {
+  using C = Cfg<NT>;
+  const int lane = threadIdx.x & 31;
+  const bool gather = args.gather != 0;
+  Ring b;
+  for (int it = c.first; it < c.items; it += c.step) {
+    const Tile t = tile_of<NT>(args, it / args.n_blocks);
+    for (int r0 = 0; r0 < t.rows; r0 += NT) {
+      const int rows = min(NT, t.rows - r0);
+      const int nbox = (rows + 15) >> 4;
+      const bool whole = !gather && (nbox * 16 == NT || args.kind == kLinear);
+      const bool mine = !whole && lane < (gather ? nbox * 4 : nbox);
+      const uint32_t bytes = whole ? C::B_BYTES : nbox * 16 * 256;
+      int tok[4] = {0, 0, 0, 0};
+      if (gather && mine) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          tok[j] = gather_token(t.rb + r0 + 4 * lane + j, t.rb + t.rows, args.row_route, nullptr,
+                                args.top_k, args.num_routes, args.x_rows);
+      }
+      for (int kb = c.kb0; kb < c.kb1; ++kb) {
+        if (!wait(c.ab_empty + 8 * b.stage, b.phase ^ 1, c.abort)) return;
+        const uint32_t bar = c.b_full + 8 * b.stage;
+        const uint32_t dst = c.s_b + b.stage * C::B_BYTES;
+        const int c0 = kb * w4::kBlockK;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(bar, bytes);
+          if (whole) {
+            tma_load_2d(dst, tm_whole, bar, c0, t.rb + r0);
+            tma_load_2d(dst + NT * 128, tm_whole, bar, c0 + 64, t.rb + r0);
+          }
+        }
+        __syncwarp();
+        if (mine) {
+          if (gather) {
+            tma_gather4(dst + lane * 512, tm, bar, c0, tok[0], tok[1], tok[2], tok[3]);
+            tma_gather4(dst + NT * 128 + lane * 512, tm, bar, c0 + 64, tok[0], tok[1], tok[2],
+                        tok[3]);
+          } else {
+            tma_load_2d(dst + lane * 2048, tm, bar, c0, t.rb + r0 + lane * 16);
+            tma_load_2d(dst + NT * 128 + lane * 2048, tm, bar, c0 + 64, t.rb + r0 + lane * 16);
+          }
+        }
+        __syncwarp();
+        b.next(C::BS);
+      }
+    }
+  }
+}
+
+// Matrix instructions.  One lane.
+template <int NT, int GPB>
+__device__ __forceinline__ void issue_mma(const Args &args, const Ctx &c) {
+  using C = Cfg<NT>;
+  constexpr int KK = 8 / GPB;  // instructions of 16 k per group
+  Ring b, d;
+  // Descriptor of stage 0; the start address field counts 16 bytes.
+  const uint64_t desc0 = sw128_kmajor_desc(c.s_b);
+  for (int it = c.first; it < c.items; it += c.step) {
+    const Tile t = tile_of<NT>(args, it / args.n_blocks);
+    for (int r0 = 0; r0 < t.rows; r0 += NT) {
+      const int n_mma = (min(NT, t.rows - r0) + 15) & ~15;
+      const uint32_t idesc = idesc_bf16_f32(128, n_mma);
+      for (int kb = c.kb0; kb < c.kb1; ++kb) {
+        // Tried together: each alone costs its latency.
+        const bool b_ready = mbar_try_wait(c.b_full + 8 * b.stage, b.phase);
+        const bool a_ready = mbar_try_wait(c.a_full + 8 * b.stage, b.phase);
+        if (__builtin_expect(!(b_ready && a_ready), 0)) {
+          if (!wait_more<false>(c.b_full + 8 * b.stage, b.phase, c.abort)) return;
+          if (!wait_more<false>(c.a_full + 8 * b.stage, b.phase, c.abort)) return;
+        }
+        const uint64_t desc = desc0 + static_cast<uint32_t>(b.stage * (C::B_BYTES >> 4));
+        const uint32_t ta = c.tmem + C::D_COLS + b.stage * 64;
+#pragma unroll
+        for (int g = 0; g < GPB; ++g) {
+          if (!wait(c.d_empty + 8 * d.stage, d.phase ^ 1, c.abort)) return;
+          tc_fence_after();
+          const uint32_t td = c.tmem + d.stage * NT;
+#pragma unroll
+          for (int j = 0; j < KK; ++j) {
+            const int kk = g * KK + j;
+            mma_ts(td, ta + kk * 8, desc + ((kk >> 2) * (NT * 8) + (kk & 3) * 2), idesc, j != 0);
+          }
+          tc_commit(c.d_full + 8 * d.stage);
+          d.next(C::ND);
+        }
+        tc_commit(c.ab_empty + 8 * b.stage);
+        b.next(C::BS);
+      }
+    }
+  }
+}
+
+// Decoding: the codes of a block -> q - z as bf16 in the operand stage.  Group
+// `grp` of DG takes every DG-th block.  Four warps, one weight row per thread.
+template <int NT, int GPB>
+__device__ __forceinline__ void decode(const Args &args, const Ctx &c, int grp, int q) {
+  using C = Cfg<NT>;
+  const int lane = threadIdx.x & 31;
+  const int row = q * 32 + lane;
+  const bool zeros = args.sh.has_zero != 0;
+  const uint32_t tq = c.tmem + C::D_COLS + (static_cast<uint32_t>(q * 32) << 16);
+  Ring w, a;
+  w.next(args.ws, grp);
+  a.next(C::BS, grp);
+  int skip = grp;  // blocks until this group's next one
+  for (int it = c.first; it < c.items; it += c.step) {
+    const Tile t = tile_of<NT>(args, it / args.n_blocks);
+    for (int r0 = 0; r0 < t.rows; r0 += NT) {
+      int kb = c.kb0 + skip;
+      for (; kb < c.kb1; kb += C::DG) {
+        if (!wait(c.w_full + 8 * w.stage, w.phase, c.abort)) return;
+        const uint32_t st = c.s_w + w.stage * c.wbytes;
+        uint32_t code[16];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(code[4 * i]), "=r"(code[4 * i + 1]), "=r"(code[4 * i + 2]),
+                         "=r"(code[4 * i + 3])
+                       : "r"(st + i * 2048 + row * 16));
+        uint32_t zp[GPB];
+#pragma unroll
+        for (int g = 0; g < GPB; ++g) {
+          uint32_t z = 8;
+          if (zeros)
+            asm volatile("ld.shared.u8 %0, [%1];" : "=r"(z) : "r"(st + c.zero_off + g * 128 + row));
+          zp[g] = w4::zero_pair(z);
+        }
+        if (!wait(c.ab_empty + 8 * a.stage, a.phase ^ 1, c.abort)) return;
+        tc_fence_after();
+        const uint32_t ta = tq + a.stage * 64;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t r[32];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            uint32_t o[4];
+            w4::decode8(code[8 * h + j], zp[(8 * h + j) * GPB / 16], o);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[4 * j + i] = o[i];
+          }
+          tmem_st32(ta + h * 32, r);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(c.a_full + 8 * a.stage);
+          mbar_arrive(c.w_empty + 8 * w.stage);
+        }
+        w.next(args.ws, C::DG);
+        a.next(C::BS, C::DG);
+      }
+      skip = kb - c.kb1;
+    }
+  }
+}
+
+// Promoting and epilogue.  Two groups of four warps (alternate column chunks),
+// one weight row per thread.
+template <int NT, int GPB>
+__device__ __forceinline__ void promote(const Args &args, const Ctx &c, int half, int q) {
+  using C = Cfg<NT>;
+  const int lane = threadIdx.x & 31;
+  const int row = q * 32 + lane;
+  const uint32_t tq = c.tmem + (static_cast<uint32_t>(q * 32) << 16);
+  Ring w, d;
+  uint32_t red_phase = 0;
+  for (int it = c.first; it < c.items; it += c.step) {
+    const Tile t = tile_of<NT>(args, it / args.n_blocks);
+    const int fb = it % args.n_blocks;
+    for (int r0 = 0; r0 < t.rows; r0 += NT) {
+      const int rows = min(NT, t.rows - r0);
+      const int n_mma = (rows + 15) & ~15;
+      float acc[C::NCH][C::C];
+#pragma unroll
+      for (int i = 0; i < C::NCH; ++i)
+#pragma unroll
+        for (int j = 0; j < C::C; ++j) acc[i][j] = 0.f;
+      for (int kb = c.kb0; kb < c.kb1; ++kb) {
+        const uint32_t scales = c.s_w + w.stage * c.wbytes + c.scale_off + row * 2;
+#pragma unroll
+        for (int g = 0; g < GPB; ++g) {
+          // A finished product implies the codes and scales of its stage: the
+          // decoding warps waited for the copy before they signalled it.
+          if (!wait(c.d_full + 8 * d.stage, d.phase, c.abort)) return;
+          tc_fence_after();
+          uint16_t bits;
+          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(bits) : "r"(scales + g * 256));
+          const float s = w4::scale_f32(bits, args.sh.half_scale);
+          const uint32_t td = tq + d.stage * NT;
+#pragma unroll
+          for (int i = 0; i < C::NCH; i += 2) {
+            float v0[C::C], v1[C::C];
+            constexpr bool pair = C::NCH > 1;
+            const int c0 = (2 * i + half) * C::C;
+            // Columns beyond n_mma hold old sums; they are never stored.
+            if (C::NCH <= 2 || c0 < n_mma) {
+              tmem_ld(td + c0, v0);
+              if (pair) tmem_ld(td + c0 + 2 * C::C, v1);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < C::C; ++j) acc[i][j] = fmaf(s, v0[j], acc[i][j]);
+              if constexpr (pair) {
+#pragma unroll
+                for (int j = 0; j < C::C; ++j) acc[i + 1][j] = fmaf(s, v1[j], acc[i + 1][j]);
+              }
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(c.d_empty + 8 * d.stage);
+          d.next(C::ND);
+        }
+        if (lane == 0) mbar_arrive(c.w_empty + 8 * w.stage);
+        w.next(args.ws);
+      }
+      if (c.split > 1) {
+        if (c.rank != 0) {
+          // This CTA's sums into the first one's shared memory.
+          if (!wait<true>(c.red_empty, red_phase ^ 1, c.abort)) return;
+          const uint32_t dst = map_rank(c.s_red + ((c.rank - 1) * NT * 128 + row) * 4, 0);
+#pragma unroll
+          for (int i = 0; i < C::NCH; ++i) {
+            const int col = (2 * i + half) * C::C;
+            if (col < n_mma) {
+#pragma unroll
+              for (int j = 0; j < C::C; ++j) st_cluster(dst + (col + j) * 512, acc[i][j]);
+            }
+          }
+          __syncwarp();
+          if (lane == 0) arrive_cluster(map_rank(c.red_full, 0));
+          red_phase ^= 1;
+          continue;
+        }
+        if (!wait<true>(c.red_full, red_phase, c.abort)) return;
+        red_phase ^= 1;
+        for (int p = 0; p < c.split - 1; ++p) {
+#pragma unroll
+          for (int i = 0; i < C::NCH; ++i) {
+            const int col = (2 * i + half) * C::C;
+            if (col < n_mma) {
+#pragma unroll
+              for (int j = 0; j < C::C; ++j) {
+                float v;
+                asm volatile("ld.shared.f32 %0, [%1];"
+                             : "=f"(v)
+                             : "r"(c.s_red + ((p * NT + col + j) * 128 + row) * 4));
+                acc[i][j] += v;
+              }
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0)
+          for (int p = 1; p < c.split; ++p) arrive_cluster(map_rank(c.red_empty, p));
+      }
+      const int64_t row0 = static_cast<int64_t>(t.rb) + r0;
+      if (args.kind == kGateUp) {
+        // Lanes 0-15 hold gate rows, 16-31 the up rows of the same features:
+        // of each pair of columns the lower half finishes the first, the upper
+        // half the second.
+        auto *out = static_cast<__nv_bfloat16 *>(args.out);
+        const int f = fb * 64 + q * 16 + (lane & 15);
+        const bool up = lane >= 16;
+#pragma unroll
+        for (int i = 0; i < C::NCH; ++i) {
+          const int col = (2 * i + half) * C::C;
+          if (col < n_mma) {
+#pragma unroll
+            for (int j = 0; j < C::C; j += 2) {
+              const float other =
+                  __shfl_xor_sync(0xffffffffu, up ? acc[i][j] : acc[i][j + 1], 16);
+              const float gv = up ? other : acc[i][j];
+              const float uv = up ? acc[i][j + 1] : other;
+              const int n = col + j + (up ? 1 : 0);
+              if (f < args.n_out && n < rows)
+                out[(row0 + n) * args.n_out + f] = __float2bfloat16_rn(silu_fast(gv) * uv);
+            }
+          }
+        }
+      } else {
+        const int f = fb * 128 + row;
+#pragma unroll
+        for (int i = 0; i < C::NCH; ++i) {
+          const int col = (2 * i + half) * C::C;
+          if (col < n_mma) {
+            // Lane j knows the route and the weight of column col + j.
+            int32_t route = -1;
+            float weight = 0.f;
+            if (args.kind == kDown && lane < C::C && col + lane < rows) {
+              route = args.row_route[row0 + col + lane];
+              if (route < 0 || route >= args.num_routes) {
+                atomicOr(&g_status, kStatusIndex);
+                route = -1;
+              } else {
+                weight = __bfloat162float(args.route_w[route]);
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < C::C; ++j) {
+              const int n = col + j;
+              const int32_t r = __shfl_sync(0xffffffffu, route, j);
+              const float wgt = __shfl_sync(0xffffffffu, weight, j);
+              if (f < args.n_out && n < rows) {
+                if (args.kind == kDown) {
+                  if (r >= 0)
+                    static_cast<float *>(args.out)[static_cast<int64_t>(r) * args.n_out + f] =
+                        acc[i][j] * wgt;
+                } else {
+                  static_cast<__nv_bfloat16 *>(args.out)[(row0 + n) * args.n_out + f] =
+                      __float2bfloat16_rn(acc[i][j]);
+                }
+              }
+            }
+          }
+        }
+      }
+    }
+  }
+}
+
+// NT: rows of x per tile; GPB: groups per block of 128 k.
+template <int NT, int GPB>
 __global__ void __launch_bounds__(Cfg<NT>::THREADS, 1)
-    w4_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ Args args) {
+    w4_gemm_kernel(const __grid_constant__ CUtensorMap tmX,
+                   const __grid_constant__ CUtensorMap tmWhole, const __grid_constant__ Args args) {
   using C = Cfg<NT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                               ~static_cast<uintptr_t>(1023));
-  const int wbytes = args.sh.block_bytes();
-  uint8_t *s_b = smem;
-  uint8_t *s_w = smem + C::BS * C::B_BYTES;
-  float *s_red = reinterpret_cast<float *>(s_w + args.ws * wbytes);  // [split - 1][NT][128]
-  uint64_t *bars = reinterpret_cast<uint64_t *>(s_red + (args.split - 1) * NT * 128);
-  uint64_t *w_full = bars;
-  uint64_t *w_empty = w_full + MAX_WS;
-  uint64_t *b_full = w_empty + MAX_WS;
-  uint64_t *b_empty = b_full + C::BS;
-  uint64_t *a_full = b_empty + C::BS;
-  uint64_t *a_empty = a_full + A_STAGES;
-  uint64_t *d_full = a_empty + A_STAGES;
-  uint64_t *d_empty = d_full + C::ND;
-  uint64_t *red_full = d_empty + C::ND;
-  uint64_t *red_empty = red_full + 1;
-  uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(red_empty + 1);
-  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_holder + 1);
-
-  const int warp = threadIdx.x >> 5;
-  const int lane = threadIdx.x & 31;
   const int split = args.split;
-  const int rank = split > 1 ? static_cast<int>(cluster_rank()) : 0;
+  Ctx c;
+  c.wbytes = args.sh.block_bytes();
+  c.scale_off = args.sh.scale_off();
+  c.zero_off = args.sh.zero_off();
+  uint8_t *s_w = smem + C::BS * C::B_BYTES;
+  uint8_t *s_red = s_w + args.ws * c.wbytes;  // [split - 1][NT][128] fp32
+  uint64_t *bars = reinterpret_cast<uint64_t *>(s_red + (split - 1) * NT * 512);
+  c.s_b = smem_u32(smem);
+  c.s_w = smem_u32(s_w);
+  c.s_red = smem_u32(s_red);
+  c.w_full = smem_u32(bars);
+  c.w_empty = c.w_full + 8 * MAX_WS;
+  c.b_full = c.w_empty + 8 * MAX_WS;
+  c.a_full = c.b_full + 8 * C::BS;
+  c.ab_empty = c.a_full + 8 * C::BS;
+  c.d_full = c.ab_empty + 8 * C::BS;
+  c.d_empty = c.d_full + 8 * C::ND;
+  c.red_full = c.d_empty + 8 * C::ND;
+  c.red_empty = c.red_full + 8;
+  uint32_t *tmem_holder =
+      reinterpret_cast<uint32_t *>(bars + 2 * MAX_WS + 3 * C::BS + 2 * C::ND + 2);
+  c.abort = reinterpret_cast<volatile int *>(tmem_holder + 1);
+
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31;
+  c.split = split;
+  c.rank = split > 1 ? static_cast<int>(cluster_rank()) : 0;
   pdl_trigger();
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < args.ws; ++s) {
-      mbar_init(smem_u32(&w_full[s]), 1);
-      mbar_init(smem_u32(&w_empty[s]), 12);  // four decoding and eight promoting warps
+      mbar_init(c.w_full + 8 * s, 1);
+      mbar_init(c.w_empty + 8 * s, 12);  // four decoding and eight promoting warps
     }
     for (int s = 0; s < C::BS; ++s) {
-      mbar_init(smem_u32(&b_full[s]), 1);
-      mbar_init(smem_u32(&b_empty[s]), 1);
-    }
-    for (int s = 0; s < A_STAGES; ++s) {
-      mbar_init(smem_u32(&a_full[s]), 4);
-      mbar_init(smem_u32(&a_empty[s]), 1);
+      mbar_init(c.b_full + 8 * s, 1);
+      mbar_init(c.a_full + 8 * s, 4);
+      mbar_init(c.ab_empty + 8 * s, 1);
     }
     for (int s = 0; s < C::ND; ++s) {
-      mbar_init(smem_u32(&d_full[s]), 1);
-      mbar_init(smem_u32(&d_empty[s]), 8);
+      mbar_init(c.d_full + 8 * s, 1);
+      mbar_init(c.d_empty + 8 * s, 8);
     }
-    mbar_init(smem_u32(red_full), 8 * (split > 1 ? split - 1 : 1));
-    mbar_init(smem_u32(red_empty), 8);
-    *abort_flag = 0;
+    mbar_init(c.red_full, 8 * (split > 1 ? split - 1 : 1));
+    mbar_init(c.red_empty, 8);
+    *c.abort = 0;
     fence_mbar_init();
   }
-  if (warp == 1 && lane == 0) prefetch_tmap(&tmX);
+  if (warp == 1 && lane == 0) {
+    prefetch_tmap(&tmX);
+    prefetch_tmap(&tmWhole);
+  }
   if (warp == 3) {
     tmem_alloc(smem_u32(tmem_holder), 512);
     tmem_relinquish();
@@ -268,365 +668,34 @@ __global__ void __launch_bounds__(Cfg<NT>::THREADS, 1)
   __syncthreads();
   tc_fence_after();
   if (split > 1) cluster_sync();  // the peers' barriers are ready
-  const uint32_t tmem = *tmem_holder;
+  c.tmem = *tmem_holder;
   // Codes are constant; a dense call's items are known too, so its first
   // blocks are fetched while the previous kernel still runs.
   if (!(args.kind == kLinear && warp == 0)) pdl_wait();
   const int mt = args.kind == kLinear
                      ? static_cast<int>((args.m + NT - 1) / NT)
                      : static_cast<int>(min64(args.counters[B200MOE_CNT_MTILES], args.max_mtiles));
-  const int items = mt * args.n_blocks;
-  const int first = blockIdx.x / split;
-  const int step = gridDim.x / split;
-  const int kb0 = rank * args.num_kb / split;
-  const int kb1 = (rank + 1) * args.num_kb / split;
-  const int gpb = args.sh.groups_per_block();
+  c.items = mt * args.n_blocks;
+  c.first = blockIdx.x / split;
+  c.step = gridDim.x / split;
+  c.kb0 = c.rank * args.num_kb / split;
+  c.kb1 = (c.rank + 1) * args.num_kb / split;
 
-  if (warp < 4) {
-    if (warp == 0) {
-      // ---------------- codes ----------------
-      if (lane == 0) {
-        Ring w;
-        bool ok = true;
-        for (int it = first; it < items && ok; it += step) {
-          const Tile t = tile_of<NT>(args, it / args.n_blocks);
-          const uint8_t *src = args.w + (static_cast<int64_t>(t.e) * args.n_blocks +
-                                         it % args.n_blocks) * args.num_kb * wbytes;
-          for (int r0 = 0; r0 < t.rows && ok; r0 += NT)
-            for (int kb = kb0; kb < kb1; ++kb) {
-              if (!mbar_wait_bounded(smem_u32(&w_empty[w.stage]), w.phase ^ 1, abort_flag)) {
-                ok = false;
-                break;
-              }
-              const uint32_t bar = smem_u32(&w_full[w.stage]);
-              mbar_arrive_expect_tx(bar, wbytes);
-              bulk_load(smem_u32(s_w + w.stage * wbytes), src + static_cast<int64_t>(kb) * wbytes,
-                        wbytes, bar);
-              w.next(args.ws);
-            }
-        }
-      }
-    } else if (warp == 1) {
-      // ---------------- rows of x ----------------
-      // Lane b loads the b-th 16 rows (or, gathering, the b-th four rows).
-      const bool gather = args.gather != 0;
-      Ring b;
-      bool ok = true;
-      for (int it = first; it < items && ok; it += step) {
-        const Tile t = tile_of<NT>(args, it / args.n_blocks);
-        for (int r0 = 0; r0 < t.rows && ok; r0 += NT) {
-          const int rows = min(NT, t.rows - r0);
-          const int nbox = (rows + 15) >> 4;
-          const bool mine = lane < (gather ? nbox * 4 : nbox);
-          int tok[4] = {0, 0, 0, 0};
-          if (gather && mine) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              tok[j] = gather_token(t.rb + r0 + 4 * lane + j, t.rb + t.rows, args.row_route,
-                                    nullptr, args.top_k, args.num_routes, args.x_rows);
-          }
-          for (int kb = kb0; kb < kb1; ++kb) {
-            bool got = true;
-            if (lane == 0)
-              got = mbar_wait_bounded(smem_u32(&b_empty[b.stage]), b.phase ^ 1, abort_flag);
-            if (!__shfl_sync(0xffffffffu, got ? 1 : 0, 0)) {
-              ok = false;
-              break;
-            }
-            const uint32_t bar = smem_u32(&b_full[b.stage]);
-            const uint32_t dst = smem_u32(s_b + b.stage * C::B_BYTES);
-            if (lane == 0) mbar_arrive_expect_tx(bar, nbox * 16 * 256);
-            __syncwarp();
-            if (mine) {
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const uint32_t half = dst + h * NT * 128;
-                const int c0 = kb * w4::kBlockK + h * 64;
-                if (gather)
-                  tma_gather4(half + lane * 512, &tmX, bar, c0, tok[0], tok[1], tok[2], tok[3]);
-                else
-                  tma_load_2d(half + lane * 2048, &tmX, bar, c0, t.rb + r0 + lane * 16);
-              }
-            }
-            b.next(C::BS);
-          }
-        }
-      }
-    } else if (warp == 2) {
-      // ---------------- matrix instructions ----------------
-      if (lane == 0) {
-        Ring b, a, d;
-        bool ok = true;
-        const int kk_per_group = args.sh.group / 16;
-        for (int it = first; it < items && ok; it += step) {
-          const Tile t = tile_of<NT>(args, it / args.n_blocks);
-          for (int r0 = 0; r0 < t.rows && ok; r0 += NT) {
-            const int n_mma = (min(NT, t.rows - r0) + 15) & ~15;
-            const uint32_t idesc = idesc_bf16_f32(128, n_mma);
-            for (int kb = kb0; kb < kb1 && ok; ++kb) {
-              ok = mbar_wait_bounded(smem_u32(&b_full[b.stage]), b.phase, abort_flag) &&
-                   mbar_wait_bounded(smem_u32(&a_full[a.stage]), a.phase, abort_flag);
-              if (!ok) break;
-              const uint32_t sb = smem_u32(s_b + b.stage * C::B_BYTES);
-              const uint32_t ta = tmem + A_COL0 + a.stage * 64;
-              int kk = 0;
-              for (int g = 0; g < gpb; ++g) {
-                if (!mbar_wait_bounded(smem_u32(&d_empty[d.stage]), d.phase ^ 1, abort_flag)) {
-                  ok = false;
-                  break;
-                }
-                tc_fence_after();
-                const uint32_t td = tmem + d.stage * NT;
-                for (int j = 0; j < kk_per_group; ++j, ++kk)
-                  mma_ts(td, ta + kk * 8,
-                         sw128_kmajor_desc(sb + (kk >> 2) * NT * 128 + (kk & 3) * 32), idesc,
-                         j != 0);
-                tc_commit(smem_u32(&d_full[d.stage]));
-                d.next(C::ND);
-              }
-              if (!ok) break;
-              tc_commit(smem_u32(&a_empty[a.stage]));
-              tc_commit(smem_u32(&b_empty[b.stage]));
-              a.next(A_STAGES);
-              b.next(C::BS);
-            }
-          }
-        }
-      }
-    }
-  } else if (warp < C::PROMOTE0) {
-    // ---------------- decoding: codes -> q - z in TMEM ----------------
-    const int q = warp & 3;
-    const int row = q * 32 + lane;
-    const int grp = (warp - 4) >> 2;
-    const int gshift = args.sh.group == 32 ? 0 : args.sh.group == 64 ? 1 : 2;
-    Ring w, a;
-    int turn = 0;
-    bool ok = true;
-    for (int it = first; it < items && ok; it += step) {
-      const Tile t = tile_of<NT>(args, it / args.n_blocks);
-      for (int r0 = 0; r0 < t.rows && ok; r0 += NT)
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (turn == grp) {
-            if (!mbar_wait_bounded(smem_u32(&w_full[w.stage]), w.phase, abort_flag)) {
-              ok = false;
-              break;
-            }
-            const uint8_t *st = s_w + w.stage * wbytes;
-            uint4 codes[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              codes[c] = *reinterpret_cast<const uint4 *>(st + c * 2048 + row * 16);
-            uint32_t zp[4] = {0x43084308u, 0x43084308u, 0x43084308u, 0x43084308u};
-            if (args.sh.has_zero) {
-#pragma unroll
-              for (int c = 0; c < 4; ++c)
-                zp[c] = w4::zero_pair(st[args.sh.zero_off() + (c >> gshift) * 128 + row]);
-            }
-            if (!mbar_wait_bounded(smem_u32(&a_empty[a.stage]), a.phase ^ 1, abort_flag)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-            const uint32_t ta =
-                tmem + A_COL0 + a.stage * 64 + (static_cast<uint32_t>(q * 32) << 16);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t r[32];
-#pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                const uint4 v = codes[2 * h + c];
-                const uint32_t word[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  uint32_t o[4];
-                  w4::decode8(word[j], zp[2 * h + c], o);
-#pragma unroll
-                  for (int i = 0; i < 4; ++i) r[c * 16 + j * 4 + i] = o[i];
-                }
-              }
-              tmem_st32(ta + h * 32, r);
-            }
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-              mbar_arrive(smem_u32(&a_full[a.stage]));
-              mbar_arrive(smem_u32(&w_empty[w.stage]));
-            }
-          }
-          if (++turn == C::DG) turn = 0;
-          w.next(args.ws);
-          a.next(A_STAGES);
-        }
-    }
-  } else {
-    // ---------------- promoting and epilogue ----------------
-    const int q = warp & 3;
-    const int row = q * 32 + lane;
-    const int half = (warp - C::PROMOTE0) >> 2;
-    const uint32_t tq = tmem + (static_cast<uint32_t>(q * 32) << 16);
-    Ring w, d;
-    uint32_t red_phase = 0;
-    bool ok = true;
-    for (int it = first; it < items && ok; it += step) {
-      const Tile t = tile_of<NT>(args, it / args.n_blocks);
-      const int fb = it % args.n_blocks;
-      for (int r0 = 0; r0 < t.rows && ok; r0 += NT) {
-        const int rows = min(NT, t.rows - r0);
-        const int n_mma = (rows + 15) & ~15;
-        float acc[C::NCH][C::C];
-#pragma unroll
-        for (int i = 0; i < C::NCH; ++i)
-#pragma unroll
-          for (int j = 0; j < C::C; ++j) acc[i][j] = 0.f;
-        for (int kb = kb0; kb < kb1 && ok; ++kb) {
-          // The copy that wrote this stage is long complete (the decoding
-          // warps waited for it); this wait makes its writes visible here.
-          ok = mbar_wait_bounded(smem_u32(&w_full[w.stage]), w.phase, abort_flag);
-          if (!ok) break;
-          const uint16_t *scales = reinterpret_cast<const uint16_t *>(
-              s_w + w.stage * wbytes + args.sh.scale_off());
-          for (int g = 0; g < gpb; ++g) {
-            const float s = w4::scale_f32(scales[g * 128 + row], args.sh.half_scale);
-            ok = mbar_wait_bounded(smem_u32(&d_full[d.stage]), d.phase, abort_flag);
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t td = tq + d.stage * NT;
-#pragma unroll
-            for (int i = 0; i < C::NCH; i += 2) {
-              float v0[C::C], v1[C::C];
-              const int c0 = (2 * i + half) * C::C;
-              const int c1 = c0 + 2 * C::C;
-              if (c0 < n_mma) {
-                tmem_ld(td + c0, v0);
-                if (i + 1 < C::NCH && c1 < n_mma) tmem_ld(td + c1, v1);
-                tmem_ld_wait();
-#pragma unroll
-                for (int j = 0; j < C::C; ++j) acc[i][j] = fmaf(s, v0[j], acc[i][j]);
-                if (i + 1 < C::NCH && c1 < n_mma) {
-#pragma unroll
-                  for (int j = 0; j < C::C; ++j)
-                    acc[i + 1 < C::NCH ? i + 1 : i][j] =
-                        fmaf(s, v1[j], acc[i + 1 < C::NCH ? i + 1 : i][j]);
-                }
-              }
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&d_empty[d.stage]));
-            d.next(C::ND);
-          }
-          if (!ok) break;
-          if (lane == 0) mbar_arrive(smem_u32(&w_empty[w.stage]));
-          w.next(args.ws);
-        }
-        if (!ok) break;
-        if (split > 1) {
-          if (rank != 0) {
-            // This CTA's sums into the first one's shared memory.
-            ok = wait_cluster(smem_u32(red_empty), red_phase ^ 1, abort_flag);
-            if (!ok) break;
-            const uint32_t dst =
-                map_rank(smem_u32(s_red + (rank - 1) * NT * 128 + row), 0);
-#pragma unroll
-            for (int i = 0; i < C::NCH; ++i) {
-              const int c = (2 * i + half) * C::C;
-              if (c < n_mma) {
-#pragma unroll
-                for (int j = 0; j < C::C; ++j) st_cluster(dst + (c + j) * 512, acc[i][j]);
-              }
-            }
-            __syncwarp();
-            if (lane == 0) arrive_cluster(map_rank(smem_u32(red_full), 0));
-            red_phase ^= 1;
-            continue;
-          }
-          ok = wait_cluster(smem_u32(red_full), red_phase, abort_flag);
-          if (!ok) break;
-          red_phase ^= 1;
-          for (int p = 0; p < split - 1; ++p) {
-#pragma unroll
-            for (int i = 0; i < C::NCH; ++i) {
-              const int c = (2 * i + half) * C::C;
-              if (c < n_mma) {
-#pragma unroll
-                for (int j = 0; j < C::C; ++j) acc[i][j] += s_red[(p * NT + c + j) * 128 + row];
-              }
-            }
-          }
-          __syncwarp();
-          if (lane == 0)
-            for (int p = 1; p < split; ++p) arrive_cluster(map_rank(smem_u32(red_empty), p));
-        }
-        const int64_t row0 = static_cast<int64_t>(t.rb) + r0;
-        if (args.kind == kGateUp) {
-          // Lanes 0-15 hold gate rows, 16-31 the up rows of the same features:
-          // of each pair of columns the lower half finishes the first, the
-          // upper half the second.
-          auto *out = static_cast<__nv_bfloat16 *>(args.out);
-          const int f = fb * 64 + q * 16 + (lane & 15);
-          const bool up = lane >= 16;
-#pragma unroll
-          for (int i = 0; i < C::NCH; ++i) {
-            const int c = (2 * i + half) * C::C;
-            if (c < n_mma) {
-#pragma unroll
-              for (int j = 0; j < C::C; j += 2) {
-                const float other =
-                    __shfl_xor_sync(0xffffffffu, up ? acc[i][j] : acc[i][j + 1], 16);
-                const float gv = up ? other : acc[i][j];
-                const float uv = up ? acc[i][j + 1] : other;
-                const int n = c + j + (up ? 1 : 0);
-                if (f < args.n_out && n < rows)
-                  out[(row0 + n) * args.n_out + f] = __float2bfloat16_rn(silu_fast(gv) * uv);
-              }
-            }
-          }
-        } else {
-          const int f = fb * 128 + row;
-#pragma unroll
-          for (int i = 0; i < C::NCH; ++i) {
-            const int c = (2 * i + half) * C::C;
-            if (c < n_mma) {
-              // Lane j knows the route and the weight of column c + j.
-              int32_t route = -1;
-              float weight = 0.f;
-              if (args.kind == kDown && lane < C::C && c + lane < rows) {
-                route = args.row_route[row0 + c + lane];
-                if (route < 0 || route >= args.num_routes) {
-                  atomicOr(&g_status, kStatusIndex);
-                  route = -1;
-                } else {
-                  weight = __bfloat162float(args.route_w[route]);
-                }
-              }
-#pragma unroll
-              for (int j = 0; j < C::C; ++j) {
-                const int n = c + j;
-                const int32_t r = __shfl_sync(0xffffffffu, route, j);
-                const float wgt = __shfl_sync(0xffffffffu, weight, j);
-                if (f < args.n_out && n < rows) {
-                  if (args.kind == kDown) {
-                    if (r >= 0)
-                      static_cast<float *>(args.out)[static_cast<int64_t>(r) * args.n_out + f] =
-                          acc[i][j] * wgt;
-                  } else {
-                    static_cast<__nv_bfloat16 *>(args.out)[(row0 + n) * args.n_out + f] =
-                        __float2bfloat16_rn(acc[i][j]);
-                  }
-                }
-              }
-            }
-          }
-        }
-      }
-    }
+  if (warp == 0) {
+    if (elect_one()) load_codes<NT>(args, c);
+  } else if (warp == 1) {
+    load_rows<NT>(args, c, &tmX, &tmWhole);
+  } else if (warp == 2) {
+    if (elect_one()) issue_mma<NT, GPB>(args, c);
+  } else if (warp >= C::PROMOTE0) {
+    promote<NT, GPB>(args, c, (warp - C::PROMOTE0) >> 2, warp & 3);
+  } else if (warp >= 4) {
+    decode<NT, GPB>(args, c, (warp - 4) >> 2, warp & 3);
   }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (*abort_flag) {
+  if (*c.abort) {
     // A wait ran out: give copies in flight time to land before leaving.
     const uint64_t start = global_timer_ns();
     while (global_timer_ns() - start < 2000000ull) {
@@ -636,7 +705,7 @@ __global__ void __launch_bounds__(Cfg<NT>::THREADS, 1)
   if (split > 1) cluster_sync();  // nobody leaves while a peer may write here
   if (warp == 3) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(c.tmem, 512);
   }
 }
 
@@ -647,16 +716,16 @@ size_t smem_bytes(const Args &a) {
          static_cast<size_t>(a.split - 1) * NT * 512 + TAIL_BYTES;
 }
 
-template <int NT>
-int launch(const CUtensorMap &mx, Args a, double items, cudaStream_t s) {
-  static_assert((2 * MAX_WS + 2 * Cfg<NT>::BS + 2 * A_STAGES + 2 * Cfg<NT>::ND + 2) * 8 + 16 <=
+template <int NT, int GPB>
+int launch(const CUtensorMap &mx, const CUtensorMap &mwhole, Args a, double items, cudaStream_t s) {
+  static_assert((2 * MAX_WS + 3 * Cfg<NT>::BS + 2 * Cfg<NT>::ND + 2) * 8 + 16 <=
                     TAIL_BYTES,
                 "shared memory tail");
   static bool done[64] = {false};
   const int dev = current_device();
   if (!(dev >= 0 && dev < 64 && done[dev])) {
-    B200_CUDA(cudaFuncSetAttribute(w4_gemm_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                   SMEM_LIMIT + 1024));
+    B200_CUDA(cudaFuncSetAttribute(w4_gemm_kernel<NT, GPB>,
+                                   cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT + 1024));
     if (dev >= 0 && dev < 64) done[dev] = true;
   }
   // CTAs per cluster: the split whose rounds of items, each as long as its k
@@ -678,7 +747,7 @@ int launch(const CUtensorMap &mx, Args a, double items, cudaStream_t s) {
   a.ws = static_cast<int>((SMEM_LIMIT - static_cast<int64_t>(Cfg<NT>::BS) * Cfg<NT>::B_BYTES -
                            static_cast<int64_t>(a.split - 1) * NT * 512 - TAIL_BYTES) /
                           a.sh.block_bytes());
-  if (a.ws > MAX_WS) a.ws = MAX_WS;
+  a.ws = (a.ws > MAX_WS ? MAX_WS : a.ws) & ~1;  // the decoding groups step by two
   int clusters = sms / a.split;
   const int64_t most = (a.kind == kLinear ? (a.m + NT - 1) / NT : a.max_mtiles) * a.n_blocks;
   if (most < clusters) clusters = static_cast<int>(most < 1 ? 1 : most);
@@ -703,17 +772,18 @@ int launch(const CUtensorMap &mx, Args a, double items, cudaStream_t s) {
   }
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  B200_CUDA(cudaLaunchKernelEx(&cfg, w4_gemm_kernel<NT>, mx, a));
+  B200_CUDA(cudaLaunchKernelEx(&cfg, w4_gemm_kernel<NT, GPB>, mx, mwhole, a));
   B200_LAUNCHED();
   return B200MOE_OK;
 }
 
-int launch_any(const CUtensorMap &mx, const Args &a, int nt, double items, cudaStream_t s) {
-  switch (nt) {
-    case 16: return launch<16>(mx, a, items, s);
-    case 32: return launch<32>(mx, a, items, s);
-    case 64: return launch<64>(mx, a, items, s);
-    default: return launch<128>(mx, a, items, s);
+template <int NT>
+int launch_nt(const CUtensorMap &mx, const CUtensorMap &mwhole, const Args &a, double items,
+              cudaStream_t s) {
+  switch (a.sh.groups_per_block()) {
+    case 1: return launch<NT, 1>(mx, mwhole, a, items, s);
+    case 2: return launch<NT, 2>(mx, mwhole, a, items, s);
+    default: return launch<NT, 4>(mx, mwhole, a, items, s);
   }
 }
 
@@ -727,14 +797,28 @@ int rows_map(CUtensorMap *map, const void *base, int64_t rows, int k, int box_ro
 // The smallest tile that holds `rows` rows.
 int tile_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 
+// x: [rows, k]; gathered four rows at a time, or in boxes of 16 and nt rows.
+int launch_any(const void *x, int64_t rows, int k, const Args &a, int nt, double items,
+               cudaStream_t s) {
+  CUtensorMap mx, mwhole;
+  int rc = rows_map(&mx, x, rows, k, a.gather ? 1 : 16);
+  if (rc) return rc;
+  rc = a.gather ? B200MOE_OK : rows_map(&mwhole, x, rows, k, nt);
+  if (rc) return rc;
+  if (a.gather) mwhole = mx;
+  switch (nt) {
+    case 16: return launch_nt<16>(mx, mwhole, a, items, s);
+    case 32: return launch_nt<32>(mx, mwhole, a, items, s);
+    case 64: return launch_nt<64>(mx, mwhole, a, items, s);
+    default: return launch_nt<128>(mx, mwhole, a, items, s);
+  }
+}
+
 }  // namespace w4g
 
 int w4_linear_tc(const void *x, int64_t m, int n, int k, const void *w, const w4::Shape &sh,
                  void *out, cudaStream_t s) {
   using namespace w4g;
-  CUtensorMap mx;
-  const int rc = rows_map(&mx, x, m, k, 16);
-  if (rc) return rc;
   Args a = {};
   a.w = static_cast<const uint8_t *>(w);
   a.sh = sh;
@@ -745,7 +829,7 @@ int w4_linear_tc(const void *x, int64_t m, int n, int k, const void *w, const w4
   a.m = m;
   a.out = out;
   const int nt = tile_rows(m);
-  return launch_any(mx, a, nt, static_cast<double>((m + nt - 1) / nt) * a.n_blocks, s);
+  return launch_any(x, m, k, a, nt, static_cast<double>((m + nt - 1) / nt) * a.n_blocks, s);
 }
 
 // `tiles`: how many row tiles the routes are expected to fill; `rows`: rows of
@@ -755,11 +839,6 @@ int w4_gate_up_tc(const RowSource &src, int hidden, int inter, const void *w13,
                   int64_t max_mtiles, const int32_t *counters, double tiles, int64_t rows,
                   void *act, cudaStream_t s) {
   using namespace w4g;
-  CUtensorMap mx;
-  const bool gather = src.x_packed == nullptr;
-  const int rc = rows_map(&mx, gather ? src.x : src.x_packed, gather ? src.x_rows : row_capacity,
-                          hidden, gather ? 1 : 16);
-  if (rc) return rc;
   Args a = {};
   a.w = static_cast<const uint8_t *>(w13);
   a.sh = sh;
@@ -772,11 +851,14 @@ int w4_gate_up_tc(const RowSource &src, int hidden, int inter, const void *w13,
   a.max_mtiles = max_mtiles;
   a.row_route = src.row_route;
   a.num_routes = src.num_routes;
-  a.gather = gather ? 1 : 0;
+  a.gather = src.x_packed == nullptr ? 1 : 0;
   a.top_k = src.top_k;
   a.x_rows = src.x_rows;
   a.out = act;
-  return launch_any(mx, a, tile_rows(rows), tiles * a.n_blocks, s);
+  return a.gather
+             ? launch_any(src.x, src.x_rows, hidden, a, tile_rows(rows), tiles * a.n_blocks, s)
+             : launch_any(src.x_packed, row_capacity, hidden, a, tile_rows(rows),
+                          tiles * a.n_blocks, s);
 }
 
 int w4_down_tc(const void *act, int hidden, int inter, const void *w2, const w4::Shape &sh,
@@ -784,9 +866,6 @@ int w4_down_tc(const void *act, int hidden, int inter, const void *w2, const w4:
                int64_t row_capacity, const int32_t *mtiles, int64_t max_mtiles,
                const int32_t *counters, double tiles, int64_t rows, float *y, cudaStream_t s) {
   using namespace w4g;
-  CUtensorMap mx;
-  const int rc = rows_map(&mx, act, row_capacity, inter, 16);
-  if (rc) return rc;
   Args a = {};
   a.w = static_cast<const uint8_t *>(w2);
   a.sh = sh;
@@ -801,7 +880,7 @@ int w4_down_tc(const void *act, int hidden, int inter, const void *w2, const w4:
   a.route_w = static_cast<const __nv_bfloat16 *>(route_weights);
   a.num_routes = num_routes;
   a.out = y;
-  return launch_any(mx, a, tile_rows(rows), tiles * a.n_blocks, s);
+  return launch_any(act, row_capacity, inter, a, tile_rows(rows), tiles * a.n_blocks, s);
 }
 
 }  // namespace b200moe
