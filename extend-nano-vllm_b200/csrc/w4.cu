@@ -5,13 +5,20 @@
 #include "w4.cuh"
 
 namespace b200moe {
-int w4_linear_gemv(const void *x, int64_t m, int n, int k, const void *w, const w4::Shape &sh,
-                   void *out, cudaStream_t s);
+int w4_linear_stream(const void *x, int64_t m, int n, int k, const void *w, const w4::Shape &sh,
+                     void *out, cudaStream_t s);
+int w4_gate_up_stream(const RowSource &src, int hidden, int inter, const void *w13,
+                      const w4::Shape &sh, const int32_t *mtiles, int64_t max_mtiles,
+                      const int32_t *counters, double tiles, int64_t rows, void *act,
+                      cudaStream_t s);
+int w4_down_stream(const void *act, int hidden, int inter, const void *w2, const w4::Shape &sh,
+                   const int32_t *row_route, const void *route_weights, int64_t num_routes,
+                   const int32_t *mtiles, int64_t max_mtiles, const int32_t *counters,
+                   double tiles, int64_t rows, float *y, cudaStream_t s);
 int w4_route_experts(const void *x, int64_t tokens, int hidden, int inter, const int64_t *ids,
                      const void *weights, int top_k, int num_experts, const void *w13,
-                     const w4::Shape &sh13, const void *w2, const w4::Shape &sh2, float *act,
+                     const w4::Shape &sh13, const void *w2, const w4::Shape &sh2, void *act,
                      void *out, cudaStream_t s);
-
 int w4_linear_tc(const void *x, int64_t m, int n, int k, const void *w, const w4::Shape &sh,
                  void *out, cudaStream_t s);
 int w4_gate_up_tc(const RowSource &src, int hidden, int inter, const void *w13,
@@ -26,10 +33,11 @@ int w4_down_tc(const void *act, int hidden, int inter, const void *w2, const w4:
 namespace {
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// Rows up to which the dense product and routes up to which the experts run
-// on the CUDA cores.
-constexpr int64_t kGemvRows = 4;
-constexpr int64_t kGemvRoutes = 16;
+// Rows of x up to which the weights are streamed (w4_stream.cu); with more,
+// tcgen05 (w4_gemm_sm100.cu).  For experts: rows of a full tile to expect.
+constexpr int64_t kStreamRows = 16;
+// Routes up to which the experts run route by route, without packing.
+constexpr int64_t kRouteRoutes = 16;
 // Routes up to which the gate/up product gathers its rows in its own loads
 // instead of reading a packed copy.
 constexpr int64_t kGatherRoutes = 512;
@@ -48,12 +56,11 @@ struct Workspace {
 
 struct ExpertBuffers {
   int64_t row_capacity = 0, max_mtiles = 0, scratch_bytes = 0;
-  float *act_f32 = nullptr;  // CUDA-core path: [routes, inter]
   int32_t *row_route = nullptr, *route_row = nullptr, *combine_rows = nullptr,
           *tile_expert = nullptr, *offsets = nullptr, *counts = nullptr, *mtiles = nullptr,
           *counters = nullptr, *scratch = nullptr;
   __nv_bfloat16 *x_packed = nullptr;  // above kGatherRoutes routes
-  __nv_bfloat16 *act = nullptr;       // [row_capacity, inter], packed order
+  __nv_bfloat16 *act = nullptr;       // [row_capacity, inter], packed order (few routes: route order)
   float *y = nullptr;                 // [routes, hidden], route order
 };
 
@@ -61,8 +68,8 @@ ExpertBuffers expert_buffers(Workspace &ws, int64_t tokens, int hidden, int inte
                              int num_experts) {
   ExpertBuffers b;
   const int64_t routes = tokens * top_k;
-  if (routes <= kGemvRoutes) {
-    b.act_f32 = ws.take<float>(routes * inter);
+  if (routes <= kRouteRoutes) {
+    b.act = ws.take<__nv_bfloat16>(routes * inter);
     return b;
   }
   b.row_capacity = b200moe_pack_row_capacity(routes, num_experts);
@@ -142,8 +149,8 @@ int b200moe_w4_linear(const void *x, int64_t m, int n, int k, const void *w, int
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const w4::Shape sh = w4::shape_of(group, flags);
   B200_UNSUPPORTED(m < (int64_t)0x7fffffff, "too many rows");
-  return m <= kGemvRows ? w4_linear_gemv(x, m, n, k, w, sh, out, s)
-                        : w4_linear_tc(x, m, n, k, w, sh, out, s);
+  return m <= kStreamRows ? w4_linear_stream(x, m, n, k, w, sh, out, s)
+                          : w4_linear_tc(x, m, n, k, w, sh, out, s);
 }
 
 int64_t b200moe_w4_experts_workspace(int64_t tokens, int hidden, int inter, int top_k,
@@ -182,9 +189,9 @@ int b200moe_w4_experts(const void *x, int64_t tokens, int hidden, int inter,
   Workspace ws;
   ws.base = static_cast<char *>(workspace);
   const ExpertBuffers b = expert_buffers(ws, tokens, hidden, inter, top_k, num_experts);
-  if (routes <= kGemvRoutes)
+  if (routes <= kRouteRoutes)
     return w4_route_experts(x, tokens, hidden, inter, expert_ids, weights, top_k, num_experts, w13,
-                            sh13, w2, sh2, b.act_f32, out, s);
+                            sh13, w2, sh2, b.act, out, s);
   // Without a capacity the packing call writes neither ids nor weights.
   int rc = b200moe_pack_routes(const_cast<int64_t *>(expert_ids), nullptr, routes, num_experts,
                                nullptr, 0, num_experts, nullptr, -1, b.row_capacity, b.row_route,
@@ -207,12 +214,20 @@ int b200moe_w4_experts(const void *x, int64_t tokens, int hidden, int inter,
   // Row tiles to expect when routes fall evenly, and rows of a full one.
   const double mean = static_cast<double>(routes) / num_experts;
   const double tiles = num_experts * (1.0 - exp(-mean)) + static_cast<double>(routes) / 128;
-  const int64_t rows = min64(tokens, static_cast<int64_t>(2.5 * mean) + 16);
-  rc = w4_gate_up_tc(src, hidden, inter, w13, sh13, b.row_capacity, b.mtiles, b.max_mtiles,
-                     b.counters, tiles, rows, b.act, s);
-  if (rc) return rc;
-  rc = w4_down_tc(b.act, hidden, inter, w2, sh2, b.row_route, weights, routes, b.row_capacity,
-                  b.mtiles, b.max_mtiles, b.counters, tiles, rows, b.y, s);
+  const int64_t rows = min64(tokens, static_cast<int64_t>(2.0 * mean + 4.0));
+  if (rows <= kStreamRows) {
+    rc = w4_gate_up_stream(src, hidden, inter, w13, sh13, b.mtiles, b.max_mtiles, b.counters,
+                           tiles, rows, b.act, s);
+    if (rc) return rc;
+    rc = w4_down_stream(b.act, hidden, inter, w2, sh2, b.row_route, weights, routes, b.mtiles,
+                        b.max_mtiles, b.counters, tiles, rows, b.y, s);
+  } else {
+    rc = w4_gate_up_tc(src, hidden, inter, w13, sh13, b.row_capacity, b.mtiles, b.max_mtiles,
+                       b.counters, tiles, rows, b.act, s);
+    if (rc) return rc;
+    rc = w4_down_tc(b.act, hidden, inter, w2, sh2, b.row_route, weights, routes, b.row_capacity,
+                    b.mtiles, b.max_mtiles, b.counters, tiles, rows, b.y, s);
+  }
   if (rc) return rc;
   const int64_t threads = tokens * (hidden / 4);
   B200_LAUNCH_PDL(kPdlCombine, w4_combine_kernel,

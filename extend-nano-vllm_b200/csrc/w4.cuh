@@ -6,14 +6,17 @@
 //
 // A matrix [rows, k] is laid out once as tiles of 128 rows; a tile is a run of
 // blocks of 128 k, each one contiguous piece of memory:
-//   codes  4 chunks x 128 rows x 16 bytes: chunk c holds 32 k of every row, so
-//          32 lanes that own 32 rows read 512 consecutive bytes;
-//   scales [128 / g][128 rows] of 16 bits (bf16 or fp16);
-//   zeros  [128 / g][128 rows] of 8 bits, only with zero points.
-// In each 32-bit word of a chunk, k = 8 j + 2 i sits at bit 4 i and
-// k = 8 j + 2 i + 1 at bit 16 + 4 i: (word >> 4 i) & 0x000f000f is a pair of
-// neighbouring k in the halves of a register, which is how the matrix
-// instruction wants them.  Rows and k beyond the matrix have scale 0.
+//   codes  4 units x 128 rows x 16 bytes: word c of unit u holds the eight k
+//          32 c + 8 u .. + 7 of a row.  A thread that owns a row reads four
+//          units; in a warp matrix instruction lane t of a row reads unit t;
+//   scales [128 / g][128] of 16 bits (bf16 or fp16), in each quarter of 32 rows
+//          row r at place 4 (r % 8) + r / 8 (scale_place): the four rows
+//          r, r + 8, r + 16, r + 24 that one lane needs are neighbours;
+//   zeros  [128 / g][128] of 8 bits in the same order, only with zero points.
+// In each word k = 2 i sits at bit 4 i and k = 2 i + 1 at bit 16 + 4 i:
+// (word >> 4 i) & 0x000f000f is a pair of neighbouring k in the halves of a
+// register, which is how the matrix instructions want them.  Rows and k beyond
+// the matrix have scale 0.
 //
 // "gate_up" order: a tile holds 64 features of a SwiGLU pair [2 I, k] (gate
 // rows first); each quarter of 32 rows is 16 gate rows, then the 16 up rows of
@@ -46,6 +49,10 @@ inline Shape shape_of(int group, int flags) {
 }
 inline bool group_ok(int group) { return group == 32 || group == 64 || group == 128; }
 __host__ __device__ inline int64_t blocks_of(int64_t k) { return (k + kBlockK - 1) / kBlockK; }
+
+__host__ __device__ __forceinline__ int scale_place(int row) {
+  return (row & ~31) | ((row & 7) << 2) | ((row >> 3) & 3);
+}
 
 __device__ __forceinline__ float scale_f32(uint16_t bits, int half_scale) {
   return half_scale ? __half2float(__ushort_as_half(bits))

@@ -45,27 +45,34 @@ constexpr int TAIL_BYTES = 1024;  // barriers
 
 template <int NT>
 struct Cfg {
-  // TMEM: accumulators first, then operand stages of 64 columns (128 k in bf16
-  // pairs).  The operand stages and those of the x rows advance together, so
-  // one completion frees both.
-  static constexpr int D_COLS = NT == 128 ? 256 : 128;
-  static constexpr int ND = D_COLS / NT;             // accumulators
-  static constexpr int BS = (512 - D_COLS) / 64;     // operand stages
-  static constexpr int B_BYTES = NT * 256;           // 128 k of NT rows
+  // TMEM: accumulators in the lower half, operand stages of 64 columns (128 k
+  // in bf16 pairs) in the upper.  The operand stages and those of the x rows
+  // advance together, so one completion frees both.
+  static constexpr int D_COLS = 256;
+  static constexpr int ND = NT == 16 ? 8 : NT == 128 ? 2 : 4;  // accumulators
+  static constexpr int BS = 4;                                  // operand stages
+  static constexpr int B_BYTES = NT * 256;                      // 128 k of NT rows
   static constexpr int C = NT == 16 ? 8 : 16;                  // columns per chunk
   static constexpr int NCH = NT / C / 2;                       // chunks per promoting group
   // Decoding groups: one keeps up with 128-row tiles (512 cycles of matrix
   // instructions per block) and leaves the 64 sums per promoting thread room
   // in the register file; smaller tiles are bound by the code stream.
   static constexpr int DG = NT == 128 ? 1 : 2;
+  static constexpr int UNROLL = NT == 128 ? 1 : 2;  // blocks per loop turn
   static constexpr int PROMOTE0 = 4 + 4 * DG;  // first promoting warp
   static constexpr int THREADS = 32 * (PROMOTE0 + 8);
 };
 
+// One group per block and as many accumulators as operand stages: the two rings
+// are one.
+template <int NT, int GPB>
+__host__ __device__ constexpr bool lockstep() {
+  return GPB == 1 && Cfg<NT>::ND == Cfg<NT>::BS;
+}
+
 struct Args {
   const uint8_t *w;
   Shape sh;
-  int kind;
   int n_blocks;  // weight tiles per matrix
   int num_kb;
   int n_out;     // features written per row
@@ -90,9 +97,9 @@ struct Tile {
   int e, rb, rows;
 };
 
-template <int NT>
+template <int NT, int KIND>
 __device__ __forceinline__ Tile tile_of(const Args &a, int m) {
-  if (a.kind == kLinear) {
+  if (KIND == kLinear) {
     const int64_t rb = static_cast<int64_t>(m) * NT;
     return Tile{0, static_cast<int>(rb), static_cast<int>(min64(NT, a.m - rb))};
   }
@@ -138,16 +145,33 @@ __device__ __forceinline__ void tmem_st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[16]) { tmem_ld16(taddr, v); }
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[8]) {
-  uint32_t r[8];
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[8]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
         "=r"(r[7])
       : "r"(taddr));
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// Two fp32 values in one register pair, and acc += s * (lo, hi) on both.
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void fma2(uint64_t &acc, uint64_t s, uint32_t lo, uint32_t hi) {
+  uint64_t v;
+  asm volatile("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+  asm volatile("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(s), "l"(v));
 }
 
 // ---- cluster helpers ------------------------------------------------------
@@ -252,14 +276,15 @@ struct Ctx {
 };
 
 // Codes: one bulk copy per block of 128 k.  One lane.
-template <int NT>
+template <int NT, int KIND>
 __device__ __forceinline__ void load_codes(const Args &args, const Ctx &c) {
   Ring w;
   for (int it = c.first; it < c.items; it += c.step) {
-    const Tile t = tile_of<NT>(args, it / args.n_blocks);
+    const Tile t = tile_of<NT, KIND>(args, it / args.n_blocks);
     const uint8_t *src = args.w + (static_cast<int64_t>(t.e) * args.n_blocks + it % args.n_blocks) *
                                       args.num_kb * c.wbytes;
     for (int r0 = 0; r0 < t.rows; r0 += NT)
+#pragma unroll 4
       for (int kb = c.kb0; kb < c.kb1; ++kb) {
         if (!wait(c.w_empty + 8 * w.stage, w.phase ^ 1, c.abort)) return;
         const uint32_t bar = c.w_full + 8 * w.stage;
@@ -274,19 +299,19 @@ __device__ __forceinline__ void load_codes(const Args &args, const Ctx &c) {
 // Rows of x.  Dense rows and full tiles come as one box of NT rows per 64 k,
 // the rows of other tiles as boxes of 16 (lane b loads the b-th), gathered
 // rows four at a time (lane l loads the l-th four).  A whole warp.
-template <int NT>
+template <int NT, int KIND>
 __device__ __forceinline__ void load_rows(const Args &args, const Ctx &c, const CUtensorMap *tm,
                                           const CUtensorMap *tm_whole) {
   using C = Cfg<NT>;
   const int lane = threadIdx.x & 31;
-  const bool gather = args.gather != 0;
+  const bool gather = KIND == kGateUp && args.gather != 0;
   Ring b;
   for (int it = c.first; it < c.items; it += c.step) {
-    const Tile t = tile_of<NT>(args, it / args.n_blocks);
+    const Tile t = tile_of<NT, KIND>(args, it / args.n_blocks);
     for (int r0 = 0; r0 < t.rows; r0 += NT) {
       const int rows = min(NT, t.rows - r0);
       const int nbox = (rows + 15) >> 4;
-      const bool whole = !gather && (nbox * 16 == NT || args.kind == kLinear);
+      const bool whole = !gather && (nbox * 16 == NT || KIND == kLinear);
       const bool mine = !whole && lane < (gather ? nbox * 4 : nbox);
       const uint32_t bytes = whole ? C::B_BYTES : nbox * 16 * 256;
       int tok[4] = {0, 0, 0, 0};
@@ -296,6 +321,7 @@ __device__ __forceinline__ void load_rows(const Args &args, const Ctx &c, const 
           tok[j] = gather_token(t.rb + r0 + 4 * lane + j, t.rb + t.rows, args.row_route, nullptr,
                                 args.top_k, args.num_routes, args.x_rows);
       }
+#pragma unroll 2
       for (int kb = c.kb0; kb < c.kb1; ++kb) {
         if (!wait(c.ab_empty + 8 * b.stage, b.phase ^ 1, c.abort)) return;
         const uint32_t bar = c.b_full + 8 * b.stage;
@@ -327,7 +353,7 @@ __device__ __forceinline__ void load_rows(const Args &args, const Ctx &c, const 
 }
 
 // Matrix instructions.  One lane.
-template <int NT, int GPB>
+template <int NT, int GPB, int KIND>
 __device__ __forceinline__ void issue_mma(const Args &args, const Ctx &c) {
   using C = Cfg<NT>;
   constexpr int KK = 8 / GPB;  // instructions of 16 k per group
@@ -335,23 +361,28 @@ __device__ __forceinline__ void issue_mma(const Args &args, const Ctx &c) {
   // Descriptor of stage 0; the start address field counts 16 bytes.
   const uint64_t desc0 = sw128_kmajor_desc(c.s_b);
   for (int it = c.first; it < c.items; it += c.step) {
-    const Tile t = tile_of<NT>(args, it / args.n_blocks);
+    const Tile t = tile_of<NT, KIND>(args, it / args.n_blocks);
     for (int r0 = 0; r0 < t.rows; r0 += NT) {
       const int n_mma = (min(NT, t.rows - r0) + 15) & ~15;
       const uint32_t idesc = idesc_bf16_f32(128, n_mma);
+#pragma unroll 4
       for (int kb = c.kb0; kb < c.kb1; ++kb) {
         // Tried together: each alone costs its latency.
-        const bool b_ready = mbar_try_wait(c.b_full + 8 * b.stage, b.phase);
-        const bool a_ready = mbar_try_wait(c.a_full + 8 * b.stage, b.phase);
-        if (__builtin_expect(!(b_ready && a_ready), 0)) {
-          if (!wait_more<false>(c.b_full + 8 * b.stage, b.phase, c.abort)) return;
-          if (!wait_more<false>(c.a_full + 8 * b.stage, b.phase, c.abort)) return;
+        const uint32_t b_full = c.b_full + 8 * b.stage, a_full = c.a_full + 8 * b.stage;
+        const uint32_t d_empty = c.d_empty + 8 * d.stage;
+        const bool b_ready = mbar_try_wait(b_full, b.phase);
+        const bool a_ready = mbar_try_wait(a_full, b.phase);
+        const bool d_ready = mbar_try_wait(d_empty, d.phase ^ 1);
+        if (__builtin_expect(!(b_ready && a_ready && d_ready), 0)) {
+          if (!wait_more<false>(b_full, b.phase, c.abort)) return;
+          if (!wait_more<false>(a_full, b.phase, c.abort)) return;
+          if (!wait_more<false>(d_empty, d.phase ^ 1, c.abort)) return;
         }
         const uint64_t desc = desc0 + static_cast<uint32_t>(b.stage * (C::B_BYTES >> 4));
         const uint32_t ta = c.tmem + C::D_COLS + b.stage * 64;
 #pragma unroll
         for (int g = 0; g < GPB; ++g) {
-          if (!wait(c.d_empty + 8 * d.stage, d.phase ^ 1, c.abort)) return;
+          if (g > 0 && !wait(c.d_empty + 8 * d.stage, d.phase ^ 1, c.abort)) return;
           tc_fence_after();
           const uint32_t td = c.tmem + d.stage * NT;
 #pragma unroll
@@ -359,7 +390,9 @@ __device__ __forceinline__ void issue_mma(const Args &args, const Ctx &c) {
             const int kk = g * KK + j;
             mma_ts(td, ta + kk * 8, desc + ((kk >> 2) * (NT * 8) + (kk & 3) * 2), idesc, j != 0);
           }
-          tc_commit(c.d_full + 8 * d.stage);
+          // Accumulators in step with the operand stages: one completion
+          // serves both.
+          if (!lockstep<NT, GPB>()) tc_commit(c.d_full + 8 * d.stage);
           d.next(C::ND);
         }
         tc_commit(c.ab_empty + 8 * b.stage);
@@ -371,11 +404,12 @@ __device__ __forceinline__ void issue_mma(const Args &args, const Ctx &c) {
 
 // Decoding: the codes of a block -> q - z as bf16 in the operand stage.  Group
 // `grp` of DG takes every DG-th block.  Four warps, one weight row per thread.
-template <int NT, int GPB>
+template <int NT, int GPB, int KIND>
 __device__ __forceinline__ void decode(const Args &args, const Ctx &c, int grp, int q) {
   using C = Cfg<NT>;
   const int lane = threadIdx.x & 31;
   const int row = q * 32 + lane;
+  const int place = w4::scale_place(row);
   const bool zeros = args.sh.has_zero != 0;
   const uint32_t tq = c.tmem + C::D_COLS + (static_cast<uint32_t>(q * 32) << 16);
   Ring w, a;
@@ -383,9 +417,10 @@ __device__ __forceinline__ void decode(const Args &args, const Ctx &c, int grp, 
   a.next(C::BS, grp);
   int skip = grp;  // blocks until this group's next one
   for (int it = c.first; it < c.items; it += c.step) {
-    const Tile t = tile_of<NT>(args, it / args.n_blocks);
+    const Tile t = tile_of<NT, KIND>(args, it / args.n_blocks);
     for (int r0 = 0; r0 < t.rows; r0 += NT) {
       int kb = c.kb0 + skip;
+#pragma unroll C::UNROLL
       for (; kb < c.kb1; kb += C::DG) {
         if (!wait(c.w_full + 8 * w.stage, w.phase, c.abort)) return;
         const uint32_t st = c.s_w + w.stage * c.wbytes;
@@ -401,7 +436,7 @@ __device__ __forceinline__ void decode(const Args &args, const Ctx &c, int grp, 
         for (int g = 0; g < GPB; ++g) {
           uint32_t z = 8;
           if (zeros)
-            asm volatile("ld.shared.u8 %0, [%1];" : "=r"(z) : "r"(st + c.zero_off + g * 128 + row));
+            asm volatile("ld.shared.u8 %0, [%1];" : "=r"(z) : "r"(st + c.zero_off + g * 128 + place));
           zp[g] = w4::zero_pair(z);
         }
         if (!wait(c.ab_empty + 8 * a.stage, a.phase ^ 1, c.abort)) return;
@@ -412,8 +447,9 @@ __device__ __forceinline__ void decode(const Args &args, const Ctx &c, int grp, 
           uint32_t r[32];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
+            const int ch = 2 * h + (j >> 2), u = j & 3;  // chunk of 32 k, unit
             uint32_t o[4];
-            w4::decode8(code[8 * h + j], zp[(8 * h + j) * GPB / 16], o);
+            w4::decode8(code[4 * u + ch], zp[ch * GPB / 4], o);
 #pragma unroll
             for (int i = 0; i < 4; ++i) r[4 * j + i] = o[i];
           }
@@ -436,7 +472,7 @@ __device__ __forceinline__ void decode(const Args &args, const Ctx &c, int grp, 
 
 // Promoting and epilogue.  Two groups of four warps (alternate column chunks),
 // one weight row per thread.
-template <int NT, int GPB>
+template <int NT, int GPB, int KIND>
 __device__ __forceinline__ void promote(const Args &args, const Ctx &c, int half, int q) {
   using C = Cfg<NT>;
   const int lane = threadIdx.x & 31;
@@ -445,45 +481,42 @@ __device__ __forceinline__ void promote(const Args &args, const Ctx &c, int half
   Ring w, d;
   uint32_t red_phase = 0;
   for (int it = c.first; it < c.items; it += c.step) {
-    const Tile t = tile_of<NT>(args, it / args.n_blocks);
+    const Tile t = tile_of<NT, KIND>(args, it / args.n_blocks);
     const int fb = it % args.n_blocks;
     for (int r0 = 0; r0 < t.rows; r0 += NT) {
       const int rows = min(NT, t.rows - r0);
       const int n_mma = (rows + 15) & ~15;
-      float acc[C::NCH][C::C];
+      uint64_t acc2[C::NCH][C::C / 2];  // pairs of neighbouring columns
 #pragma unroll
       for (int i = 0; i < C::NCH; ++i)
 #pragma unroll
-        for (int j = 0; j < C::C; ++j) acc[i][j] = 0.f;
+        for (int j = 0; j < C::C / 2; ++j) acc2[i][j] = 0;
+#pragma unroll C::UNROLL
       for (int kb = c.kb0; kb < c.kb1; ++kb) {
-        const uint32_t scales = c.s_w + w.stage * c.wbytes + c.scale_off + row * 2;
+        const uint32_t scales = c.s_w + w.stage * c.wbytes + c.scale_off + w4::scale_place(row) * 2;
 #pragma unroll
         for (int g = 0; g < GPB; ++g) {
           // A finished product implies the codes and scales of its stage: the
           // decoding warps waited for the copy before they signalled it.
-          if (!wait(c.d_full + 8 * d.stage, d.phase, c.abort)) return;
+          if (!wait((lockstep<NT, GPB>() ? c.ab_empty : c.d_full) + 8 * d.stage, d.phase, c.abort))
+            return;
           tc_fence_after();
           uint16_t bits;
           asm volatile("ld.shared.u16 %0, [%1];" : "=h"(bits) : "r"(scales + g * 256));
           const float s = w4::scale_f32(bits, args.sh.half_scale);
-          const uint32_t td = tq + d.stage * NT;
+          const uint64_t s2 = pack2(s, s);
+          const uint32_t td = tq + d.stage * NT + half * C::C;
+          // The next chunk loads while this one is added.  Columns beyond
+          // n_mma hold old sums; they are never stored.
+          uint32_t v[2][C::C];
+          tmem_ld(td, v[0]);
 #pragma unroll
-          for (int i = 0; i < C::NCH; i += 2) {
-            float v0[C::C], v1[C::C];
-            constexpr bool pair = C::NCH > 1;
-            const int c0 = (2 * i + half) * C::C;
-            // Columns beyond n_mma hold old sums; they are never stored.
-            if (C::NCH <= 2 || c0 < n_mma) {
-              tmem_ld(td + c0, v0);
-              if (pair) tmem_ld(td + c0 + 2 * C::C, v1);
-              tmem_ld_wait();
+          for (int i = 0; i < C::NCH; ++i) {
+            tmem_ld_wait();
+            if (i + 1 < C::NCH) tmem_ld(td + (i + 1) * 2 * C::C, v[(i + 1) & 1]);
 #pragma unroll
-              for (int j = 0; j < C::C; ++j) acc[i][j] = fmaf(s, v0[j], acc[i][j]);
-              if constexpr (pair) {
-#pragma unroll
-                for (int j = 0; j < C::C; ++j) acc[i + 1][j] = fmaf(s, v1[j], acc[i + 1][j]);
-              }
-            }
+            for (int j = 0; j < C::C / 2; ++j)
+              fma2(acc2[i][j], s2, v[i & 1][2 * j], v[i & 1][2 * j + 1]);
           }
           tc_fence_before();
           __syncwarp();
@@ -493,6 +526,12 @@ __device__ __forceinline__ void promote(const Args &args, const Ctx &c, int half
         if (lane == 0) mbar_arrive(c.w_empty + 8 * w.stage);
         w.next(args.ws);
       }
+      float acc[C::NCH][C::C];
+#pragma unroll
+      for (int i = 0; i < C::NCH; ++i)
+#pragma unroll
+        for (int j = 0; j < C::C / 2; ++j)
+          asm("mov.b64 {%0, %1}, %2;" : "=f"(acc[i][2 * j]), "=f"(acc[i][2 * j + 1]) : "l"(acc2[i][j]));
       if (c.split > 1) {
         if (c.rank != 0) {
           // This CTA's sums into the first one's shared memory.
@@ -534,31 +573,33 @@ __device__ __forceinline__ void promote(const Args &args, const Ctx &c, int half
           for (int p = 1; p < c.split; ++p) arrive_cluster(map_rank(c.red_empty, p));
       }
       const int64_t row0 = static_cast<int64_t>(t.rb) + r0;
-      if (args.kind == kGateUp) {
+      if constexpr (KIND == kGateUp) {
         // Lanes 0-15 hold gate rows, 16-31 the up rows of the same features:
         // of each pair of columns the lower half finishes the first, the upper
         // half the second.
-        auto *out = static_cast<__nv_bfloat16 *>(args.out);
         const int f = fb * 64 + q * 16 + (lane & 15);
         const bool up = lane >= 16;
+        const int odd = up ? 1 : 0;
+        const int last = f < args.n_out ? rows : 0;
 #pragma unroll
         for (int i = 0; i < C::NCH; ++i) {
           const int col = (2 * i + half) * C::C;
           if (col < n_mma) {
+            auto *out = static_cast<__nv_bfloat16 *>(args.out) + (row0 + col + odd) * args.n_out + f;
 #pragma unroll
             for (int j = 0; j < C::C; j += 2) {
               const float other =
                   __shfl_xor_sync(0xffffffffu, up ? acc[i][j] : acc[i][j + 1], 16);
               const float gv = up ? other : acc[i][j];
               const float uv = up ? acc[i][j + 1] : other;
-              const int n = col + j + (up ? 1 : 0);
-              if (f < args.n_out && n < rows)
-                out[(row0 + n) * args.n_out + f] = __float2bfloat16_rn(silu_fast(gv) * uv);
+              if (col + j + odd < last) *out = __float2bfloat16_rn(silu_fast(gv) * uv);
+              out += 2 * static_cast<int64_t>(args.n_out);
             }
           }
         }
-      } else {
+      } else if constexpr (KIND == kDown) {
         const int f = fb * 128 + row;
+        const bool in = f < args.n_out;
 #pragma unroll
         for (int i = 0; i < C::NCH; ++i) {
           const int col = (2 * i + half) * C::C;
@@ -566,7 +607,7 @@ __device__ __forceinline__ void promote(const Args &args, const Ctx &c, int half
             // Lane j knows the route and the weight of column col + j.
             int32_t route = -1;
             float weight = 0.f;
-            if (args.kind == kDown && lane < C::C && col + lane < rows) {
+            if (lane < C::C && col + lane < rows) {
               route = args.row_route[row0 + col + lane];
               if (route < 0 || route >= args.num_routes) {
                 atomicOr(&g_status, kStatusIndex);
@@ -577,19 +618,26 @@ __device__ __forceinline__ void promote(const Args &args, const Ctx &c, int half
             }
 #pragma unroll
             for (int j = 0; j < C::C; ++j) {
-              const int n = col + j;
               const int32_t r = __shfl_sync(0xffffffffu, route, j);
               const float wgt = __shfl_sync(0xffffffffu, weight, j);
-              if (f < args.n_out && n < rows) {
-                if (args.kind == kDown) {
-                  if (r >= 0)
-                    static_cast<float *>(args.out)[static_cast<int64_t>(r) * args.n_out + f] =
-                        acc[i][j] * wgt;
-                } else {
-                  static_cast<__nv_bfloat16 *>(args.out)[(row0 + n) * args.n_out + f] =
-                      __float2bfloat16_rn(acc[i][j]);
-                }
-              }
+              if (in && r >= 0)
+                static_cast<float *>(args.out)[static_cast<int64_t>(r) * args.n_out + f] =
+                    acc[i][j] * wgt;
+            }
+          }
+        }
+      } else {
+        const int f = fb * 128 + row;
+        const int last = f < args.n_out ? rows : 0;
+#pragma unroll
+        for (int i = 0; i < C::NCH; ++i) {
+          const int col = (2 * i + half) * C::C;
+          if (col < n_mma) {
+            auto *out = static_cast<__nv_bfloat16 *>(args.out) + (row0 + col) * args.n_out + f;
+#pragma unroll
+            for (int j = 0; j < C::C; ++j) {
+              if (col + j < last) *out = __float2bfloat16_rn(acc[i][j]);
+              out += args.n_out;
             }
           }
         }
@@ -599,7 +647,7 @@ __device__ __forceinline__ void promote(const Args &args, const Ctx &c, int half
 }
 
 // NT: rows of x per tile; GPB: groups per block of 128 k.
-template <int NT, int GPB>
+template <int NT, int GPB, int KIND>
 __global__ void __launch_bounds__(Cfg<NT>::THREADS, 1)
     w4_gemm_kernel(const __grid_constant__ CUtensorMap tmX,
                    const __grid_constant__ CUtensorMap tmWhole, const __grid_constant__ Args args) {
@@ -671,8 +719,8 @@ __global__ void __launch_bounds__(Cfg<NT>::THREADS, 1)
   c.tmem = *tmem_holder;
   // Codes are constant; a dense call's items are known too, so its first
   // blocks are fetched while the previous kernel still runs.
-  if (!(args.kind == kLinear && warp == 0)) pdl_wait();
-  const int mt = args.kind == kLinear
+  if (!(KIND == kLinear && warp == 0)) pdl_wait();
+  const int mt = KIND == kLinear
                      ? static_cast<int>((args.m + NT - 1) / NT)
                      : static_cast<int>(min64(args.counters[B200MOE_CNT_MTILES], args.max_mtiles));
   c.items = mt * args.n_blocks;
@@ -682,15 +730,15 @@ __global__ void __launch_bounds__(Cfg<NT>::THREADS, 1)
   c.kb1 = (c.rank + 1) * args.num_kb / split;
 
   if (warp == 0) {
-    if (elect_one()) load_codes<NT>(args, c);
+    if (elect_one()) load_codes<NT, KIND>(args, c);
   } else if (warp == 1) {
-    load_rows<NT>(args, c, &tmX, &tmWhole);
+    load_rows<NT, KIND>(args, c, &tmX, &tmWhole);
   } else if (warp == 2) {
-    if (elect_one()) issue_mma<NT, GPB>(args, c);
+    if (elect_one()) issue_mma<NT, GPB, KIND>(args, c);
   } else if (warp >= C::PROMOTE0) {
-    promote<NT, GPB>(args, c, (warp - C::PROMOTE0) >> 2, warp & 3);
+    promote<NT, GPB, KIND>(args, c, (warp - C::PROMOTE0) >> 2, warp & 3);
   } else if (warp >= 4) {
-    decode<NT, GPB>(args, c, (warp - 4) >> 2, warp & 3);
+    decode<NT, GPB, KIND>(args, c, (warp - 4) >> 2, warp & 3);
   }
   __syncwarp();
   tc_fence_before();
@@ -716,7 +764,7 @@ size_t smem_bytes(const Args &a) {
          static_cast<size_t>(a.split - 1) * NT * 512 + TAIL_BYTES;
 }
 
-template <int NT, int GPB>
+template <int NT, int GPB, int KIND>
 int launch(const CUtensorMap &mx, const CUtensorMap &mwhole, Args a, double items, cudaStream_t s) {
   static_assert((2 * MAX_WS + 3 * Cfg<NT>::BS + 2 * Cfg<NT>::ND + 2) * 8 + 16 <=
                     TAIL_BYTES,
@@ -724,7 +772,7 @@ int launch(const CUtensorMap &mx, const CUtensorMap &mwhole, Args a, double item
   static bool done[64] = {false};
   const int dev = current_device();
   if (!(dev >= 0 && dev < 64 && done[dev])) {
-    B200_CUDA(cudaFuncSetAttribute(w4_gemm_kernel<NT, GPB>,
+    B200_CUDA(cudaFuncSetAttribute(w4_gemm_kernel<NT, GPB, KIND>,
                                    cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT + 1024));
     if (dev >= 0 && dev < 64) done[dev] = true;
   }
@@ -749,7 +797,7 @@ int launch(const CUtensorMap &mx, const CUtensorMap &mwhole, Args a, double item
                           a.sh.block_bytes());
   a.ws = (a.ws > MAX_WS ? MAX_WS : a.ws) & ~1;  // the decoding groups step by two
   int clusters = sms / a.split;
-  const int64_t most = (a.kind == kLinear ? (a.m + NT - 1) / NT : a.max_mtiles) * a.n_blocks;
+  const int64_t most = (KIND == kLinear ? (a.m + NT - 1) / NT : a.max_mtiles) * a.n_blocks;
   if (most < clusters) clusters = static_cast<int>(most < 1 ? 1 : most);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(clusters * a.split);
@@ -772,18 +820,18 @@ int launch(const CUtensorMap &mx, const CUtensorMap &mwhole, Args a, double item
   }
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  B200_CUDA(cudaLaunchKernelEx(&cfg, w4_gemm_kernel<NT, GPB>, mx, mwhole, a));
+  B200_CUDA(cudaLaunchKernelEx(&cfg, w4_gemm_kernel<NT, GPB, KIND>, mx, mwhole, a));
   B200_LAUNCHED();
   return B200MOE_OK;
 }
 
-template <int NT>
+template <int NT, int KIND>
 int launch_nt(const CUtensorMap &mx, const CUtensorMap &mwhole, const Args &a, double items,
               cudaStream_t s) {
   switch (a.sh.groups_per_block()) {
-    case 1: return launch<NT, 1>(mx, mwhole, a, items, s);
-    case 2: return launch<NT, 2>(mx, mwhole, a, items, s);
-    default: return launch<NT, 4>(mx, mwhole, a, items, s);
+    case 1: return launch<NT, 1, KIND>(mx, mwhole, a, items, s);
+    case 2: return launch<NT, 2, KIND>(mx, mwhole, a, items, s);
+    default: return launch<NT, 4, KIND>(mx, mwhole, a, items, s);
   }
 }
 
@@ -798,6 +846,7 @@ int rows_map(CUtensorMap *map, const void *base, int64_t rows, int k, int box_ro
 int tile_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 
 // x: [rows, k]; gathered four rows at a time, or in boxes of 16 and nt rows.
+template <int KIND>
 int launch_any(const void *x, int64_t rows, int k, const Args &a, int nt, double items,
                cudaStream_t s) {
   CUtensorMap mx, mwhole;
@@ -807,10 +856,10 @@ int launch_any(const void *x, int64_t rows, int k, const Args &a, int nt, double
   if (rc) return rc;
   if (a.gather) mwhole = mx;
   switch (nt) {
-    case 16: return launch_nt<16>(mx, mwhole, a, items, s);
-    case 32: return launch_nt<32>(mx, mwhole, a, items, s);
-    case 64: return launch_nt<64>(mx, mwhole, a, items, s);
-    default: return launch_nt<128>(mx, mwhole, a, items, s);
+    case 16: return launch_nt<16, KIND>(mx, mwhole, a, items, s);
+    case 32: return launch_nt<32, KIND>(mx, mwhole, a, items, s);
+    case 64: return launch_nt<64, KIND>(mx, mwhole, a, items, s);
+    default: return launch_nt<128, KIND>(mx, mwhole, a, items, s);
   }
 }
 
@@ -822,14 +871,13 @@ int w4_linear_tc(const void *x, int64_t m, int n, int k, const void *w, const w4
   Args a = {};
   a.w = static_cast<const uint8_t *>(w);
   a.sh = sh;
-  a.kind = kLinear;
   a.n_blocks = (n + 127) / 128;
   a.num_kb = static_cast<int>(w4::blocks_of(k));
   a.n_out = n;
   a.m = m;
   a.out = out;
   const int nt = tile_rows(m);
-  return launch_any(x, m, k, a, nt, static_cast<double>((m + nt - 1) / nt) * a.n_blocks, s);
+  return launch_any<kLinear>(x, m, k, a, nt, static_cast<double>((m + nt - 1) / nt) * a.n_blocks, s);
 }
 
 // `tiles`: how many row tiles the routes are expected to fill; `rows`: rows of
@@ -842,7 +890,6 @@ int w4_gate_up_tc(const RowSource &src, int hidden, int inter, const void *w13,
   Args a = {};
   a.w = static_cast<const uint8_t *>(w13);
   a.sh = sh;
-  a.kind = kGateUp;
   a.n_blocks = (inter + 63) / 64;
   a.num_kb = static_cast<int>(w4::blocks_of(hidden));
   a.n_out = inter;
@@ -856,8 +903,8 @@ int w4_gate_up_tc(const RowSource &src, int hidden, int inter, const void *w13,
   a.x_rows = src.x_rows;
   a.out = act;
   return a.gather
-             ? launch_any(src.x, src.x_rows, hidden, a, tile_rows(rows), tiles * a.n_blocks, s)
-             : launch_any(src.x_packed, row_capacity, hidden, a, tile_rows(rows),
+             ? launch_any<kGateUp>(src.x, src.x_rows, hidden, a, tile_rows(rows), tiles * a.n_blocks, s)
+             : launch_any<kGateUp>(src.x_packed, row_capacity, hidden, a, tile_rows(rows),
                           tiles * a.n_blocks, s);
 }
 
@@ -869,7 +916,6 @@ int w4_down_tc(const void *act, int hidden, int inter, const void *w2, const w4:
   Args a = {};
   a.w = static_cast<const uint8_t *>(w2);
   a.sh = sh;
-  a.kind = kDown;
   a.n_blocks = (hidden + 127) / 128;
   a.num_kb = static_cast<int>(w4::blocks_of(inter));
   a.n_out = hidden;
@@ -880,7 +926,7 @@ int w4_down_tc(const void *act, int hidden, int inter, const void *w2, const w4:
   a.route_w = static_cast<const __nv_bfloat16 *>(route_weights);
   a.num_routes = num_routes;
   a.out = y;
-  return launch_any(act, row_capacity, inter, a, tile_rows(rows), tiles * a.n_blocks, s);
+  return launch_any<kDown>(act, row_capacity, inter, a, tile_rows(rows), tiles * a.n_blocks, s);
 }
 
 }  // namespace b200moe

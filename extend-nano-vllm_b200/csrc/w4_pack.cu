@@ -25,33 +25,39 @@ __global__ void __launch_bounds__(w4::kTileRows) w4_pack_kernel(
     valid = src < rows;
   }
   const int64_t groups = k / sh.group;
+  const int place = w4::scale_place(row);
   const uint8_t *crow = codes + (mat * rows + src) * k;
+  uint32_t word[4][4];  // [unit][chunk of 32 k]
+#pragma unroll
   for (int c = 0; c < 4; ++c) {
-    uint32_t word[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int u = 0; u < 4; ++u) word[u][c] = 0u;
     const int64_t k0 = kb * w4::kBlockK + c * 32;
     if (valid && k0 < k) {  // k is a multiple of 32
       uint32_t in[8];
       *reinterpret_cast<uint4 *>(in) = *reinterpret_cast<const uint4 *>(crow + k0);
       *reinterpret_cast<uint4 *>(in + 4) = *reinterpret_cast<const uint4 *>(crow + k0 + 16);
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int u = 0; u < 4; ++u)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const uint32_t q = (in[2 * j + i / 4] >> (8 * (i & 3))) & 15u;
-          word[j] |= q << ((i & 1) * 16 + (i >> 1) * 4);
+          const uint32_t q = (in[2 * u + i / 4] >> (8 * (i & 3))) & 15u;
+          word[u][c] |= q << ((i & 1) * 16 + (i >> 1) * 4);
         }
     }
-    *reinterpret_cast<uint4 *>(block + c * 2048 + row * 16) =
-        make_uint4(word[0], word[1], word[2], word[3]);
   }
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    *reinterpret_cast<uint4 *>(block + u * 2048 + row * 16) =
+        make_uint4(word[u][0], word[u][1], word[u][2], word[u][3]);
   for (int g = 0; g < sh.groups_per_block(); ++g) {
     const int64_t gi = kb * sh.groups_per_block() + g;
     const bool in = valid && gi < groups;
     const int64_t at = (mat * rows + src) * groups + gi;
-    reinterpret_cast<uint16_t *>(block + sh.scale_off())[g * w4::kTileRows + row] =
+    reinterpret_cast<uint16_t *>(block + sh.scale_off())[g * w4::kTileRows + place] =
         in ? scales[at] : static_cast<uint16_t>(0);
     if (sh.has_zero)
-      block[sh.zero_off() + g * w4::kTileRows + row] =
+      block[sh.zero_off() + g * w4::kTileRows + place] =
           in ? static_cast<uint8_t>(zeros[at] & 15) : static_cast<uint8_t>(0);
   }
 }

@@ -1,0 +1,587 @@
+// Products of a few rows with 4-bit weights (layout: w4.cuh), bound by reading
+// the weights: the dense product and the experts' gate/up (+ SwiGLU) and down
+// projections.
+//
+//   D_g[f, r] = sum_{k in group g} (q[f, k] - z[f, g]) * x[r, k]
+//   y[r, f]   = sum_g s[f, g] * D_g[f, r]
+//
+// Each warp streams its own weights, global memory -> registers -> integers
+// q - z (exact in bf16) -> warp matrix instructions (m16n8k16: 16 weight rows,
+// 8 rows of x), and adds a group's sum to fp32 registers times its scale.  No
+// shared memory, no barrier and no second warp is on the way of a weight, which
+// is what a stream of 4-bit weights needs: at the copy rate an SM has some 23
+// cycles for 512 codes, and the decoding alone takes 7 of each scheduler's.
+// (tcgen05 wants the operand decoded by one warp, waited for by another and
+// read back by a third; that pays from more than 16 rows on, w4_gemm_sm100.cu.)
+//
+// A warp owns 32 weight rows (a quarter of a tile): two 16-row operands, which
+// in gate_up order are the gate and the up rows of the same 16 features, so the
+// SwiGLU product needs no exchange.  Lane (g, t) = (lane / 4, lane % 4) reads
+// 16 bytes of rows g, g + 8 of each operand: word c holds k = 32 c + 8 t ..
+// + 7.  The order of k inside one instruction is free as long as both operands
+// agree, so lane t feeds it its own eight k, and reads the same eight k of x.
+//
+// The blocks of k of an item are split over WK warps of the thread block where
+// items are few, and summed through shared memory in a fixed order.
+#include "w4.cuh"
+
+namespace b200moe {
+namespace w4s {
+
+using w4::Shape;
+
+enum Kind { kLinear = 0, kGateUp = 1, kDown = 2 };
+constexpr int kWarps = 8;
+
+struct Args {
+  const uint8_t *w;
+  Shape sh;
+  int n_blocks;  // tiles per matrix
+  int num_kb;
+  int n_out;
+  int k;
+  int wk;  // warps that share an item's k
+  int m;   // dense rows
+  const void *x;  // bf16 rows of k values
+  int64_t x_rows;
+  const int32_t *mtiles;
+  const int32_t *counters;
+  int64_t max_mtiles;
+  const int32_t *row_route;
+  const __nv_bfloat16 *route_w;
+  int64_t num_routes;
+  int gather;  // x is the token matrix, rows through row_route
+  int top_k;
+  // Few routes: no packing, row tile m is route m alone (ids[m] its expert).
+  const int64_t *ids;
+  int num_experts;
+  void *out;  // bf16 rows (linear, gate/up) or fp32 route rows (down)
+};
+
+__device__ __forceinline__ uint4 load_codes(const uint8_t *p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+__device__ __forceinline__ uint32_t word(const uint4 &v, int c) {
+  return c == 0 ? v.x : c == 1 ? v.y : c == 2 ? v.z : v.w;
+}
+
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                    uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// One block's share of a lane: 16 bytes of rows g, g + 8, ... (two per operand
+// of 16 rows), and those rows' scales and zero points.
+template <int GPB>
+struct Block {
+  uint4 codes[4];
+  uint2 scale[GPB];     // four of 16 bits
+  uint32_t zero[GPB];   // four of 8 bits
+
+  __device__ __forceinline__ void load(const uint8_t *block, int quarter, int g, int t,
+                                       bool zeros) {
+    const uint8_t *c = block + t * 2048 + (quarter * 32 + g) * 16;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) codes[i] = load_codes(c + i * 128);
+    const uint8_t *s = block + w4::kCodeBytes + (quarter * 32 + 4 * g) * 2;
+#pragma unroll
+    for (int j = 0; j < GPB; ++j) scale[j] = __ldg(reinterpret_cast<const uint2 *>(s + j * 256));
+    if (zeros) {
+      const uint8_t *z = block + w4::kCodeBytes + GPB * 256 + quarter * 32 + 4 * g;
+#pragma unroll
+      for (int j = 0; j < GPB; ++j) zero[j] = __ldg(reinterpret_cast<const uint32_t *>(z + j * 128));
+    }
+  }
+  // Scale and zero of row g + 8 i.
+  __device__ __forceinline__ float scale_of(int j, int i, int half_scale) const {
+    const uint32_t v = i < 2 ? scale[j].x : scale[j].y;
+    return w4::scale_f32(static_cast<uint16_t>((i & 1) ? v >> 16 : v & 0xffffu), half_scale);
+  }
+  __device__ __forceinline__ uint32_t zpair_of(int j, int i, bool zeros) const {
+    return w4::zero_pair(zeros ? (zero[j] >> (8 * i)) & 15u : 8u);
+  }
+};
+
+// Adds one block to tot[operand][column tile][4].  xp[n]: this lane's eight k
+// of chunk 0 of row 8 n + g, null for a row that is not there.
+template <int GPB, int NB>
+__device__ __forceinline__ void add_block(const Block<GPB> &b, int half_scale, bool zeros,
+                                          const __nv_bfloat16 *const (&xp)[NB], int k0, int k,
+                                          float (&tot)[2][NB][4]) {
+#pragma unroll
+  for (int j = 0; j < GPB; ++j) {
+    uint4 xv[4 / GPB][NB];
+#pragma unroll
+    for (int cc = 0; cc < 4 / GPB; ++cc)
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        const int at = k0 + 32 * (j * (4 / GPB) + cc);
+        xv[cc][n] = xp[n] != nullptr && at < k ? *reinterpret_cast<const uint4 *>(xp[n] + at)
+                                               : make_uint4(0, 0, 0, 0);
+      }
+    float acc[2][NB][4];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.f;
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const uint32_t z0 = b.zpair_of(j, 2 * m, zeros), z1 = b.zpair_of(j, 2 * m + 1, zeros);
+#pragma unroll
+      for (int cc = 0; cc < 4 / GPB; ++cc) {
+        const int c = j * (4 / GPB) + cc;
+        uint32_t lo[4], hi[4];
+        w4::decode8(word(b.codes[2 * m], c), z0, lo);
+        w4::decode8(word(b.codes[2 * m + 1], c), z1, hi);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          mma(acc[m][n], lo[0], hi[0], lo[1], hi[1], xv[cc][n].x, xv[cc][n].y);
+          mma(acc[m][n], lo[2], hi[2], lo[3], hi[3], xv[cc][n].z, xv[cc][n].w);
+        }
+      }
+      const float s0 = b.scale_of(j, 2 * m, half_scale), s1 = b.scale_of(j, 2 * m + 1, half_scale);
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        tot[m][n][0] = fmaf(s0, acc[m][n][0], tot[m][n][0]);
+        tot[m][n][1] = fmaf(s0, acc[m][n][1], tot[m][n][1]);
+        tot[m][n][2] = fmaf(s1, acc[m][n][2], tot[m][n][2]);
+        tot[m][n][3] = fmaf(s1, acc[m][n][3], tot[m][n][3]);
+      }
+    }
+  }
+}
+
+// A work item of a warp: a quarter of a tile, against the rows of one row tile.
+struct Item {
+  const uint8_t *w;  // the tile's first block
+  int rb, rows;
+  int tile, quarter;
+};
+
+template <int KIND>
+__device__ __forceinline__ Item item_of(const Args &a, int it) {
+  const int per_tile = 4 * a.n_blocks;
+  const int m = it / per_tile;
+  const int rest = it - m * per_tile;
+  Item r;
+  r.tile = rest >> 2;
+  r.quarter = rest & 3;
+  int e = 0;
+  if (KIND == kLinear) {
+    r.rb = 0;
+    r.rows = a.m;
+  } else if (KIND == kGateUp && a.ids != nullptr) {
+    const int64_t id = a.ids[m];
+    const bool live = id >= 0 && id < a.num_experts;
+    e = live ? static_cast<int>(id) : 0;
+    r.rb = m;
+    r.rows = live ? 1 : 0;
+  } else {
+    const int32_t *t = a.mtiles + m * B200MOE_MTILE_WORDS;
+    e = t[0];
+    r.rb = t[1];
+    r.rows = t[2] - t[1];
+  }
+  r.w = a.w + (static_cast<int64_t>(e) * a.n_blocks + r.tile) * a.num_kb * a.sh.block_bytes();
+  return r;
+}
+
+// The finished sums of one operand row pair, to memory.  f: feature row of the
+// item's operand (g or g + 8 within 16), n: column.
+template <int KIND>
+__device__ __forceinline__ void store(const Args &a, const Item &it, int r0, int g, int n,
+                                      float v0, float v1) {
+  // v0: first operand (gate rows, or rows 0-15), v1: second (up, or 16-31).
+  const int col = r0 + n;
+  if (col >= it.rows) return;
+  const int64_t row = it.rb + col;
+  if constexpr (KIND == kGateUp) {
+    const int f = it.tile * 64 + it.quarter * 16 + g;
+    if (f < a.n_out)
+      static_cast<__nv_bfloat16 *>(a.out)[row * a.n_out + f] =
+          __float2bfloat16_rn(__fdividef(v0, 1.0f + __expf(-v0)) * v1);
+  } else {
+    const int f = it.tile * 128 + it.quarter * 32 + g;
+    if constexpr (KIND == kDown) {
+      const int32_t r = a.row_route[row];
+      if (r < 0 || r >= a.num_routes) {
+        atomicOr(&g_status, kStatusIndex);
+        return;
+      }
+      const float w = __bfloat162float(a.route_w[r]);
+      float *out = static_cast<float *>(a.out) + static_cast<int64_t>(r) * a.n_out + f;
+      if (f < a.n_out) out[0] = v0 * w;
+      if (f + 16 < a.n_out) out[16] = v1 * w;
+    } else {
+      __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(a.out) + row * a.n_out + f;
+      if (f < a.n_out) out[0] = __float2bfloat16_rn(v0);
+      if (f + 16 < a.n_out) out[16] = __float2bfloat16_rn(v1);
+    }
+  }
+}
+
+// NB * 8 rows of x at a time.
+template <int GPB, int KIND, int NB>
+__global__ void __launch_bounds__(32 * kWarps, 2) w4_stream_kernel(
+    const __grid_constant__ Args a) {
+  __shared__ float red[kWarps][2 * NB * 4][32];
+  pdl_trigger();
+  const int lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  const int wk = a.wk;
+  const int wr = kWarps / wk;  // items of a thread block at a time
+  const int part = warp / wr;
+  const bool zeros = a.sh.has_zero != 0;
+  const int bytes = a.sh.block_bytes();
+  if (KIND != kLinear) pdl_wait();
+  const int mt = KIND == kLinear ? 1
+                 : KIND == kGateUp && a.ids != nullptr
+                     ? static_cast<int>(a.num_routes)
+                     : static_cast<int>(min64(a.counters[B200MOE_CNT_MTILES], a.max_mtiles));
+  const int items = mt * 4 * a.n_blocks;
+  const int stride = gridDim.x * wr;
+  int cur = blockIdx.x * wr + warp % wr;
+  // All warps of a block take the same number of turns (they meet when k is
+  // shared); a turn past the end does nothing.
+  Block<GPB> next;
+  Item it = {};
+  if (cur < items) {
+    it = item_of<KIND>(a, cur);
+    next.load(it.w + static_cast<int64_t>(part) * bytes, it.quarter, g, t, zeros);
+  }
+  if (KIND == kLinear) pdl_wait();  // codes are constant, x is not
+  for (int turn = blockIdx.x * wr; turn < items; turn += stride, cur += stride) {
+    const bool live = cur < items;
+    const bool more = cur + stride < items;
+    Item following = it;
+    if (more) following = item_of<KIND>(a, cur + stride);
+    const int rows = live ? it.rows : 0;
+    for (int r0 = 0; r0 < rows || (r0 == 0 && wk > 1); r0 += 8 * NB) {
+      const __nv_bfloat16 *xp[NB];
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        const int col = r0 + 8 * n + g;
+        xp[n] = nullptr;
+        if (col < rows) {
+          int64_t row = it.rb + col;
+          if (KIND == kGateUp && a.gather)
+            row = a.ids != nullptr
+                      ? row / a.top_k
+                      : gather_token(row, it.rb + it.rows, a.row_route, nullptr, a.top_k,
+                                     a.num_routes, a.x_rows);
+          xp[n] = static_cast<const __nv_bfloat16 *>(a.x) + row * a.k + 8 * t;
+        }
+      }
+      float tot[2][NB][4];
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) tot[m][n][j] = 0.f;
+      const bool last = r0 + 8 * NB >= rows;
+      if (live) {
+        for (int kb = part; kb < a.num_kb; kb += wk) {
+          const Block<GPB> now = next;
+          // The next block, or the first of this warp's next turn.
+          const uint8_t *from = nullptr;
+          int quarter = it.quarter;
+          if (kb + wk < a.num_kb) {
+            from = it.w + static_cast<int64_t>(kb + wk) * bytes;
+          } else if (!last) {
+            from = it.w + static_cast<int64_t>(part) * bytes;
+          } else if (more) {
+            from = following.w + static_cast<int64_t>(part) * bytes;
+            quarter = following.quarter;
+          }
+          if (from != nullptr) next.load(from, quarter, g, t, zeros);
+          add_block<GPB, NB>(now, a.sh.half_scale, zeros, xp, kb * w4::kBlockK, a.k, tot);
+        }
+      }
+      if (wk == 1) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            store<KIND>(a, it, r0, g + (j >> 1) * 8, 8 * n + 2 * t + (j & 1), tot[0][n][j],
+                        tot[1][n][j]);
+      } else {
+        __syncthreads();
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) red[warp][(m * NB + n) * 4 + j][lane] = tot[m][n][j];
+        __syncthreads();
+        // Warp `part` of the wk that share an item finishes every wk-th of its
+        // values.
+        for (int v = part; v < NB * 4; v += wk) {
+          float v0 = 0.f, v1 = 0.f;
+          for (int p = 0; p < wk; ++p) {
+            v0 += red[p * wr + warp % wr][v][lane];
+            v1 += red[p * wr + warp % wr][NB * 4 + v][lane];
+          }
+          const int n = v >> 2, j = v & 3;
+          if (live)
+            store<KIND>(a, it, r0, g + (j >> 1) * 8, 8 * n + 2 * t + (j & 1), v0, v1);
+        }
+      }
+    }
+    it = following;
+  }
+}
+
+// Few routes: out[t, f] = sum_s weight[t, s] * (D_e act[t, s])[f] in slot order.
+// grid (16-row slabs, tokens); warp w takes slots w, w + 8, ...
+template <int GPB>
+__global__ void __launch_bounds__(32 * kWarps) w4_down_slots_kernel(
+    const __nv_bfloat16 *act, int hidden, int inter, const int64_t *ids,
+    const __nv_bfloat16 *weights, int top_k, int num_experts, const uint8_t *w2, const Shape sh,
+    int tiles, int num_kb, __nv_bfloat16 *__restrict__ out) {
+  constexpr int BATCH = GPB == 4 ? 4 : 6;  // blocks in flight
+  __shared__ float part[32][16];
+  pdl_trigger();
+  const int lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  const int tile = blockIdx.x >> 3, quarter = (blockIdx.x >> 1) & 3, op = blockIdx.x & 1;
+  const int64_t token = blockIdx.y;
+  const bool zeros = sh.has_zero != 0;
+  const int bytes = sh.block_bytes();
+  pdl_wait();
+  for (int s = warp; s < top_k; s += kWarps) {
+    const int64_t route = token * top_k + s;
+    const int64_t e = ids[route];
+    const bool live = e >= 0 && e < num_experts;
+    float tot[4] = {0.f, 0.f, 0.f, 0.f};
+    if (live) {
+      const uint8_t *w = w2 + (e * tiles + tile) * num_kb * bytes;
+      const __nv_bfloat16 *x = act + route * inter + 8 * t;
+      for (int kb0 = 0; kb0 < num_kb; kb0 += BATCH) {
+        uint4 codes[BATCH][2];
+        uint32_t scale[BATCH][GPB];
+        uint32_t zero[BATCH][GPB];
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b)
+          if (kb0 + b < num_kb) {
+            const uint8_t *block = w + static_cast<int64_t>(kb0 + b) * bytes;
+            const uint8_t *c = block + t * 2048 + (quarter * 32 + op * 16 + g) * 16;
+            codes[b][0] = load_codes(c);
+            codes[b][1] = load_codes(c + 128);
+            const uint8_t *sc = block + w4::kCodeBytes + (quarter * 32 + 4 * g + 2 * op) * 2;
+#pragma unroll
+            for (int j = 0; j < GPB; ++j) {
+              scale[b][j] = __ldg(reinterpret_cast<const uint32_t *>(sc + j * 256));
+              if (zeros)
+                zero[b][j] = __ldg(reinterpret_cast<const uint16_t *>(
+                    block + w4::kCodeBytes + GPB * 256 + j * 128 + quarter * 32 + 4 * g + 2 * op));
+            }
+          }
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b)
+          if (kb0 + b < num_kb) {
+#pragma unroll
+            for (int j = 0; j < GPB; ++j) {
+              float acc[4] = {0.f, 0.f, 0.f, 0.f};
+              const uint32_t z0 = w4::zero_pair(zeros ? zero[b][j] & 15u : 8u);
+              const uint32_t z1 = w4::zero_pair(zeros ? (zero[b][j] >> 8) & 15u : 8u);
+#pragma unroll
+              for (int cc = 0; cc < 4 / GPB; ++cc) {
+                const int c = j * (4 / GPB) + cc;
+                const int at = (kb0 + b) * w4::kBlockK + 32 * c;
+                // Column 0 is the act row, the other columns are zero.
+                const uint4 xv = g == 0 && at < inter ? *reinterpret_cast<const uint4 *>(x + at)
+                                                      : make_uint4(0, 0, 0, 0);
+                uint32_t lo[4], hi[4];
+                w4::decode8(word(codes[b][0], c), z0, lo);
+                w4::decode8(word(codes[b][1], c), z1, hi);
+                mma(acc, lo[0], hi[0], lo[1], hi[1], xv.x, xv.y);
+                mma(acc, lo[2], hi[2], lo[3], hi[3], xv.z, xv.w);
+              }
+              const float s0 = w4::scale_f32(scale[b][j] & 0xffffu, sh.half_scale);
+              const float s1 = w4::scale_f32(scale[b][j] >> 16, sh.half_scale);
+              tot[0] = fmaf(s0, acc[0], tot[0]);
+              tot[2] = fmaf(s1, acc[2], tot[2]);
+            }
+          }
+      }
+    }
+    if (t == 0) {
+      const float w = live ? __bfloat162float(weights[route]) : 0.f;
+      part[s][g] = live ? tot[0] * w : 0.f;
+      part[s][g + 8] = live ? tot[2] * w : 0.f;
+    }
+  }
+  __syncthreads();
+  const int f = tile * w4::kTileRows + quarter * 32 + op * 16 + threadIdx.x;
+  if (threadIdx.x < 16 && f < hidden) {
+    float v = 0.f;
+    for (int s = 0; s < top_k; ++s) v += part[s][threadIdx.x];
+    out[token * hidden + f] = __float2bfloat16_rn(v);
+  }
+}
+
+template <int GPB, int KIND, int NB>
+int launch(const Args &a, int64_t blocks, cudaStream_t s) {
+  B200_LAUNCH_PDL(kPdlStream, w4_stream_kernel<GPB, KIND, NB>, dim3(static_cast<unsigned>(blocks)),
+                  dim3(32 * kWarps), 0, s, a);
+  B200_LAUNCHED();
+  return B200MOE_OK;
+}
+
+// items: warp items expected; most: an upper bound.  rows: of a row tile.
+template <int KIND>
+int run(Args a, double items, int64_t most, int64_t rows, cudaStream_t s) {
+  const int nb = rows <= 8 ? 1 : 2;
+  const int64_t slots = static_cast<int64_t>(sm_count()) * 2;
+  // Warps per item: the number whose rounds of items, each as long as its
+  // blocks and two more to begin and end, are over first.
+  double best = 1e30;
+  for (int wk = 1; wk <= kWarps && (wk == 1 || wk <= a.num_kb); wk *= 2) {
+    const int64_t rounds = static_cast<int64_t>((items * wk + slots * kWarps - 1) /
+                                                (slots * kWarps));
+    const double time = static_cast<double>(rounds < 1 ? 1 : rounds) *
+                        ((a.num_kb + wk - 1) / wk + 2.0);
+    if (time < best - 1e-9) {
+      best = time;
+      a.wk = wk;
+    }
+  }
+  const int wr = kWarps / a.wk;
+  int64_t blocks = (most + wr - 1) / wr;
+  if (blocks > slots) blocks = slots;
+  if (blocks < 1) blocks = 1;
+#define B200_W4S(G)                                                         \
+  return nb == 1 ? launch<G, KIND, 1>(a, blocks, s) : launch<G, KIND, 2>(a, blocks, s);
+  switch (a.sh.groups_per_block()) {
+    case 1: B200_W4S(1)
+    case 2: B200_W4S(2)
+    default: B200_W4S(4)
+  }
+#undef B200_W4S
+}
+
+}  // namespace w4s
+
+int w4_linear_stream(const void *x, int64_t m, int n, int k, const void *w, const w4::Shape &sh,
+                     void *out, cudaStream_t s) {
+  using namespace w4s;
+  Args a = {};
+  a.w = static_cast<const uint8_t *>(w);
+  a.sh = sh;
+  a.n_blocks = (n + 127) / 128;
+  a.num_kb = static_cast<int>(w4::blocks_of(k));
+  a.n_out = n;
+  a.k = k;
+  a.m = static_cast<int>(m);
+  a.x = x;
+  a.x_rows = m;
+  a.out = out;
+  return run<kLinear>(a, 4.0 * a.n_blocks, 4ll * a.n_blocks, m, s);
+}
+
+int w4_gate_up_stream(const RowSource &src, int hidden, int inter, const void *w13,
+                      const w4::Shape &sh, const int32_t *mtiles, int64_t max_mtiles,
+                      const int32_t *counters, double tiles, int64_t rows, void *act,
+                      cudaStream_t s) {
+  using namespace w4s;
+  Args a = {};
+  a.w = static_cast<const uint8_t *>(w13);
+  a.sh = sh;
+  a.n_blocks = (inter + 63) / 64;
+  a.num_kb = static_cast<int>(w4::blocks_of(hidden));
+  a.n_out = inter;
+  a.k = hidden;
+  a.gather = src.x_packed == nullptr ? 1 : 0;
+  a.x = a.gather ? src.x : src.x_packed;
+  a.x_rows = src.x_rows;
+  a.mtiles = mtiles;
+  a.counters = counters;
+  a.max_mtiles = max_mtiles;
+  a.row_route = src.row_route;
+  a.num_routes = src.num_routes;
+  a.top_k = src.top_k;
+  a.out = act;
+  return run<kGateUp>(a, 4.0 * tiles * a.n_blocks, 4 * max_mtiles * a.n_blocks, rows, s);
+}
+
+int w4_down_stream(const void *act, int hidden, int inter, const void *w2, const w4::Shape &sh,
+                   const int32_t *row_route, const void *route_weights, int64_t num_routes,
+                   const int32_t *mtiles, int64_t max_mtiles, const int32_t *counters,
+                   double tiles, int64_t rows, float *y, cudaStream_t s) {
+  using namespace w4s;
+  Args a = {};
+  a.w = static_cast<const uint8_t *>(w2);
+  a.sh = sh;
+  a.n_blocks = (hidden + 127) / 128;
+  a.num_kb = static_cast<int>(w4::blocks_of(inter));
+  a.n_out = hidden;
+  a.k = inter;
+  a.x = act;
+  a.mtiles = mtiles;
+  a.counters = counters;
+  a.max_mtiles = max_mtiles;
+  a.row_route = row_route;
+  a.route_w = static_cast<const __nv_bfloat16 *>(route_weights);
+  a.num_routes = num_routes;
+  a.out = y;
+  return run<kDown>(a, 4.0 * tiles * a.n_blocks, 4 * max_mtiles * a.n_blocks, rows, s);
+}
+
+// The whole expert path for few routes, without packing, in two launches.
+// act: [tokens * top_k, inter] bf16.
+int w4_route_experts(const void *x, int64_t tokens, int hidden, int inter, const int64_t *ids,
+                     const void *weights, int top_k, int num_experts, const void *w13,
+                     const w4::Shape &sh13, const void *w2, const w4::Shape &sh2, void *act,
+                     void *out, cudaStream_t s) {
+  using namespace w4s;
+  Args a = {};
+  a.w = static_cast<const uint8_t *>(w13);
+  a.sh = sh13;
+  a.n_blocks = (inter + 63) / 64;
+  a.num_kb = static_cast<int>(w4::blocks_of(hidden));
+  a.n_out = inter;
+  a.k = hidden;
+  a.gather = 1;
+  a.x = x;
+  a.x_rows = tokens;
+  a.num_routes = tokens * top_k;
+  a.top_k = top_k;
+  a.ids = ids;
+  a.num_experts = num_experts;
+  a.out = act;
+  const int64_t items = 4 * a.num_routes * a.n_blocks;
+  const int rc = run<kGateUp>(a, static_cast<double>(items), items, 1, s);
+  if (rc) return rc;
+  const int tiles = (hidden + 127) / 128;
+  const dim3 grid(8 * tiles, static_cast<unsigned>(tokens));
+  auto down = [&](auto kernel) {
+    return launch_pdl(kPdlTiny, kernel, grid, dim3(32 * kWarps), 0, s,
+                      static_cast<const __nv_bfloat16 *>(act), hidden, inter, ids,
+                      static_cast<const __nv_bfloat16 *>(weights), top_k, num_experts,
+                      static_cast<const uint8_t *>(w2), sh2, tiles,
+                      static_cast<int>(w4::blocks_of(inter)), static_cast<__nv_bfloat16 *>(out));
+  };
+  switch (sh2.groups_per_block()) {
+    case 1: B200_CUDA(down(w4_down_slots_kernel<1>)); break;
+    case 2: B200_CUDA(down(w4_down_slots_kernel<2>)); break;
+    default: B200_CUDA(down(w4_down_slots_kernel<4>)); break;
+  }
+  B200_LAUNCHED();
+  return B200MOE_OK;
+}
+
+}  // namespace b200moe
