@@ -5,14 +5,15 @@
 //   g in {32, 64, 128}, zero = 8 where no zero points are given.
 //
 // A matrix [rows, k] is laid out once as tiles of 128 rows; a tile is a run of
-// blocks of 128 k, each one contiguous piece of memory:
-//   codes  4 units x 128 rows x 16 bytes: word c of unit u holds the eight k
+// blocks of 128 k, a block four quarters of 32 rows, and a quarter one
+// contiguous piece of memory (what one copy brings):
+//   codes  4 units x 32 rows x 16 bytes: word c of unit u holds the eight k
 //          32 c + 8 u .. + 7 of a row.  A thread that owns a row reads four
 //          units; in a warp matrix instruction lane t of a row reads unit t;
-//   scales [128 / g][128] of 16 bits (bf16 or fp16), in each quarter of 32 rows
-//          row r at place 4 (r % 8) + r / 8 (scale_place): the four rows
-//          r, r + 8, r + 16, r + 24 that one lane needs are neighbours;
-//   zeros  [128 / g][128] of 8 bits in the same order, only with zero points.
+//   scales [128 / g][32] of 16 bits (bf16 or fp16), row r at place
+//          4 (r % 8) + r / 8 (scale_place): the four rows r, r + 8, r + 16,
+//          r + 24 that one lane needs are neighbours;
+//   zeros  [128 / g][32] of 8 bits in the same order, only with zero points.
 // In each word k = 2 i sits at bit 4 i and k = 2 i + 1 at bit 16 + 4 i:
 // (word >> 4 i) & 0x000f000f is a pair of neighbouring k in the halves of a
 // register, which is how the matrix instructions want them.  Rows and k beyond
@@ -30,18 +31,21 @@ namespace w4 {
 
 constexpr int kTileRows = 128;
 constexpr int kBlockK = 128;
-constexpr int kCodeBytes = kTileRows * kBlockK / 2;  // 8192 per block
+constexpr int kQuarterRows = 32;
+constexpr int kCodeBytes = kQuarterRows * kBlockK / 2;  // 2048 per quarter
 
 struct Shape {
   int group;       // k per scale: 32, 64 or 128
   int has_zero;    // zero points follow the scales
   int half_scale;  // scales are fp16 (else bf16)
   __host__ __device__ int groups_per_block() const { return kBlockK / group; }
+  // Within a quarter.
   __host__ __device__ int scale_off() const { return kCodeBytes; }
-  __host__ __device__ int zero_off() const { return kCodeBytes + groups_per_block() * 256; }
-  __host__ __device__ int block_bytes() const {
-    return kCodeBytes + groups_per_block() * (has_zero ? 384 : 256);
+  __host__ __device__ int zero_off() const { return kCodeBytes + groups_per_block() * 64; }
+  __host__ __device__ int quarter_bytes() const {
+    return kCodeBytes + groups_per_block() * (has_zero ? 96 : 64);
   }
+  __host__ __device__ int block_bytes() const { return 4 * quarter_bytes(); }
 };
 
 inline Shape shape_of(int group, int flags) {
@@ -50,8 +54,9 @@ inline Shape shape_of(int group, int flags) {
 inline bool group_ok(int group) { return group == 32 || group == 64 || group == 128; }
 __host__ __device__ inline int64_t blocks_of(int64_t k) { return (k + kBlockK - 1) / kBlockK; }
 
+// Place of a quarter's row among its scales.
 __host__ __device__ __forceinline__ int scale_place(int row) {
-  return (row & ~31) | ((row & 7) << 2) | ((row >> 3) & 3);
+  return ((row & 7) << 2) | ((row >> 3) & 3);
 }
 
 __device__ __forceinline__ float scale_f32(uint16_t bits, int half_scale) {
@@ -68,10 +73,11 @@ __device__ __forceinline__ uint32_t zero_pair(uint32_t z) { return 0x43004300u |
 __device__ __forceinline__ void decode8(uint32_t word, uint32_t zpair, uint32_t (&out)[4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t v = ((word >> (4 * i)) & 0x000f000fu) | 0x43004300u;
-    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&v),
-                                     *reinterpret_cast<const __nv_bfloat162 *>(&zpair));
-    out[i] = *reinterpret_cast<const uint32_t *>(&d);
+    uint32_t v;  // (shifted & 0x000f000f) | 0x43004300 in one instruction
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;"
+        : "=r"(v)
+        : "r"(word >> (4 * i)), "r"(0x000f000fu), "r"(0x43004300u));
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(out[i]) : "r"(v), "r"(zpair));
   }
 }
 

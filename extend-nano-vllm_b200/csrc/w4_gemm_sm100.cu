@@ -270,7 +270,7 @@ struct Ctx {
   uint32_t w_full, w_empty, b_full, a_full, ab_empty, d_full, d_empty, red_full, red_empty;
   uint32_t tmem;
   volatile int *abort;
-  int wbytes, scale_off, zero_off;
+  int wbytes, qbytes, scale_off, zero_off;
   int items, first, step, kb0, kb1;
   int rank, split;
 };
@@ -408,8 +408,7 @@ template <int NT, int GPB, int KIND>
 __device__ __forceinline__ void decode(const Args &args, const Ctx &c, int grp, int q) {
   using C = Cfg<NT>;
   const int lane = threadIdx.x & 31;
-  const int row = q * 32 + lane;
-  const int place = w4::scale_place(row);
+  const int place = w4::scale_place(lane);
   const bool zeros = args.sh.has_zero != 0;
   const uint32_t tq = c.tmem + C::D_COLS + (static_cast<uint32_t>(q * 32) << 16);
   Ring w, a;
@@ -423,20 +422,20 @@ __device__ __forceinline__ void decode(const Args &args, const Ctx &c, int grp, 
 #pragma unroll C::UNROLL
       for (; kb < c.kb1; kb += C::DG) {
         if (!wait(c.w_full + 8 * w.stage, w.phase, c.abort)) return;
-        const uint32_t st = c.s_w + w.stage * c.wbytes;
+        const uint32_t st = c.s_w + w.stage * c.wbytes + q * c.qbytes;
         uint32_t code[16];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                        : "=r"(code[4 * i]), "=r"(code[4 * i + 1]), "=r"(code[4 * i + 2]),
                          "=r"(code[4 * i + 3])
-                       : "r"(st + i * 2048 + row * 16));
+                       : "r"(st + i * 512 + lane * 16));
         uint32_t zp[GPB];
 #pragma unroll
         for (int g = 0; g < GPB; ++g) {
           uint32_t z = 8;
           if (zeros)
-            asm volatile("ld.shared.u8 %0, [%1];" : "=r"(z) : "r"(st + c.zero_off + g * 128 + place));
+            asm volatile("ld.shared.u8 %0, [%1];" : "=r"(z) : "r"(st + c.zero_off + g * 32 + place));
           zp[g] = w4::zero_pair(z);
         }
         if (!wait(c.ab_empty + 8 * a.stage, a.phase ^ 1, c.abort)) return;
@@ -493,7 +492,7 @@ __device__ __forceinline__ void promote(const Args &args, const Ctx &c, int half
         for (int j = 0; j < C::C / 2; ++j) acc2[i][j] = 0;
 #pragma unroll C::UNROLL
       for (int kb = c.kb0; kb < c.kb1; ++kb) {
-        const uint32_t scales = c.s_w + w.stage * c.wbytes + c.scale_off + w4::scale_place(row) * 2;
+        const uint32_t scales = c.s_w + w.stage * c.wbytes + q * c.qbytes + c.scale_off + w4::scale_place(lane) * 2;
 #pragma unroll
         for (int g = 0; g < GPB; ++g) {
           // A finished product implies the codes and scales of its stage: the
@@ -502,7 +501,7 @@ __device__ __forceinline__ void promote(const Args &args, const Ctx &c, int half
             return;
           tc_fence_after();
           uint16_t bits;
-          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(bits) : "r"(scales + g * 256));
+          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(bits) : "r"(scales + g * 64));
           const float s = w4::scale_f32(bits, args.sh.half_scale);
           const uint64_t s2 = pack2(s, s);
           const uint32_t td = tq + d.stage * NT + half * C::C;
@@ -658,6 +657,7 @@ __global__ void __launch_bounds__(Cfg<NT>::THREADS, 1)
   const int split = args.split;
   Ctx c;
   c.wbytes = args.sh.block_bytes();
+  c.qbytes = args.sh.quarter_bytes();
   c.scale_off = args.sh.scale_off();
   c.zero_off = args.sh.zero_off();
   uint8_t *s_w = smem + C::BS * C::B_BYTES;

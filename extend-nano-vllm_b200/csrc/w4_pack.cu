@@ -25,7 +25,8 @@ __global__ void __launch_bounds__(w4::kTileRows) w4_pack_kernel(
     valid = src < rows;
   }
   const int64_t groups = k / sh.group;
-  const int place = w4::scale_place(row);
+  const int place = w4::scale_place(row & 31);
+  uint8_t *quarter = block + (row >> 5) * sh.quarter_bytes();
   const uint8_t *crow = codes + (mat * rows + src) * k;
   uint32_t word[4][4];  // [unit][chunk of 32 k]
 #pragma unroll
@@ -48,16 +49,16 @@ __global__ void __launch_bounds__(w4::kTileRows) w4_pack_kernel(
   }
 #pragma unroll
   for (int u = 0; u < 4; ++u)
-    *reinterpret_cast<uint4 *>(block + u * 2048 + row * 16) =
+    *reinterpret_cast<uint4 *>(quarter + u * 512 + (row & 31) * 16) =
         make_uint4(word[u][0], word[u][1], word[u][2], word[u][3]);
   for (int g = 0; g < sh.groups_per_block(); ++g) {
     const int64_t gi = kb * sh.groups_per_block() + g;
     const bool in = valid && gi < groups;
     const int64_t at = (mat * rows + src) * groups + gi;
-    reinterpret_cast<uint16_t *>(block + sh.scale_off())[g * w4::kTileRows + place] =
+    reinterpret_cast<uint16_t *>(quarter + sh.scale_off())[g * 32 + place] =
         in ? scales[at] : static_cast<uint16_t>(0);
     if (sh.has_zero)
-      block[sh.zero_off() + g * w4::kTileRows + place] =
+      quarter[sh.zero_off() + g * 32 + place] =
           in ? static_cast<uint8_t>(zeros[at] & 15) : static_cast<uint8_t>(0);
   }
 }

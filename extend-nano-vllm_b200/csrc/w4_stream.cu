@@ -5,11 +5,11 @@
 //   D_g[f, r] = sum_{k in group g} (q[f, k] - z[f, g]) * x[r, k]
 //   y[r, f]   = sum_g s[f, g] * D_g[f, r]
 //
-// Each warp streams its own weights, global memory -> registers -> integers
-// q - z (exact in bf16) -> warp matrix instructions (m16n8k16: 16 weight rows,
-// 8 rows of x), and adds a group's sum to fp32 registers times its scale.  No
-// shared memory, no barrier and no second warp is on the way of a weight, which
-// is what a stream of 4-bit weights needs: at the copy rate an SM has some 23
+// Each warp streams its own weights (asynchronous copies into a ring of its own)
+// -> registers -> integers q - z (exact in bf16) -> warp matrix instructions
+// (m16n8k16: 16 weight rows, 8 rows of x), and adds a group's sum to fp32
+// registers times its scale.  No barrier and no second warp is on the way of a
+// weight, which is what a stream of 4-bit weights needs: at the copy rate an SM has some 23
 // cycles for 512 codes, and the decoding alone takes 7 of each scheduler's.
 // (tcgen05 wants the operand decoded by one warp, waited for by another and
 // read back by a third; that pays from more than 16 rows on, w4_gemm_sm100.cu.)
@@ -79,55 +79,123 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// One block's share of a lane: 16 bytes of rows g, g + 8, ... (two per operand
-// of 16 rows), and those rows' scales and zero points.
-template <int GPB>
-struct Block {
-  uint4 codes[4];
-  uint2 scale[GPB];     // four of 16 bits
-  uint32_t zero[GPB];   // four of 8 bits
+// Blocks on their way: each warp has a ring of its own in shared memory, filled
+// by bulk copies (one per block and warp), so that six kilobytes per warp are
+// in flight however few registers are left.
+constexpr int kDepth = 4;
 
-  __device__ __forceinline__ void load(const uint8_t *block, int quarter, int g, int t,
-                                       bool zeros) {
-    const uint8_t *c = block + t * 2048 + (quarter * 32 + g) * 16;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) codes[i] = load_codes(c + i * 128);
-    const uint8_t *s = block + w4::kCodeBytes + (quarter * 32 + 4 * g) * 2;
-#pragma unroll
-    for (int j = 0; j < GPB; ++j) scale[j] = __ldg(reinterpret_cast<const uint2 *>(s + j * 256));
-    if (zeros) {
-      const uint8_t *z = block + w4::kCodeBytes + GPB * 256 + quarter * 32 + 4 * g;
-#pragma unroll
-      for (int j = 0; j < GPB; ++j) zero[j] = __ldg(reinterpret_cast<const uint32_t *>(z + j * 128));
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes,
+                                          uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          dst),
+      "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
+
+// Waits for a copy: bounded, and without a timer on the way of a satisfied wait.
+__device__ __forceinline__ bool wait_copy(uint32_t bar, uint32_t parity) {
+  if (__builtin_expect(mbar_try_wait(bar, parity), 1)) return true;
+  int64_t start = 0;
+  for (uint32_t tries = 1;; ++tries) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((tries & 1023u) == 0) {
+      const int64_t now = clock64();
+      if (start == 0) {
+        start = now;
+      } else if (now - start > 4000000000ll) {
+        atomicOr(&g_status, kStatusTimeout);
+        return false;
+      }
     }
   }
-  // Scale and zero of row g + 8 i.
-  __device__ __forceinline__ float scale_of(int j, int i, int half_scale) const {
-    const uint32_t v = i < 2 ? scale[j].x : scale[j].y;
-    return w4::scale_f32(static_cast<uint16_t>((i & 1) ? v >> 16 : v & 0xffffu), half_scale);
+}
+
+// One block's share of a lane: 16 bytes of rows g, g + 8, ... (two per operand
+// of 16 rows), and those rows' scales and zero points.
+template <int GPB, bool ZEROS>
+struct Block {
+  uint4 codes[4];
+  uint2 scale[GPB];    // four of 16 bits
+  uint32_t zero[GPB];  // four of 8 bits
+
+  __device__ __forceinline__ void read(uint32_t stage, int lane) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(codes[i].x), "=r"(codes[i].y), "=r"(codes[i].z), "=r"(codes[i].w)
+                   : "r"(stage + (lane & 3) * 512 + (lane >> 2) * 16 + i * 128));
+    const int g = lane >> 2;
+#pragma unroll
+    for (int j = 0; j < GPB; ++j)
+      asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
+                   : "=r"(scale[j].x), "=r"(scale[j].y)
+                   : "r"(stage + w4::kCodeBytes + j * 64 + g * 8));
+    if (ZEROS) {
+#pragma unroll
+      for (int j = 0; j < GPB; ++j)
+        asm volatile("ld.shared.u32 %0, [%1];"
+                     : "=r"(zero[j])
+                     : "r"(stage + w4::kCodeBytes + GPB * 64 + j * 32 + g * 4));
+    }
   }
-  __device__ __forceinline__ uint32_t zpair_of(int j, int i, bool zeros) const {
-    return w4::zero_pair(zeros ? (zero[j] >> (8 * i)) & 15u : 8u);
+  // Scales of rows g, g + 8, g + 16, g + 24.
+  __device__ __forceinline__ void scales(int j, bool half_scale, float (&s)[4]) const {
+    if (__builtin_expect(half_scale, 0)) {
+      const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&scale[j].x));
+      const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&scale[j].y));
+      s[0] = a.x, s[1] = a.y, s[2] = b.x, s[3] = b.y;
+    } else {
+      s[0] = __uint_as_float(scale[j].x << 16), s[1] = __uint_as_float(scale[j].x & 0xffff0000u);
+      s[2] = __uint_as_float(scale[j].y << 16), s[3] = __uint_as_float(scale[j].y & 0xffff0000u);
+    }
+  }
+  // Of row g + 8 i: the bytes z and 0x43 twice, 128 + z in both halves.
+  __device__ __forceinline__ uint32_t zpair(int j, int i) const {
+    return ZEROS ? __byte_perm(zero[j], 0x43434343u, 0x4040 | (i << 8) | i) : 0x43084308u;
   }
 };
 
-// Adds one block to tot[operand][column tile][4].  xp[n]: this lane's eight k
-// of chunk 0 of row 8 n + g, null for a row that is not there.
-template <int GPB, int NB>
-__device__ __forceinline__ void add_block(const Block<GPB> &b, int half_scale, bool zeros,
-                                          const __nv_bfloat16 *const (&xp)[NB], int k0, int k,
-                                          float (&tot)[2][NB][4]) {
+// In program order: the compiler would move a load that is asked for early to
+// where it is used.
+__device__ __forceinline__ uint4 load_row(const __nv_bfloat16 *p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
+
+// This lane's k of one block of its rows of x.  xp[n]: its eight k of chunk 0
+// of row 8 n + g (of some other row where there are fewer; its sums are not
+// stored).
+template <int NB>
+__device__ __forceinline__ void read_rows(uint4 (&xv)[4][NB], const __nv_bfloat16 *const (&xp)[NB],
+                                          int k0, int k) {
+  if (__builtin_expect(k0 + w4::kBlockK <= k, 1)) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+        xv[c][n] = load_row(xp[n] + k0 + 32 * c);
+  } else {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+        xv[c][n] = k0 + 32 * c < k ? load_row(xp[n] + k0 + 32 * c) : make_uint4(0, 0, 0, 0);
+  }
+}
+
+// Adds one block to tot[operand][column tile][4].
+template <int GPB, int NB, bool ZEROS>
+__device__ __forceinline__ void add_block(const Block<GPB, ZEROS> &b, bool half_scale,
+                                          const uint4 (&xv)[4][NB], float (&tot)[2][NB][4]) {
 #pragma unroll
   for (int j = 0; j < GPB; ++j) {
-    uint4 xv[4 / GPB][NB];
-#pragma unroll
-    for (int cc = 0; cc < 4 / GPB; ++cc)
-#pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        const int at = k0 + 32 * (j * (4 / GPB) + cc);
-        xv[cc][n] = xp[n] != nullptr && at < k ? *reinterpret_cast<const uint4 *>(xp[n] + at)
-                                               : make_uint4(0, 0, 0, 0);
-      }
+    float s[4];
+    b.scales(j, half_scale, s);
     float acc[2][NB][4];
 #pragma unroll
     for (int m = 0; m < 2; ++m)
@@ -137,7 +205,7 @@ __device__ __forceinline__ void add_block(const Block<GPB> &b, int half_scale, b
         for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.f;
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-      const uint32_t z0 = b.zpair_of(j, 2 * m, zeros), z1 = b.zpair_of(j, 2 * m + 1, zeros);
+      const uint32_t z0 = b.zpair(j, 2 * m), z1 = b.zpair(j, 2 * m + 1);
 #pragma unroll
       for (int cc = 0; cc < 4 / GPB; ++cc) {
         const int c = j * (4 / GPB) + cc;
@@ -146,17 +214,16 @@ __device__ __forceinline__ void add_block(const Block<GPB> &b, int half_scale, b
         w4::decode8(word(b.codes[2 * m + 1], c), z1, hi);
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-          mma(acc[m][n], lo[0], hi[0], lo[1], hi[1], xv[cc][n].x, xv[cc][n].y);
-          mma(acc[m][n], lo[2], hi[2], lo[3], hi[3], xv[cc][n].z, xv[cc][n].w);
+          mma(acc[m][n], lo[0], hi[0], lo[1], hi[1], xv[c][n].x, xv[c][n].y);
+          mma(acc[m][n], lo[2], hi[2], lo[3], hi[3], xv[c][n].z, xv[c][n].w);
         }
       }
-      const float s0 = b.scale_of(j, 2 * m, half_scale), s1 = b.scale_of(j, 2 * m + 1, half_scale);
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
-        tot[m][n][0] = fmaf(s0, acc[m][n][0], tot[m][n][0]);
-        tot[m][n][1] = fmaf(s0, acc[m][n][1], tot[m][n][1]);
-        tot[m][n][2] = fmaf(s1, acc[m][n][2], tot[m][n][2]);
-        tot[m][n][3] = fmaf(s1, acc[m][n][3], tot[m][n][3]);
+        tot[m][n][0] = fmaf(s[2 * m], acc[m][n][0], tot[m][n][0]);
+        tot[m][n][1] = fmaf(s[2 * m], acc[m][n][1], tot[m][n][1]);
+        tot[m][n][2] = fmaf(s[2 * m + 1], acc[m][n][2], tot[m][n][2]);
+        tot[m][n][3] = fmaf(s[2 * m + 1], acc[m][n][3], tot[m][n][3]);
       }
     }
   }
@@ -164,7 +231,7 @@ __device__ __forceinline__ void add_block(const Block<GPB> &b, int half_scale, b
 
 // A work item of a warp: a quarter of a tile, against the rows of one row tile.
 struct Item {
-  const uint8_t *w;  // the tile's first block
+  const uint8_t *w;  // its quarter of the tile's first block
   int rb, rows;
   int tile, quarter;
 };
@@ -193,7 +260,8 @@ __device__ __forceinline__ Item item_of(const Args &a, int it) {
     r.rb = t[1];
     r.rows = t[2] - t[1];
   }
-  r.w = a.w + (static_cast<int64_t>(e) * a.n_blocks + r.tile) * a.num_kb * a.sh.block_bytes();
+  r.w = a.w + (static_cast<int64_t>(e) * a.n_blocks + r.tile) * a.num_kb * a.sh.block_bytes() +
+        r.quarter * a.sh.quarter_bytes();
   return r;
 }
 
@@ -232,10 +300,13 @@ __device__ __forceinline__ void store(const Args &a, const Item &it, int r0, int
 }
 
 // NB * 8 rows of x at a time.
-template <int GPB, int KIND, int NB>
+template <int GPB, int KIND, int NB, bool ZEROS>
 __global__ void __launch_bounds__(32 * kWarps, 2) w4_stream_kernel(
     const __grid_constant__ Args a) {
+  extern __shared__ __align__(16) uint8_t ring_smem[];  // [kWarps][kDepth] quarter blocks
   __shared__ float red[kWarps][2 * NB * 4][32];
+  __shared__ uint64_t bars[kWarps][kDepth];
+  constexpr int kStage = w4::kCodeBytes + GPB * (ZEROS ? 96 : 64);
   pdl_trigger();
   const int lane = threadIdx.x & 31;
   const int warp = threadIdx.x >> 5;
@@ -243,8 +314,14 @@ __global__ void __launch_bounds__(32 * kWarps, 2) w4_stream_kernel(
   const int wk = a.wk;
   const int wr = kWarps / wk;  // items of a thread block at a time
   const int part = warp / wr;
-  const bool zeros = a.sh.has_zero != 0;
-  const int bytes = a.sh.block_bytes();
+  const bool half_scale = a.sh.half_scale != 0;
+  const uint32_t ring = smem_u32(ring_smem) + warp * (kDepth * kStage);
+  const uint32_t full = smem_u32(bars[warp]);
+  if (lane == 0) {
+    for (int i = 0; i < kDepth; ++i) mbar_init(full + 8 * i, 1);
+    fence_mbar_init();
+  }
+  __syncwarp();
   if (KIND != kLinear) pdl_wait();
   const int mt = KIND == kLinear ? 1
                  : KIND == kGateUp && a.ids != nullptr
@@ -252,38 +329,47 @@ __global__ void __launch_bounds__(32 * kWarps, 2) w4_stream_kernel(
                      : static_cast<int>(min64(a.counters[B200MOE_CNT_MTILES], a.max_mtiles));
   const int items = mt * 4 * a.n_blocks;
   const int stride = gridDim.x * wr;
-  int cur = blockIdx.x * wr + warp % wr;
+  const int begin = blockIdx.x * wr + warp % wr;
+
+  // Where the copies are: they run kDepth - 1 blocks ahead of the products,
+  // into the next items too.
+  const uint8_t *src = nullptr, *src_next = nullptr;
+  int src_item = begin, src_kb = a.num_kb, src_left = 0, src_stage = 0;
+  auto copy_next = [&]() {
+    if (__builtin_expect(src_kb >= a.num_kb, 0)) {  // the next pass over the item, or the next item
+      while (src_left == 0 && src_item < items) {
+        const Item n = item_of<KIND>(a, src_item);
+        src_item += stride;
+        src = n.w + static_cast<int64_t>(part) * (4 * kStage);
+        src_left = (n.rows + 8 * NB - 1) / (8 * NB);
+      }
+      if (src_left == 0) return;
+      --src_left;
+      src_kb = part;
+      src_next = src;
+    }
+    if (lane == 0) {
+      mbar_arrive_expect_tx(full + 8 * src_stage, kStage);
+      bulk_load(ring + src_stage * kStage, src_next, kStage, full + 8 * src_stage);
+    }
+    src_next += static_cast<int64_t>(wk) * (4 * kStage);
+    src_kb += wk;
+    src_stage = (src_stage + 1) % kDepth;
+  };
+#pragma unroll 1
+  for (int i = 0; i < kDepth - 1; ++i) copy_next();
+  if (KIND == kLinear) pdl_wait();  // codes are constant, x is not
+  int stage = 0;
+  uint32_t phase = 0;
+
   // All warps of a block take the same number of turns (they meet when k is
   // shared); a turn past the end does nothing.
-  Block<GPB> next;
-  Item it = {};
-  if (cur < items) {
-    it = item_of<KIND>(a, cur);
-    next.load(it.w + static_cast<int64_t>(part) * bytes, it.quarter, g, t, zeros);
-  }
-  if (KIND == kLinear) pdl_wait();  // codes are constant, x is not
+  int cur = begin;
   for (int turn = blockIdx.x * wr; turn < items; turn += stride, cur += stride) {
-    const bool live = cur < items;
-    const bool more = cur + stride < items;
-    Item following = it;
-    if (more) following = item_of<KIND>(a, cur + stride);
-    const int rows = live ? it.rows : 0;
+    Item it = {};
+    if (cur < items) it = item_of<KIND>(a, cur);
+    const int rows = it.rows;
     for (int r0 = 0; r0 < rows || (r0 == 0 && wk > 1); r0 += 8 * NB) {
-      const __nv_bfloat16 *xp[NB];
-#pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        const int col = r0 + 8 * n + g;
-        xp[n] = nullptr;
-        if (col < rows) {
-          int64_t row = it.rb + col;
-          if (KIND == kGateUp && a.gather)
-            row = a.ids != nullptr
-                      ? row / a.top_k
-                      : gather_token(row, it.rb + it.rows, a.row_route, nullptr, a.top_k,
-                                     a.num_routes, a.x_rows);
-          xp[n] = static_cast<const __nv_bfloat16 *>(a.x) + row * a.k + 8 * t;
-        }
-      }
       float tot[2][NB][4];
 #pragma unroll
       for (int m = 0; m < 2; ++m)
@@ -291,23 +377,41 @@ __global__ void __launch_bounds__(32 * kWarps, 2) w4_stream_kernel(
         for (int n = 0; n < NB; ++n)
 #pragma unroll
           for (int j = 0; j < 4; ++j) tot[m][n][j] = 0.f;
-      const bool last = r0 + 8 * NB >= rows;
-      if (live) {
-        for (int kb = part; kb < a.num_kb; kb += wk) {
-          const Block<GPB> now = next;
-          // The next block, or the first of this warp's next turn.
-          const uint8_t *from = nullptr;
-          int quarter = it.quarter;
-          if (kb + wk < a.num_kb) {
-            from = it.w + static_cast<int64_t>(kb + wk) * bytes;
-          } else if (!last) {
-            from = it.w + static_cast<int64_t>(part) * bytes;
-          } else if (more) {
-            from = following.w + static_cast<int64_t>(part) * bytes;
-            quarter = following.quarter;
+      if (rows > 0) {
+        const __nv_bfloat16 *xp[NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          const int col = r0 + 8 * n + g < rows ? r0 + 8 * n + g : 0;
+          int64_t row = it.rb + col;
+          if (KIND == kGateUp && a.gather)
+            row = a.ids != nullptr ? row / a.top_k
+                                   : gather_token(row, it.rb + it.rows, a.row_route, nullptr,
+                                                  a.top_k, a.num_routes, a.x_rows);
+          xp[n] = static_cast<const __nv_bfloat16 *>(a.x) + row * a.k + 8 * t;
+        }
+        // The rows of x come from L2 and are asked for one block ahead; with
+        // two column tiles there is no room for that.
+        uint4 xv[NB == 1 ? 2 : 1][4][NB];
+        if (NB == 1) read_rows(xv[0], xp, part * w4::kBlockK, a.k);
+        auto step = [&](int kb, uint4 (&now)[4][NB], uint4 (&next)[4][NB]) {
+          const bool arrived = wait_copy(full + 8 * stage, phase);
+          Block<GPB, ZEROS> b;
+          b.read(ring + stage * kStage, lane);
+          __syncwarp();  // every lane is done with the stage before, which is filled next
+          copy_next();
+          if (NB == 1) {
+            if (kb + wk < a.num_kb) read_rows(next, xp, (kb + wk) * w4::kBlockK, a.k);
+          } else {
+            read_rows(now, xp, kb * w4::kBlockK, a.k);
           }
-          if (from != nullptr) next.load(from, quarter, g, t, zeros);
-          add_block<GPB, NB>(now, a.sh.half_scale, zeros, xp, kb * w4::kBlockK, a.k, tot);
+          stage = (stage + 1) % kDepth;
+          phase ^= stage == 0 ? 1u : 0u;
+          if (arrived) add_block<GPB, NB, ZEROS>(b, half_scale, now, tot);
+        };
+#pragma unroll 1
+        for (int kb = part; kb < a.num_kb; kb += 2 * wk) {
+          step(kb, xv[0], xv[NB == 1 ? 1 : 0]);
+          if (kb + wk < a.num_kb) step(kb + wk, xv[NB == 1 ? 1 : 0], xv[0]);
         }
       }
       if (wk == 1) {
@@ -335,12 +439,11 @@ __global__ void __launch_bounds__(32 * kWarps, 2) w4_stream_kernel(
             v1 += red[p * wr + warp % wr][NB * 4 + v][lane];
           }
           const int n = v >> 2, j = v & 3;
-          if (live)
+          if (rows > 0)
             store<KIND>(a, it, r0, g + (j >> 1) * 8, 8 * n + 2 * t + (j & 1), v0, v1);
         }
       }
     }
-    it = following;
   }
 }
 
@@ -368,7 +471,7 @@ __global__ void __launch_bounds__(32 * kWarps) w4_down_slots_kernel(
     const bool live = e >= 0 && e < num_experts;
     float tot[4] = {0.f, 0.f, 0.f, 0.f};
     if (live) {
-      const uint8_t *w = w2 + (e * tiles + tile) * num_kb * bytes;
+      const uint8_t *w = w2 + (e * tiles + tile) * num_kb * bytes + quarter * sh.quarter_bytes();
       const __nv_bfloat16 *x = act + route * inter + 8 * t;
       for (int kb0 = 0; kb0 < num_kb; kb0 += BATCH) {
         uint4 codes[BATCH][2];
@@ -378,16 +481,16 @@ __global__ void __launch_bounds__(32 * kWarps) w4_down_slots_kernel(
         for (int b = 0; b < BATCH; ++b)
           if (kb0 + b < num_kb) {
             const uint8_t *block = w + static_cast<int64_t>(kb0 + b) * bytes;
-            const uint8_t *c = block + t * 2048 + (quarter * 32 + op * 16 + g) * 16;
+            const uint8_t *c = block + t * 512 + (op * 16 + g) * 16;
             codes[b][0] = load_codes(c);
             codes[b][1] = load_codes(c + 128);
-            const uint8_t *sc = block + w4::kCodeBytes + (quarter * 32 + 4 * g + 2 * op) * 2;
+            const uint8_t *sc = block + w4::kCodeBytes + (4 * g + 2 * op) * 2;
 #pragma unroll
             for (int j = 0; j < GPB; ++j) {
-              scale[b][j] = __ldg(reinterpret_cast<const uint32_t *>(sc + j * 256));
+              scale[b][j] = __ldg(reinterpret_cast<const uint32_t *>(sc + j * 64));
               if (zeros)
                 zero[b][j] = __ldg(reinterpret_cast<const uint16_t *>(
-                    block + w4::kCodeBytes + GPB * 256 + j * 128 + quarter * 32 + 4 * g + 2 * op));
+                    block + w4::kCodeBytes + GPB * 64 + j * 32 + 4 * g + 2 * op));
             }
           }
 #pragma unroll
@@ -434,10 +537,18 @@ __global__ void __launch_bounds__(32 * kWarps) w4_down_slots_kernel(
   }
 }
 
-template <int GPB, int KIND, int NB>
+template <int GPB, int KIND, int NB, bool ZEROS>
 int launch(const Args &a, int64_t blocks, cudaStream_t s) {
-  B200_LAUNCH_PDL(kPdlStream, w4_stream_kernel<GPB, KIND, NB>, dim3(static_cast<unsigned>(blocks)),
-                  dim3(32 * kWarps), 0, s, a);
+  constexpr int smem = kWarps * kDepth * (w4::kCodeBytes + GPB * (ZEROS ? 96 : 64));
+  static bool done[64] = {false};
+  const int dev = current_device();
+  if (!(dev >= 0 && dev < 64 && done[dev])) {
+    B200_CUDA(cudaFuncSetAttribute(w4_stream_kernel<GPB, KIND, NB, ZEROS>,
+                                   cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (dev >= 0 && dev < 64) done[dev] = true;
+  }
+  B200_LAUNCH_PDL(kPdlStream, w4_stream_kernel<GPB, KIND, NB, ZEROS>, dim3(static_cast<unsigned>(blocks)),
+                  dim3(32 * kWarps), smem, s, a);
   B200_LAUNCHED();
   return B200MOE_OK;
 }
@@ -465,7 +576,11 @@ int run(Args a, double items, int64_t most, int64_t rows, cudaStream_t s) {
   if (blocks > slots) blocks = slots;
   if (blocks < 1) blocks = 1;
 #define B200_W4S(G)                                                         \
-  return nb == 1 ? launch<G, KIND, 1>(a, blocks, s) : launch<G, KIND, 2>(a, blocks, s);
+  if (a.sh.has_zero)                                                        \
+    return nb == 1 ? launch<G, KIND, 1, true>(a, blocks, s)                 \
+                   : launch<G, KIND, 2, true>(a, blocks, s);                \
+  return nb == 1 ? launch<G, KIND, 1, false>(a, blocks, s)                  \
+                 : launch<G, KIND, 2, false>(a, blocks, s);
   switch (a.sh.groups_per_block()) {
     case 1: B200_W4S(1)
     case 2: B200_W4S(2)
