@@ -92,6 +92,7 @@ SIGNATURES: dict[str, tuple] = {
     "b200moe_w4_pack": (_I, [_P, _P, _P, _L, _L, _L, _I, _I, _P, _P]),
     "b200moe_w4_linear": (_I, [_P, _L, _I, _I, _P, _I, _I, _P, _P]),
     "b200moe_w4_experts_workspace": (_L, [_L, _I, _I, _I, _I]),
+    "b200moe_w4_experts_launches": (_I, [_L, _I, _I]),
     "b200moe_w4_experts": (_I, [_P, _L, _I, _I, _P, _P, _I, _I, _P, _I, _I, _P, _I, _I, _P, _L,
                                 _P, _P]),
 }
@@ -153,6 +154,8 @@ def _kernels_launched(name: str, args: tuple) -> int:
         return 1 if int(args[2]) <= PACK_SINGLE_LAUNCH_ROUTES else 2
     if name == "b200moe_nvl_receive":
         return 2
+    if name == "b200moe_w4_experts":
+        return int(LIB.b200moe_w4_experts_launches(int(args[1]), int(args[6]), int(args[7])))
     return 1
 
 

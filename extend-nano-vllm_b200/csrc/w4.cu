@@ -15,10 +15,12 @@ int w4_down_stream(const void *act, int hidden, int inter, const void *w2, const
                    const int32_t *row_route, const void *route_weights, int64_t num_routes,
                    const int32_t *mtiles, int64_t max_mtiles, const int32_t *counters,
                    double tiles, int64_t rows, float *y, cudaStream_t s);
-int w4_route_experts(const void *x, int64_t tokens, int hidden, int inter, const int64_t *ids,
-                     const void *weights, int top_k, int num_experts, const void *w13,
-                     const w4::Shape &sh13, const void *w2, const w4::Shape &sh2, void *act,
-                     void *out, cudaStream_t s);
+int w4_route_gate_up(const void *x, int64_t tokens, int hidden, int inter, const int64_t *ids,
+                     int top_k, int num_experts, const void *w13, const w4::Shape &sh, void *act,
+                     cudaStream_t s);
+int w4_route_down(const void *act, int64_t tokens, int hidden, int inter, const int64_t *ids,
+                  const void *weights, int top_k, int num_experts, const void *w2,
+                  const w4::Shape &sh2, void *out, cudaStream_t s);
 int w4_linear_tc(const void *x, int64_t m, int n, int k, const void *w, const w4::Shape &sh,
                  void *out, cudaStream_t s);
 int w4_gate_up_tc(const RowSource &src, int hidden, int inter, const void *w13,
@@ -54,6 +56,10 @@ struct Workspace {
   }
 };
 
+// Packing in one block: routes and experts it takes.
+constexpr int64_t kPackRoutes = 8192;
+constexpr int kPackExperts = 4096;
+
 struct ExpertBuffers {
   int64_t row_capacity = 0, max_mtiles = 0, scratch_bytes = 0;
   int32_t *row_route = nullptr, *route_row = nullptr, *combine_rows = nullptr,
@@ -76,25 +82,114 @@ ExpertBuffers expert_buffers(Workspace &ws, int64_t tokens, int hidden, int inte
   b.max_mtiles = b200moe_pack_max_mtiles(routes, num_experts);
   b.scratch_bytes = static_cast<int64_t>(b200moe_pack_scratch_bytes(routes, num_experts));
   b.row_route = ws.take<int32_t>(b.row_capacity);
-  b.route_row = ws.take<int32_t>(routes);
-  b.combine_rows = ws.take<int32_t>(routes);
-  b.tile_expert = ws.take<int32_t>(b.row_capacity / B200MOE_BLOCK_ROWS);
-  b.offsets = ws.take<int32_t>(num_experts + 1);
-  b.counts = ws.take<int32_t>(num_experts);
   b.mtiles = ws.take<int32_t>(b.max_mtiles * B200MOE_MTILE_WORDS);
   b.counters = ws.take<int32_t>(B200MOE_NUM_COUNTERS);
-  b.scratch = ws.take<int32_t>(b.scratch_bytes / 4);
+  if (routes > kPackRoutes || num_experts > kPackExperts) {
+    b.route_row = ws.take<int32_t>(routes);
+    b.combine_rows = ws.take<int32_t>(routes);
+    b.tile_expert = ws.take<int32_t>(b.row_capacity / B200MOE_BLOCK_ROWS);
+    b.offsets = ws.take<int32_t>(num_experts + 1);
+    b.counts = ws.take<int32_t>(num_experts);
+    b.scratch = ws.take<int32_t>(b.scratch_bytes / 4);
+  }
   if (routes > kGatherRoutes) b.x_packed = ws.take<__nv_bfloat16>(b.row_capacity * hidden);
   b.act = ws.take<__nv_bfloat16>(b.row_capacity * inter);
   b.y = ws.take<float>(routes * hidden);
   return b;
 }
 
-// out[t, :] = sum over slots, in slot order, of the fp32 route rows y (rows
-// that combine_rows does not name are not read).  One thread per 4 columns.
-__global__ void __launch_bounds__(256) w4_combine_kernel(const float *y, int64_t num_routes,
-                                                         const int32_t *combine_rows,
-                                                         int64_t tokens, int top_k, int hidden,
+// Packing for up to kPackRoutes routes in one block: rows by expert, every
+// expert's rows on a 16-row boundary, row tiles of 128.  The place of a route
+// among its expert's rows is whichever came first: a row's product does not
+// depend on its place, so results are the same whatever the order.
+constexpr int kPackThreads = 1024;
+
+__global__ void __launch_bounds__(kPackThreads) w4_pack_routes_kernel(
+    const int64_t *ids, int num_routes, int num_experts, int32_t *row_route, int32_t *mtiles,
+    int32_t *counters) {
+  extern __shared__ int32_t pack_smem[];  // count[E], first row[E], first tile[E]
+  __shared__ int32_t warp_rows[32], warp_tiles[32];
+  pdl_trigger();
+  pdl_wait();
+  int32_t *count = pack_smem, *row0 = count + num_experts, *tile0 = row0 + num_experts;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  for (int e = tid; e < num_experts; e += kPackThreads) count[e] = 0;
+  __syncthreads();
+  constexpr int kMost = kPackRoutes / kPackThreads;
+  int expert[kMost], place[kMost];
+#pragma unroll
+  for (int i = 0; i < kMost; ++i) {
+    const int r = tid + i * kPackThreads;
+    expert[i] = -1;
+    if (r < num_routes) {
+      const int64_t e = ids[r];
+      if (e >= 0 && e < num_experts) {
+        expert[i] = static_cast<int>(e);
+        place[i] = atomicAdd(&count[e], 1);
+      }
+    }
+  }
+  __syncthreads();
+  // Rows and tiles before each expert; thread t takes `per` experts in a row.
+  const int per = (num_experts + kPackThreads - 1) / kPackThreads;
+  int rows = 0, tiles = 0;
+  for (int i = 0; i < per; ++i) {
+    const int e = tid * per + i;
+    if (e < num_experts) {
+      rows += (count[e] + 15) & ~15;
+      tiles += (count[e] + B200MOE_MTILE_ROWS - 1) / B200MOE_MTILE_ROWS;
+    }
+  }
+  int rows_in = rows, tiles_in = tiles;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int r = __shfl_up_sync(0xffffffffu, rows_in, off);
+    const int t = __shfl_up_sync(0xffffffffu, tiles_in, off);
+    if (lane >= off) {
+      rows_in += r;
+      tiles_in += t;
+    }
+  }
+  if (lane == 31) {
+    warp_rows[warp] = rows_in;
+    warp_tiles[warp] = tiles_in;
+  }
+  __syncthreads();
+  int row = rows_in - rows, tile = tiles_in - tiles;
+  for (int w = 0; w < warp; ++w) {
+    row += warp_rows[w];
+    tile += warp_tiles[w];
+  }
+  if (tid == kPackThreads - 1) {
+    counters[B200MOE_CNT_PADDED_ROWS] = row + rows;
+    counters[B200MOE_CNT_MTILES] = tile + tiles;
+  }
+  for (int i = 0; i < per; ++i) {
+    const int e = tid * per + i;
+    if (e < num_experts) {
+      const int n = count[e];
+      row0[e] = row;
+      for (int r = 0; r < n; r += B200MOE_MTILE_ROWS, ++tile) {
+        mtiles[tile * B200MOE_MTILE_WORDS + 0] = e;
+        mtiles[tile * B200MOE_MTILE_WORDS + 1] = row + r;
+        mtiles[tile * B200MOE_MTILE_WORDS + 2] = row + min(n, r + B200MOE_MTILE_ROWS);
+      }
+      // The rows that fill an expert's last sixteen belong to no route.
+      for (int r = n; r < ((n + 15) & ~15); ++r) row_route[row + r] = num_routes;
+      row += (n + 15) & ~15;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kMost; ++i)
+    if (expert[i] >= 0) row_route[row0[expert[i]] + place[i]] = tid + i * kPackThreads;
+}
+
+// out[t, :] = sum over slots, in slot order, of the fp32 route rows y (rows of
+// routes whose id is no expert are not read).  One thread per 4 columns.
+__global__ void __launch_bounds__(256) w4_combine_kernel(const float *y, const int64_t *ids,
+                                                         int num_experts, int64_t tokens,
+                                                         int top_k, int hidden,
                                                          __nv_bfloat16 *__restrict__ out) {
   pdl_trigger();
   pdl_wait();
@@ -103,21 +198,23 @@ __global__ void __launch_bounds__(256) w4_combine_kernel(const float *y, int64_t
   const int64_t token = idx / vecs;
   const int col = static_cast<int>(idx - token * vecs) * 4;
   if (token >= tokens) return;
+  const float *row = y + token * top_k * hidden + col;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s0 = 0; s0 < top_k; s0 += 4) {
-    // Four slots' row numbers, then their rows, are in flight together.
-    int64_t row[4];
-    float4 v[4];
+  for (int s0 = 0; s0 < top_k; s0 += 8) {
+    // Eight slots' ids and rows are in flight together.
+    bool live[8];
+    float4 v[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      row[j] = s0 + j < top_k ? combine_rows[token * top_k + s0 + j] : num_routes;
+    for (int j = 0; j < 8; ++j) {
+      const int64_t id = s0 + j < top_k ? ids[token * top_k + s0 + j] : -1;
+      live[j] = id >= 0 && id < num_experts;
+    }
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (row[j] >= 0 && row[j] < num_routes)
-        v[j] = *reinterpret_cast<const float4 *>(y + row[j] * hidden + col);
+    for (int j = 0; j < 8; ++j)
+      if (live[j]) v[j] = *reinterpret_cast<const float4 *>(row + (s0 + j) * static_cast<int64_t>(hidden));
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (row[j] >= 0 && row[j] < num_routes) {
+    for (int j = 0; j < 8; ++j)
+      if (live[j]) {
         acc.x += v[j].x;
         acc.y += v[j].y;
         acc.z += v[j].z;
@@ -161,6 +258,15 @@ int64_t b200moe_w4_experts_workspace(int64_t tokens, int hidden, int inter, int 
   return ws.bytes;
 }
 
+int b200moe_w4_experts_launches(int64_t tokens, int top_k, int num_experts) {
+  using namespace b200moe;
+  const int64_t routes = tokens * top_k;
+  if (routes <= 0) return 0;
+  if (routes <= kRouteRoutes) return 2;
+  return (routes <= kPackRoutes && num_experts <= kPackExperts ? 1 : 2) +
+         (routes > kGatherRoutes ? 1 : 0) + 3;
+}
+
 int b200moe_w4_experts(const void *x, int64_t tokens, int hidden, int inter,
                        const int64_t *expert_ids, const void *weights, int top_k, int num_experts,
                        const void *w13, int group13, int flags13, const void *w2, int group2,
@@ -189,16 +295,33 @@ int b200moe_w4_experts(const void *x, int64_t tokens, int hidden, int inter,
   Workspace ws;
   ws.base = static_cast<char *>(workspace);
   const ExpertBuffers b = expert_buffers(ws, tokens, hidden, inter, top_k, num_experts);
-  if (routes <= kRouteRoutes)
-    return w4_route_experts(x, tokens, hidden, inter, expert_ids, weights, top_k, num_experts, w13,
-                            sh13, w2, sh2, b.act, out, s);
-  // Without a capacity the packing call writes neither ids nor weights.
-  int rc = b200moe_pack_routes(const_cast<int64_t *>(expert_ids), nullptr, routes, num_experts,
-                               nullptr, 0, num_experts, nullptr, -1, b.row_capacity, b.row_route,
-                               b.route_row, b.combine_rows, b.tile_expert, b.offsets, b.counts,
-                               b.mtiles, b.max_mtiles, nullptr, b.counters, nullptr, b.scratch,
-                               static_cast<size_t>(b.scratch_bytes), stream);
-  if (rc) return rc;
+  int rc;
+  if (routes <= kRouteRoutes) {
+    rc = w4_route_gate_up(x, tokens, hidden, inter, expert_ids, top_k, num_experts, w13, sh13,
+                          b.act, s);
+    return rc ? rc
+              : w4_route_down(b.act, tokens, hidden, inter, expert_ids, weights, top_k,
+                              num_experts, w2, sh2, out, s);
+  }
+  if (b.scratch == nullptr) {
+    const size_t smem = static_cast<size_t>(num_experts) * 12;
+    if (smem > 46 * 1024)
+      B200_CUDA(cudaFuncSetAttribute(w4_pack_routes_kernel,
+                                     cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     kPackExperts * 12));
+    B200_LAUNCH_PDL(kPdlPack, w4_pack_routes_kernel, dim3(1), dim3(kPackThreads), smem, s,
+                    expert_ids, static_cast<int>(routes), num_experts, b.row_route, b.mtiles,
+                    b.counters);
+    B200_LAUNCHED();
+  } else {
+    // Without a capacity the packing call writes neither ids nor weights.
+    rc = b200moe_pack_routes(const_cast<int64_t *>(expert_ids), nullptr, routes, num_experts,
+                             nullptr, 0, num_experts, nullptr, -1, b.row_capacity, b.row_route,
+                             b.route_row, b.combine_rows, b.tile_expert, b.offsets, b.counts,
+                             b.mtiles, b.max_mtiles, nullptr, b.counters, nullptr, b.scratch,
+                             static_cast<size_t>(b.scratch_bytes), stream);
+    if (rc) return rc;
+  }
   RowSource src = {};
   src.x = x;
   src.x_rows = tokens;
@@ -231,8 +354,8 @@ int b200moe_w4_experts(const void *x, int64_t tokens, int hidden, int inter,
   if (rc) return rc;
   const int64_t threads = tokens * (hidden / 4);
   B200_LAUNCH_PDL(kPdlCombine, w4_combine_kernel,
-                  dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, s, b.y, routes,
-                  b.combine_rows, tokens, top_k, hidden, static_cast<__nv_bfloat16 *>(out));
+                  dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, s, b.y, expert_ids,
+                  num_experts, tokens, top_k, hidden, static_cast<__nv_bfloat16 *>(out));
   B200_LAUNCHED();
   return B200MOE_OK;
 }

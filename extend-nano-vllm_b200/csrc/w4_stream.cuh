@@ -23,6 +23,8 @@
 //
 // The blocks of k of an item are split over WK warps of the thread block where
 // items are few, and summed through shared memory in a fixed order.
+#pragma once
+
 #include "w4.cuh"
 
 namespace b200moe {
@@ -70,6 +72,15 @@ __device__ __forceinline__ uint32_t word(const uint4 &v, int c) {
   return c == 0 ? v.x : c == 1 ? v.y : c == 2 ? v.z : v.w;
 }
 
+// d = a b, or d += a b.
+__device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                          uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                     uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -81,7 +92,9 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
 
 // Blocks on their way: each warp has a ring of its own in shared memory, filled
 // by bulk copies (one per block and warp), so that six kilobytes per warp are
-// in flight however few registers are left.
+// in flight however few registers are left.  Measured at 8 rows x [151552,
+// 4096]: depth 4 with two thread blocks per SM 86 us, depth 6 95, three or four
+// thread blocks (whose rings leave less of the L1 to x) 94-108.
 constexpr int kDepth = 4;
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes,
@@ -177,8 +190,7 @@ __device__ __forceinline__ void read_rows(uint4 (&xv)[4][NB], const __nv_bfloat1
 #pragma unroll
     for (int c = 0; c < 4; ++c)
 #pragma unroll
-      for (int n = 0; n < NB; ++n)
-        xv[c][n] = load_row(xp[n] + k0 + 32 * c);
+      for (int n = 0; n < NB; ++n) xv[c][n] = load_row(xp[n] + k0 + 32 * c);
   } else {
 #pragma unroll
     for (int c = 0; c < 4; ++c)
@@ -192,38 +204,36 @@ __device__ __forceinline__ void read_rows(uint4 (&xv)[4][NB], const __nv_bfloat1
 template <int GPB, int NB, bool ZEROS>
 __device__ __forceinline__ void add_block(const Block<GPB, ZEROS> &b, bool half_scale,
                                           const uint4 (&xv)[4][NB], float (&tot)[2][NB][4]) {
+  constexpr int CPG = 4 / GPB;  // chunks per group
 #pragma unroll
   for (int j = 0; j < GPB; ++j) {
     float s[4];
     b.scales(j, half_scale, s);
-    float acc[2][NB][4];
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-      for (int n = 0; n < NB; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.f;
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
+      float acc[NB][4];
       const uint32_t z0 = b.zpair(j, 2 * m), z1 = b.zpair(j, 2 * m + 1);
 #pragma unroll
-      for (int cc = 0; cc < 4 / GPB; ++cc) {
-        const int c = j * (4 / GPB) + cc;
+      for (int cc = 0; cc < CPG; ++cc) {
+        const int c = j * CPG + cc;
         uint32_t lo[4], hi[4];
         w4::decode8(word(b.codes[2 * m], c), z0, lo);
         w4::decode8(word(b.codes[2 * m + 1], c), z1, hi);
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-          mma(acc[m][n], lo[0], hi[0], lo[1], hi[1], xv[c][n].x, xv[c][n].y);
-          mma(acc[m][n], lo[2], hi[2], lo[3], hi[3], xv[c][n].z, xv[c][n].w);
+          if (cc == 0)
+            mma_first(acc[n], lo[0], hi[0], lo[1], hi[1], xv[c][n].x, xv[c][n].y);
+          else
+            mma(acc[n], lo[0], hi[0], lo[1], hi[1], xv[c][n].x, xv[c][n].y);
+          mma(acc[n], lo[2], hi[2], lo[3], hi[3], xv[c][n].z, xv[c][n].w);
         }
       }
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
-        tot[m][n][0] = fmaf(s[2 * m], acc[m][n][0], tot[m][n][0]);
-        tot[m][n][1] = fmaf(s[2 * m], acc[m][n][1], tot[m][n][1]);
-        tot[m][n][2] = fmaf(s[2 * m + 1], acc[m][n][2], tot[m][n][2]);
-        tot[m][n][3] = fmaf(s[2 * m + 1], acc[m][n][3], tot[m][n][3]);
+        tot[m][n][0] = fmaf(s[2 * m], acc[n][0], tot[m][n][0]);
+        tot[m][n][1] = fmaf(s[2 * m], acc[n][1], tot[m][n][1]);
+        tot[m][n][2] = fmaf(s[2 * m + 1], acc[n][2], tot[m][n][2]);
+        tot[m][n][3] = fmaf(s[2 * m + 1], acc[n][3], tot[m][n][3]);
       }
     }
   }
@@ -266,7 +276,7 @@ __device__ __forceinline__ Item item_of(const Args &a, int it) {
 }
 
 // The finished sums of one operand row pair, to memory.  f: feature row of the
-// item's operand (g or g + 8 within 16), n: column.
+// quarter's operand (g or g + 8 within 16), n: column.
 template <int KIND>
 __device__ __forceinline__ void store(const Args &a, const Item &it, int r0, int g, int n,
                                       float v0, float v1) {
@@ -305,9 +315,12 @@ __global__ void __launch_bounds__(32 * kWarps, 2) w4_stream_kernel(
     const __grid_constant__ Args a) {
   extern __shared__ __align__(16) uint8_t ring_smem[];  // [kWarps][kDepth] quarter blocks
   __shared__ float red[kWarps][2 * NB * 4][32];
-  __shared__ uint64_t bars[kWarps][kDepth];
   constexpr int kStage = w4::kCodeBytes + GPB * (ZEROS ? 96 : 64);
-  pdl_trigger();
+  __shared__ uint64_t bars[kWarps][kDepth];
+  // Route by route, the next kernel reads the routes before it waits for this
+  // one, so it may start only when they are there.
+  const bool by_route = KIND == kGateUp && a.ids != nullptr;
+  if (!by_route) pdl_trigger();
   const int lane = threadIdx.x & 31;
   const int warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
@@ -323,6 +336,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) w4_stream_kernel(
   }
   __syncwarp();
   if (KIND != kLinear) pdl_wait();
+  if (by_route) pdl_trigger();
   const int mt = KIND == kLinear ? 1
                  : KIND == kGateUp && a.ids != nullptr
                      ? static_cast<int>(a.num_routes)
@@ -389,8 +403,8 @@ __global__ void __launch_bounds__(32 * kWarps, 2) w4_stream_kernel(
                                                   a.top_k, a.num_routes, a.x_rows);
           xp[n] = static_cast<const __nv_bfloat16 *>(a.x) + row * a.k + 8 * t;
         }
-        // The rows of x come from L2 and are asked for one block ahead; with
-        // two column tiles there is no room for that.
+        // The rows of x come from L1 or L2 and are asked for one block ahead;
+        // with two column tiles there is no room for that.
         uint4 xv[NB == 1 ? 2 : 1][4][NB];
         if (NB == 1) read_rows(xv[0], xp, part * w4::kBlockK, a.k);
         auto step = [&](int kb, uint4 (&now)[4][NB], uint4 (&next)[4][NB]) {
@@ -415,12 +429,14 @@ __global__ void __launch_bounds__(32 * kWarps, 2) w4_stream_kernel(
         }
       }
       if (wk == 1) {
+        if (rows > 0) {
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
+          for (int n = 0; n < NB; ++n)
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            store<KIND>(a, it, r0, g + (j >> 1) * 8, 8 * n + 2 * t + (j & 1), tot[0][n][j],
-                        tot[1][n][j]);
+            for (int j = 0; j < 4; ++j)
+              store<KIND>(a, it, r0, g + (j >> 1) * 8, 8 * n + 2 * t + (j & 1), tot[0][n][j],
+                          tot[1][n][j]);
+        }
       } else {
         __syncthreads();
 #pragma unroll
@@ -447,96 +463,6 @@ __global__ void __launch_bounds__(32 * kWarps, 2) w4_stream_kernel(
   }
 }
 
-// Few routes: out[t, f] = sum_s weight[t, s] * (D_e act[t, s])[f] in slot order.
-// grid (16-row slabs, tokens); warp w takes slots w, w + 8, ...
-template <int GPB>
-__global__ void __launch_bounds__(32 * kWarps) w4_down_slots_kernel(
-    const __nv_bfloat16 *act, int hidden, int inter, const int64_t *ids,
-    const __nv_bfloat16 *weights, int top_k, int num_experts, const uint8_t *w2, const Shape sh,
-    int tiles, int num_kb, __nv_bfloat16 *__restrict__ out) {
-  constexpr int BATCH = GPB == 4 ? 4 : 6;  // blocks in flight
-  __shared__ float part[32][16];
-  pdl_trigger();
-  const int lane = threadIdx.x & 31;
-  const int warp = threadIdx.x >> 5;
-  const int g = lane >> 2, t = lane & 3;
-  const int tile = blockIdx.x >> 3, quarter = (blockIdx.x >> 1) & 3, op = blockIdx.x & 1;
-  const int64_t token = blockIdx.y;
-  const bool zeros = sh.has_zero != 0;
-  const int bytes = sh.block_bytes();
-  pdl_wait();
-  for (int s = warp; s < top_k; s += kWarps) {
-    const int64_t route = token * top_k + s;
-    const int64_t e = ids[route];
-    const bool live = e >= 0 && e < num_experts;
-    float tot[4] = {0.f, 0.f, 0.f, 0.f};
-    if (live) {
-      const uint8_t *w = w2 + (e * tiles + tile) * num_kb * bytes + quarter * sh.quarter_bytes();
-      const __nv_bfloat16 *x = act + route * inter + 8 * t;
-      for (int kb0 = 0; kb0 < num_kb; kb0 += BATCH) {
-        uint4 codes[BATCH][2];
-        uint32_t scale[BATCH][GPB];
-        uint32_t zero[BATCH][GPB];
-#pragma unroll
-        for (int b = 0; b < BATCH; ++b)
-          if (kb0 + b < num_kb) {
-            const uint8_t *block = w + static_cast<int64_t>(kb0 + b) * bytes;
-            const uint8_t *c = block + t * 512 + (op * 16 + g) * 16;
-            codes[b][0] = load_codes(c);
-            codes[b][1] = load_codes(c + 128);
-            const uint8_t *sc = block + w4::kCodeBytes + (4 * g + 2 * op) * 2;
-#pragma unroll
-            for (int j = 0; j < GPB; ++j) {
-              scale[b][j] = __ldg(reinterpret_cast<const uint32_t *>(sc + j * 64));
-              if (zeros)
-                zero[b][j] = __ldg(reinterpret_cast<const uint16_t *>(
-                    block + w4::kCodeBytes + GPB * 64 + j * 32 + 4 * g + 2 * op));
-            }
-          }
-#pragma unroll
-        for (int b = 0; b < BATCH; ++b)
-          if (kb0 + b < num_kb) {
-#pragma unroll
-            for (int j = 0; j < GPB; ++j) {
-              float acc[4] = {0.f, 0.f, 0.f, 0.f};
-              const uint32_t z0 = w4::zero_pair(zeros ? zero[b][j] & 15u : 8u);
-              const uint32_t z1 = w4::zero_pair(zeros ? (zero[b][j] >> 8) & 15u : 8u);
-#pragma unroll
-              for (int cc = 0; cc < 4 / GPB; ++cc) {
-                const int c = j * (4 / GPB) + cc;
-                const int at = (kb0 + b) * w4::kBlockK + 32 * c;
-                // Column 0 is the act row, the other columns are zero.
-                const uint4 xv = g == 0 && at < inter ? *reinterpret_cast<const uint4 *>(x + at)
-                                                      : make_uint4(0, 0, 0, 0);
-                uint32_t lo[4], hi[4];
-                w4::decode8(word(codes[b][0], c), z0, lo);
-                w4::decode8(word(codes[b][1], c), z1, hi);
-                mma(acc, lo[0], hi[0], lo[1], hi[1], xv.x, xv.y);
-                mma(acc, lo[2], hi[2], lo[3], hi[3], xv.z, xv.w);
-              }
-              const float s0 = w4::scale_f32(scale[b][j] & 0xffffu, sh.half_scale);
-              const float s1 = w4::scale_f32(scale[b][j] >> 16, sh.half_scale);
-              tot[0] = fmaf(s0, acc[0], tot[0]);
-              tot[2] = fmaf(s1, acc[2], tot[2]);
-            }
-          }
-      }
-    }
-    if (t == 0) {
-      const float w = live ? __bfloat162float(weights[route]) : 0.f;
-      part[s][g] = live ? tot[0] * w : 0.f;
-      part[s][g + 8] = live ? tot[2] * w : 0.f;
-    }
-  }
-  __syncthreads();
-  const int f = tile * w4::kTileRows + quarter * 32 + op * 16 + threadIdx.x;
-  if (threadIdx.x < 16 && f < hidden) {
-    float v = 0.f;
-    for (int s = 0; s < top_k; ++s) v += part[s][threadIdx.x];
-    out[token * hidden + f] = __float2bfloat16_rn(v);
-  }
-}
-
 template <int GPB, int KIND, int NB, bool ZEROS>
 int launch(const Args &a, int64_t blocks, cudaStream_t s) {
   constexpr int smem = kWarps * kDepth * (w4::kCodeBytes + GPB * (ZEROS ? 96 : 64));
@@ -553,14 +479,27 @@ int launch(const Args &a, int64_t blocks, cudaStream_t s) {
   return B200MOE_OK;
 }
 
-// items: warp items expected; most: an upper bound.  rows: of a row tile.
+template <int KIND, int NB>
+int launch_tile(const Args &a, int64_t blocks, cudaStream_t s) {
+  switch (a.sh.groups_per_block() * 2 + (a.sh.has_zero ? 1 : 0)) {
+    case 2: return launch<1, KIND, NB, false>(a, blocks, s);
+    case 3: return launch<1, KIND, NB, true>(a, blocks, s);
+    case 4: return launch<2, KIND, NB, false>(a, blocks, s);
+    case 5: return launch<2, KIND, NB, true>(a, blocks, s);
+    case 8: return launch<4, KIND, NB, false>(a, blocks, s);
+    default: return launch<4, KIND, NB, true>(a, blocks, s);
+  }
+}
+
+// items: warp items (quarters of tiles) that the call is expected to work off;
+// most: an upper bound.  rows: of a row tile.
 template <int KIND>
 int run(Args a, double items, int64_t most, int64_t rows, cudaStream_t s) {
-  const int nb = rows <= 8 ? 1 : 2;
-  const int64_t slots = static_cast<int64_t>(sm_count()) * 2;
+  const int64_t slots = static_cast<int64_t>(sm_count()) * 2;  // resident blocks
   // Warps per item: the number whose rounds of items, each as long as its
   // blocks and two more to begin and end, are over first.
   double best = 1e30;
+  a.wk = 1;
   for (int wk = 1; wk <= kWarps && (wk == 1 || wk <= a.num_kb); wk *= 2) {
     const int64_t rounds = static_cast<int64_t>((items * wk + slots * kWarps - 1) /
                                                 (slots * kWarps));
@@ -575,128 +514,8 @@ int run(Args a, double items, int64_t most, int64_t rows, cudaStream_t s) {
   int64_t blocks = (most + wr - 1) / wr;
   if (blocks > slots) blocks = slots;
   if (blocks < 1) blocks = 1;
-#define B200_W4S(G)                                                         \
-  if (a.sh.has_zero)                                                        \
-    return nb == 1 ? launch<G, KIND, 1, true>(a, blocks, s)                 \
-                   : launch<G, KIND, 2, true>(a, blocks, s);                \
-  return nb == 1 ? launch<G, KIND, 1, false>(a, blocks, s)                  \
-                 : launch<G, KIND, 2, false>(a, blocks, s);
-  switch (a.sh.groups_per_block()) {
-    case 1: B200_W4S(1)
-    case 2: B200_W4S(2)
-    default: B200_W4S(4)
-  }
-#undef B200_W4S
+  return rows <= 8 ? launch_tile<KIND, 1>(a, blocks, s) : launch_tile<KIND, 2>(a, blocks, s);
 }
 
 }  // namespace w4s
-
-int w4_linear_stream(const void *x, int64_t m, int n, int k, const void *w, const w4::Shape &sh,
-                     void *out, cudaStream_t s) {
-  using namespace w4s;
-  Args a = {};
-  a.w = static_cast<const uint8_t *>(w);
-  a.sh = sh;
-  a.n_blocks = (n + 127) / 128;
-  a.num_kb = static_cast<int>(w4::blocks_of(k));
-  a.n_out = n;
-  a.k = k;
-  a.m = static_cast<int>(m);
-  a.x = x;
-  a.x_rows = m;
-  a.out = out;
-  return run<kLinear>(a, 4.0 * a.n_blocks, 4ll * a.n_blocks, m, s);
-}
-
-int w4_gate_up_stream(const RowSource &src, int hidden, int inter, const void *w13,
-                      const w4::Shape &sh, const int32_t *mtiles, int64_t max_mtiles,
-                      const int32_t *counters, double tiles, int64_t rows, void *act,
-                      cudaStream_t s) {
-  using namespace w4s;
-  Args a = {};
-  a.w = static_cast<const uint8_t *>(w13);
-  a.sh = sh;
-  a.n_blocks = (inter + 63) / 64;
-  a.num_kb = static_cast<int>(w4::blocks_of(hidden));
-  a.n_out = inter;
-  a.k = hidden;
-  a.gather = src.x_packed == nullptr ? 1 : 0;
-  a.x = a.gather ? src.x : src.x_packed;
-  a.x_rows = src.x_rows;
-  a.mtiles = mtiles;
-  a.counters = counters;
-  a.max_mtiles = max_mtiles;
-  a.row_route = src.row_route;
-  a.num_routes = src.num_routes;
-  a.top_k = src.top_k;
-  a.out = act;
-  return run<kGateUp>(a, 4.0 * tiles * a.n_blocks, 4 * max_mtiles * a.n_blocks, rows, s);
-}
-
-int w4_down_stream(const void *act, int hidden, int inter, const void *w2, const w4::Shape &sh,
-                   const int32_t *row_route, const void *route_weights, int64_t num_routes,
-                   const int32_t *mtiles, int64_t max_mtiles, const int32_t *counters,
-                   double tiles, int64_t rows, float *y, cudaStream_t s) {
-  using namespace w4s;
-  Args a = {};
-  a.w = static_cast<const uint8_t *>(w2);
-  a.sh = sh;
-  a.n_blocks = (hidden + 127) / 128;
-  a.num_kb = static_cast<int>(w4::blocks_of(inter));
-  a.n_out = hidden;
-  a.k = inter;
-  a.x = act;
-  a.mtiles = mtiles;
-  a.counters = counters;
-  a.max_mtiles = max_mtiles;
-  a.row_route = row_route;
-  a.route_w = static_cast<const __nv_bfloat16 *>(route_weights);
-  a.num_routes = num_routes;
-  a.out = y;
-  return run<kDown>(a, 4.0 * tiles * a.n_blocks, 4 * max_mtiles * a.n_blocks, rows, s);
-}
-
-// The whole expert path for few routes, without packing, in two launches.
-// act: [tokens * top_k, inter] bf16.
-int w4_route_experts(const void *x, int64_t tokens, int hidden, int inter, const int64_t *ids,
-                     const void *weights, int top_k, int num_experts, const void *w13,
-                     const w4::Shape &sh13, const void *w2, const w4::Shape &sh2, void *act,
-                     void *out, cudaStream_t s) {
-  using namespace w4s;
-  Args a = {};
-  a.w = static_cast<const uint8_t *>(w13);
-  a.sh = sh13;
-  a.n_blocks = (inter + 63) / 64;
-  a.num_kb = static_cast<int>(w4::blocks_of(hidden));
-  a.n_out = inter;
-  a.k = hidden;
-  a.gather = 1;
-  a.x = x;
-  a.x_rows = tokens;
-  a.num_routes = tokens * top_k;
-  a.top_k = top_k;
-  a.ids = ids;
-  a.num_experts = num_experts;
-  a.out = act;
-  const int64_t items = 4 * a.num_routes * a.n_blocks;
-  const int rc = run<kGateUp>(a, static_cast<double>(items), items, 1, s);
-  if (rc) return rc;
-  const int tiles = (hidden + 127) / 128;
-  const dim3 grid(8 * tiles, static_cast<unsigned>(tokens));
-  auto down = [&](auto kernel) {
-    return launch_pdl(kPdlTiny, kernel, grid, dim3(32 * kWarps), 0, s,
-                      static_cast<const __nv_bfloat16 *>(act), hidden, inter, ids,
-                      static_cast<const __nv_bfloat16 *>(weights), top_k, num_experts,
-                      static_cast<const uint8_t *>(w2), sh2, tiles,
-                      static_cast<int>(w4::blocks_of(inter)), static_cast<__nv_bfloat16 *>(out));
-  };
-  switch (sh2.groups_per_block()) {
-    case 1: B200_CUDA(down(w4_down_slots_kernel<1>)); break;
-    case 2: B200_CUDA(down(w4_down_slots_kernel<2>)); break;
-    default: B200_CUDA(down(w4_down_slots_kernel<4>)); break;
-  }
-  B200_LAUNCHED();
-  return B200MOE_OK;
-}
-
 }  // namespace b200moe

@@ -481,6 +481,21 @@ def nvl_wait_return(rank: int, bufs) -> None:
 # ---------------------------------------------------------------------------
 # Scored routing.
 # ---------------------------------------------------------------------------
+# These calls are a few microseconds of GPU work, so the host side counts:
+# addresses go to the library as plain integers, and the current stream is read
+# without building a Stream object where torch offers that (2 us a call).
+_current_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _raw_stream(device_index: int) -> int:
+    if _current_raw_stream is not None:
+        return _current_raw_stream(device_index)
+    return torch.cuda.current_stream(device_index).cuda_stream
+
+
+_LOGIT_DTYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16, torch.float32: _lib.F32}
+
+
 def route_scored_topk(logits: torch.Tensor, top_k: int, *, score: str = "softmax",
                       bias: torch.Tensor | None = None, num_groups: int = 1,
                       topk_groups: int = 1, group_score: str = "top2", renormalize: bool = True,
@@ -494,14 +509,18 @@ def route_scored_topk(logits: torch.Tensor, top_k: int, *, score: str = "softmax
     groups and only the ``topk_groups`` best ones are on offer; a group's
     score is its largest biased score ("max") or the sum of its two largest
     ("top2").  Equal values go to the lowest index."""
-    _require_cuda(logits, bias)
+    if not logits.is_cuda:
+        _require_cuda(logits)
+    dtype = _LOGIT_DTYPES.get(logits.dtype)
+    if dtype is None:
+        raise TypeError(f"router logits must be fp32/bf16/fp16, got {logits.dtype}")
     if logits.dim() != 2:
         raise ValueError("router logits must be [tokens, experts]")
-    if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
-        raise TypeError(f"router logits must be fp32/bf16/fp16, got {logits.dtype}")
-    if score not in _lib.SCORE_CODES:
+    score_code = _lib.SCORE_CODES.get(score)
+    if score_code is None:
         raise ValueError(f"unknown score function {score!r}")
-    if group_score not in _lib.GROUP_SCORE_CODES:
+    group_code = _lib.GROUP_SCORE_CODES.get(group_score)
+    if group_code is None:
         raise ValueError(f"unknown group score {group_score!r}")
     tokens, experts = logits.shape
     if bias is not None:
@@ -511,12 +530,12 @@ def route_scored_topk(logits: torch.Tensor, top_k: int, *, score: str = "softmax
             raise ValueError("bias must be on the logits' device")
         bias = bias.contiguous()
     logits = logits.contiguous()
-    weights = torch.empty((tokens, top_k), device=logits.device, dtype=torch.bfloat16)
-    ids = torch.empty((tokens, top_k), device=logits.device, dtype=torch.int64)
-    call("b200moe_route_scored_topk", _p(logits), _DTYPE_CODES[logits.dtype], tokens, experts,
-         top_k, _lib.SCORE_CODES[score], _p(bias), num_groups, topk_groups,
-         _lib.GROUP_SCORE_CODES[group_score], int(bool(renormalize)), scale, _p(weights), _p(ids),
-         _stream(logits))
+    weights = logits.new_empty((tokens, top_k), dtype=torch.bfloat16)
+    ids = logits.new_empty((tokens, top_k), dtype=torch.int64)
+    call("b200moe_route_scored_topk", logits.data_ptr(), dtype, tokens, experts, top_k, score_code,
+         None if bias is None else bias.data_ptr(), num_groups, topk_groups, group_code,
+         1 if renormalize else 0, scale, weights.data_ptr(), ids.data_ptr(),
+         _raw_stream(logits.get_device()))
     return weights, ids
 
 
@@ -611,9 +630,11 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
 
 
 def _check_w4(x: torch.Tensor, weight: W4Weight, k: int) -> None:
+    if not x.is_cuda:
+        _require_cuda(x)
     if x.dtype != torch.bfloat16:
         raise TypeError(f"the 4-bit products take bf16 activations, got {x.dtype}")
-    if weight.device != x.device:
+    if weight.data.get_device() != x.get_device():
         raise ValueError("weights and activations must be on one device")
     if weight.k != k:
         raise ValueError(f"the weight has k = {weight.k}, the activations {k}")
@@ -621,15 +642,15 @@ def _check_w4(x: torch.Tensor, weight: W4Weight, k: int) -> None:
 
 def linear_w4(x: torch.Tensor, weight: W4Weight) -> torch.Tensor:
     """x [..., k] W^T with a 4-bit weight [rows, k] -> bf16 [..., rows]."""
-    _require_cuda(x)
-    _check_w4(x, weight, x.size(-1))
+    shape = x.shape
+    _check_w4(x, weight, shape[-1])
     if weight.matrices != 1 or weight.flags & _lib.W4_GATE_UP:
         raise ValueError("linear_w4 takes one weight in the \"rows\" layout")
-    rows = x.numel() // weight.k
-    out = torch.empty((*x.shape[:-1], weight.rows), device=x.device, dtype=torch.bfloat16)
+    out = x.new_empty((*shape[:-1], weight.rows))
     x = _aligned(x)
-    call("b200moe_w4_linear", _p(x), rows, weight.rows, weight.k, _p(weight.data), weight.group,
-         weight.flags, _p(out), _stream(x))
+    call("b200moe_w4_linear", x.data_ptr(), x.numel() // weight.k, weight.rows, weight.k,
+         weight.data.data_ptr(), weight.group, weight.flags, out.data_ptr(),
+         _raw_stream(x.get_device()))
     return out
 
 
@@ -641,7 +662,6 @@ def experts_w4(x: torch.Tensor, expert_ids: torch.Tensor, route_weights: torch.T
     routers return them); w13: every expert's gate and up rows [E, 2 I, H]
     packed with ``layout="gate_up"``; w2 [E, H, I].  A route whose id is outside
     [0, E) (a dropped one) contributes nothing."""
-    _require_cuda(x, expert_ids, route_weights)
     if x.dim() != 2:
         raise ValueError("x must be [tokens, hidden]")
     tokens, hidden = x.shape
@@ -652,19 +672,22 @@ def experts_w4(x: torch.Tensor, expert_ids: torch.Tensor, route_weights: torch.T
         raise TypeError("route_weights must be bf16 of the ids' shape")
     if not w13.flags & _lib.W4_GATE_UP or w2.flags & _lib.W4_GATE_UP:
         raise ValueError("w13 needs the \"gate_up\" layout and w2 the \"rows\" layout")
-    inter = w13.rows // 2
-    if w2.matrices != w13.matrices or w2.rows != hidden or w2.k != inter:
-        raise ValueError(f"w2 must be {w13.matrices} x [{hidden}, {inter}]")
-    if any(t.device != x.device for t in (expert_ids, route_weights, w2.data)):
+    inter, experts = w13.rows // 2, w13.matrices
+    if w2.matrices != experts or w2.rows != hidden or w2.k != inter:
+        raise ValueError(f"w2 must be {experts} x [{hidden}, {inter}]")
+    device = x.get_device()
+    if not (expert_ids.get_device() == route_weights.get_device() == w2.data.get_device()
+            == device):
         raise ValueError("weights, routes and activations must be on one device")
-    top_k, experts = expert_ids.size(1), w13.matrices
-    out = torch.empty((tokens, hidden), device=x.device, dtype=torch.bfloat16)
+    top_k = expert_ids.size(1)
+    out = torch.empty_like(x, memory_format=torch.contiguous_format)
     size = _w4_workspace(tokens, hidden, inter, top_k, experts)
-    workspace = torch.empty(size, device=x.device, dtype=torch.uint8)
+    workspace = x.new_empty((size,), dtype=torch.uint8)
     x, expert_ids, route_weights = _aligned(x), expert_ids.contiguous(), route_weights.contiguous()
-    call("b200moe_w4_experts", _p(x), tokens, hidden, inter, _p(expert_ids), _p(route_weights),
-         top_k, experts, _p(w13.data), w13.group, w13.flags, _p(w2.data), w2.group, w2.flags,
-         _p(workspace), size, _p(out), _stream(x))
+    call("b200moe_w4_experts", x.data_ptr(), tokens, hidden, inter, expert_ids.data_ptr(),
+         route_weights.data_ptr(), top_k, experts, w13.data.data_ptr(), w13.group, w13.flags,
+         w2.data.data_ptr(), w2.group, w2.flags, workspace.data_ptr(), size, out.data_ptr(),
+         _raw_stream(device))
     return out
 
 

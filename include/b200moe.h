@@ -656,9 +656,11 @@ B200MOE_API int b200moe_w4_linear(const void *x, int64_t m, int n, int k, const 
  *   hidden] (B200MOE_W4_GATE_UP), w2 [num_experts] matrices [hidden, inter],
  *   out [tokens, hidden] bf16; pointers 16-byte aligned.
  *   workspace: b200moe_w4_experts_workspace bytes, 256-byte aligned.
+ * b200moe_w4_experts_launches: kernels that a call launches.
  */
 B200MOE_API int64_t b200moe_w4_experts_workspace(int64_t tokens, int hidden, int inter, int top_k,
                                                  int num_experts);
+B200MOE_API int b200moe_w4_experts_launches(int64_t tokens, int top_k, int num_experts);
 B200MOE_API int b200moe_w4_experts(const void *x, int64_t tokens, int hidden, int inter,
                                    const int64_t *expert_ids, const void *weights, int top_k,
                                    int num_experts, const void *w13, int group13, int flags13,
