@@ -17,9 +17,9 @@
 // in rank order, from its shared memory.
 //
 // Warps of a CTA: 0 codes (one bulk copy per block of 128 k), 1 rows of x
-// (TMA boxes, or four-row gathers), 2 matrix instructions, 3 TMEM allocation,
+// (TMA boxes, or four-row gathers), 2 TMEM allocation and matrix instructions,
 // then decoding (groups of four, alternate blocks), then promoting and epilogue
-// (two groups of four, alternate column chunks).
+// (groups of four, alternate column chunks).
 // Every wait is bounded; on expiry the CTA records a status bit and leaves.
 #include <cudaTypedefs.h>
 
@@ -43,32 +43,40 @@ constexpr int MAX_WS = 16;
 constexpr int SMEM_LIMIT = 226 * 1024;
 constexpr int TAIL_BYTES = 1024;  // barriers
 
-template <int NT>
+// NT: rows of x per tile (the N side); GPB: groups per block of 128 k.
+template <int NT, int GPB, int KIND>
 struct Cfg {
   // TMEM: accumulators in the lower half, operand stages of 64 columns (128 k
   // in bf16 pairs) in the upper.  The operand stages and those of the x rows
   // advance together, so one completion frees both.
   static constexpr int D_COLS = 256;
-  static constexpr int ND = NT == 16 ? 8 : NT == 128 ? 2 : 4;  // accumulators
-  static constexpr int BS = 4;                                  // operand stages
-  static constexpr int B_BYTES = NT * 256;                      // 128 k of NT rows
-  static constexpr int C = NT == 16 ? 8 : 16;                  // columns per chunk
-  static constexpr int NCH = NT / C / 2;                       // chunks per promoting group
-  // Decoding groups: one keeps up with 128-row tiles (512 cycles of matrix
-  // instructions per block) and leaves the 64 sums per promoting thread room
-  // in the register file; smaller tiles are bound by the code stream.
-  static constexpr int DG = NT == 128 ? 1 : 2;
-  static constexpr int UNROLL = NT == 128 ? 1 : 2;  // blocks per loop turn
-  static constexpr int PROMOTE0 = 4 + 4 * DG;  // first promoting warp
-  static constexpr int THREADS = 32 * (PROMOTE0 + 8);
+  // A unit: the accumulators of U groups, handed over at once.  As many groups
+  // as leave room for two units, because each hand-over costs its latency.
+  static constexpr int U = GPB < 128 / NT ? GPB : 128 / NT;
+  static constexpr int UPB = GPB / U;                               // units per block
+  static constexpr int ND = 256 / (U * NT) < 4 ? 256 / (U * NT) : 4;  // units in TMEM
+  // Operand stages; the down projection's largest tile leaves one to the
+  // staging of its fp32 rows.
+  static constexpr int BS = KIND == kDown && NT == 128 ? 3 : 4;
+  static constexpr bool LOCKSTEP = UPB == 1 && ND == BS;  // the two rings are one
+  static constexpr int B_BYTES = NT * 256;                // 128 k of NT rows
+  static constexpr int C = NT == 16 || NT == 128 ? 8 : 16;  // columns per chunk
+  static constexpr int DG = 2;                              // decoding groups
+  static constexpr int PG = NT == 128 ? 4 : 2;              // promoting groups
+  static constexpr int NCH = NT / C / PG;                   // chunks per promoting group
+  static constexpr int UNROLL = NT == 128 ? 1 : 2;          // blocks per loop turn
+  static constexpr int PROMOTE0 = 3 + 4 * DG;               // first promoting warp
+  static constexpr int PROMOTERS = 4 * PG;
+  static constexpr int THREADS = 32 * (PROMOTE0 + PROMOTERS);
+  // Finished rows of a tile on their way out: [NT][128] (gate/up: 64) values.
+  static constexpr int OUT_ROW = KIND == kDown ? 512 : KIND == kLinear ? 256 : 128;  // bytes
+  static constexpr int OUT_BYTES = NT * OUT_ROW;
+  // Scales as fp32, by block: [SCALES][GPB][128].  The decoding warps are at
+  // most seven blocks ahead of the promoting ones (four operand stages, four
+  // accumulators), so eight places need no barrier of their own.
+  static constexpr int SCALES = 8;
+  static constexpr int SCALE_BYTES = SCALES * GPB * 512;
 };
-
-// One group per block and as many accumulators as operand stages: the two rings
-// are one.
-template <int NT, int GPB>
-__host__ __device__ constexpr bool lockstep() {
-  return GPB == 1 && Cfg<NT>::ND == Cfg<NT>::BS;
-}
 
 struct Args {
   const uint8_t *w;
@@ -78,6 +86,7 @@ struct Args {
   int n_out;     // features written per row
   int ws;        // stages of codes
   int split;     // CTAs per cluster
+  int staged;    // output rows allow 16-byte copies
   // dense rows
   int64_t m;
   // experts
@@ -174,6 +183,12 @@ __device__ __forceinline__ void fma2(uint64_t &acc, uint64_t s, uint32_t lo, uin
   asm volatile("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(s), "l"(v));
 }
 
+__device__ __forceinline__ void st_shared(uint32_t addr, float v) {
+  asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+__device__ __forceinline__ void st_shared(uint32_t addr, __nv_bfloat16 v) {
+  asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(__bfloat16_as_ushort(v)) : "memory");
+}
 // ---- cluster helpers ------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -268,6 +283,7 @@ struct Ring {
 struct Ctx {
   uint32_t s_b, s_w, s_red;
   uint32_t w_full, w_empty, b_full, a_full, ab_empty, d_full, d_empty, red_full, red_empty;
+  uint32_t s_out, s_scale, out_free, out_full;
   uint32_t tmem;
   volatile int *abort;
   int wbytes, qbytes, scale_off, zero_off;
@@ -299,10 +315,10 @@ __device__ __forceinline__ void load_codes(const Args &args, const Ctx &c) {
 // Rows of x.  Dense rows and full tiles come as one box of NT rows per 64 k,
 // the rows of other tiles as boxes of 16 (lane b loads the b-th), gathered
 // rows four at a time (lane l loads the l-th four).  A whole warp.
-template <int NT, int KIND>
+template <int NT, int GPB, int KIND>
 __device__ __forceinline__ void load_rows(const Args &args, const Ctx &c, const CUtensorMap *tm,
                                           const CUtensorMap *tm_whole) {
-  using C = Cfg<NT>;
+  using C = Cfg<NT, GPB, KIND>;
   const int lane = threadIdx.x & 31;
   const bool gather = KIND == kGateUp && args.gather != 0;
   Ring b;
@@ -355,7 +371,7 @@ __device__ __forceinline__ void load_rows(const Args &args, const Ctx &c, const 
 // Matrix instructions.  One lane.
 template <int NT, int GPB, int KIND>
 __device__ __forceinline__ void issue_mma(const Args &args, const Ctx &c) {
-  using C = Cfg<NT>;
+  using C = Cfg<NT, GPB, KIND>;
   constexpr int KK = 8 / GPB;  // instructions of 16 k per group
   Ring b, d;
   // Descriptor of stage 0; the start address field counts 16 bytes.
@@ -381,18 +397,21 @@ __device__ __forceinline__ void issue_mma(const Args &args, const Ctx &c) {
         const uint64_t desc = desc0 + static_cast<uint32_t>(b.stage * (C::B_BYTES >> 4));
         const uint32_t ta = c.tmem + C::D_COLS + b.stage * 64;
 #pragma unroll
-        for (int g = 0; g < GPB; ++g) {
-          if (g > 0 && !wait(c.d_empty + 8 * d.stage, d.phase ^ 1, c.abort)) return;
+        for (int u = 0; u < C::UPB; ++u) {
+          if (u > 0 && !wait(c.d_empty + 8 * d.stage, d.phase ^ 1, c.abort)) return;
           tc_fence_after();
-          const uint32_t td = c.tmem + d.stage * NT;
 #pragma unroll
-          for (int j = 0; j < KK; ++j) {
-            const int kk = g * KK + j;
-            mma_ts(td, ta + kk * 8, desc + ((kk >> 2) * (NT * 8) + (kk & 3) * 2), idesc, j != 0);
+          for (int g = 0; g < C::U; ++g) {
+            const uint32_t td = c.tmem + (d.stage * C::U + g) * NT;
+#pragma unroll
+            for (int j = 0; j < KK; ++j) {
+              const int kk = (u * C::U + g) * KK + j;
+              mma_ts(td, ta + kk * 8, desc + ((kk >> 2) * (NT * 8) + (kk & 3) * 2), idesc, j != 0);
+            }
           }
           // Accumulators in step with the operand stages: one completion
           // serves both.
-          if (!lockstep<NT, GPB>()) tc_commit(c.d_full + 8 * d.stage);
+          if (!C::LOCKSTEP) tc_commit(c.d_full + 8 * d.stage);
           d.next(C::ND);
         }
         tc_commit(c.ab_empty + 8 * b.stage);
@@ -406,7 +425,7 @@ __device__ __forceinline__ void issue_mma(const Args &args, const Ctx &c) {
 // `grp` of DG takes every DG-th block.  Four warps, one weight row per thread.
 template <int NT, int GPB, int KIND>
 __device__ __forceinline__ void decode(const Args &args, const Ctx &c, int grp, int q) {
-  using C = Cfg<NT>;
+  using C = Cfg<NT, GPB, KIND>;
   const int lane = threadIdx.x & 31;
   const int place = w4::scale_place(lane);
   const bool zeros = args.sh.has_zero != 0;
@@ -414,7 +433,8 @@ __device__ __forceinline__ void decode(const Args &args, const Ctx &c, int grp, 
   Ring w, a;
   w.next(args.ws, grp);
   a.next(C::BS, grp);
-  int skip = grp;  // blocks until this group's next one
+  int skip = grp;   // blocks until this group's next one
+  int block = grp;  // of all this CTA's blocks
   for (int it = c.first; it < c.items; it += c.step) {
     const Tile t = tile_of<NT, KIND>(args, it / args.n_blocks);
     for (int r0 = 0; r0 < t.rows; r0 += NT) {
@@ -438,9 +458,20 @@ __device__ __forceinline__ void decode(const Args &args, const Ctx &c, int grp, 
             asm volatile("ld.shared.u8 %0, [%1];" : "=r"(z) : "r"(st + c.zero_off + g * 32 + place));
           zp[g] = w4::zero_pair(z);
         }
+        uint16_t scale[GPB];
+#pragma unroll
+        for (int g = 0; g < GPB; ++g)
+          asm volatile("ld.shared.u16 %0, [%1];"
+                       : "=h"(scale[g])
+                       : "r"(st + c.scale_off + g * 64 + place * 2));
         if (!wait(c.ab_empty + 8 * a.stage, a.phase ^ 1, c.abort)) return;
         tc_fence_after();
         const uint32_t ta = tq + a.stage * 64;
+        const uint32_t ss = c.s_scale + (block & (C::SCALES - 1)) * (GPB * 512) + (q * 32 + lane) * 4;
+#pragma unroll
+        for (int g = 0; g < GPB; ++g)
+          st_shared(ss + g * 512, w4::scale_f32(scale[g], args.sh.half_scale));
+        block += C::DG;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t r[32];
@@ -469,16 +500,17 @@ __device__ __forceinline__ void decode(const Args &args, const Ctx &c, int grp, 
   }
 }
 
-// Promoting and epilogue.  Two groups of four warps (alternate column chunks),
-// one weight row per thread.
+// Promoting and epilogue.  PG groups of four warps (alternate column chunks), one
+// weight row per thread.
 template <int NT, int GPB, int KIND>
 __device__ __forceinline__ void promote(const Args &args, const Ctx &c, int half, int q) {
-  using C = Cfg<NT>;
+  using C = Cfg<NT, GPB, KIND>;
   const int lane = threadIdx.x & 31;
   const int row = q * 32 + lane;
   const uint32_t tq = c.tmem + (static_cast<uint32_t>(q * 32) << 16);
-  Ring w, d;
-  uint32_t red_phase = 0;
+  Ring d;
+  int block = 0;
+  uint32_t red_phase = 0, out_phase = 0;
   for (int it = c.first; it < c.items; it += c.step) {
     const Tile t = tile_of<NT, KIND>(args, it / args.n_blocks);
     const int fb = it % args.n_blocks;
@@ -492,38 +524,44 @@ __device__ __forceinline__ void promote(const Args &args, const Ctx &c, int half
         for (int j = 0; j < C::C / 2; ++j) acc2[i][j] = 0;
 #pragma unroll C::UNROLL
       for (int kb = c.kb0; kb < c.kb1; ++kb) {
-        const uint32_t scales = c.s_w + w.stage * c.wbytes + q * c.qbytes + c.scale_off + w4::scale_place(lane) * 2;
+        const uint32_t scales =
+            c.s_scale + (block & (C::SCALES - 1)) * (GPB * 512) + row * 4;
+        ++block;
 #pragma unroll
-        for (int g = 0; g < GPB; ++g) {
-          // A finished product implies the codes and scales of its stage: the
-          // decoding warps waited for the copy before they signalled it.
-          if (!wait((lockstep<NT, GPB>() ? c.ab_empty : c.d_full) + 8 * d.stage, d.phase, c.abort))
-            return;
+        for (int u = 0; u < C::UPB; ++u) {
+          // A finished product implies its scales: the decoding warps wrote
+          // them before they signalled the operand.
+          if (!wait((C::LOCKSTEP ? c.ab_empty : c.d_full) + 8 * d.stage, d.phase, c.abort)) return;
           tc_fence_after();
-          uint16_t bits;
-          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(bits) : "r"(scales + g * 64));
-          const float s = w4::scale_f32(bits, args.sh.half_scale);
-          const uint64_t s2 = pack2(s, s);
-          const uint32_t td = tq + d.stage * NT + half * C::C;
-          // The next chunk loads while this one is added.  Columns beyond
-          // n_mma hold old sums; they are never stored.
+          const uint32_t td = tq + d.stage * (C::U * NT) + half * C::C;
+          // Piece l = (group, chunk): the next one loads while this one is
+          // added.  Columns beyond n_mma hold old sums; they are never stored.
           uint32_t v[2][C::C];
           tmem_ld(td, v[0]);
+          uint64_t s2[C::U];
 #pragma unroll
-          for (int i = 0; i < C::NCH; ++i) {
+          for (int g = 0; g < C::U; ++g) {
+            float s;
+            asm volatile("ld.shared.f32 %0, [%1];"
+                         : "=f"(s)
+                         : "r"(scales + (u * C::U + g) * 512));
+            s2[g] = pack2(s, s);
+          }
+#pragma unroll
+          for (int l = 0; l < C::U * C::NCH; ++l) {
+            const int g = l / C::NCH, i = l % C::NCH;
             tmem_ld_wait();
-            if (i + 1 < C::NCH) tmem_ld(td + (i + 1) * 2 * C::C, v[(i + 1) & 1]);
+            if (l + 1 < C::U * C::NCH)
+              tmem_ld(td + ((l + 1) / C::NCH) * NT + ((l + 1) % C::NCH) * C::PG * C::C, v[(l + 1) & 1]);
 #pragma unroll
             for (int j = 0; j < C::C / 2; ++j)
-              fma2(acc2[i][j], s2, v[i & 1][2 * j], v[i & 1][2 * j + 1]);
+              fma2(acc2[i][j], s2[g], v[l & 1][2 * j], v[l & 1][2 * j + 1]);
           }
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(c.d_empty + 8 * d.stage);
           d.next(C::ND);
         }
-        if (lane == 0) mbar_arrive(c.w_empty + 8 * w.stage);
-        w.next(args.ws);
       }
       float acc[C::NCH][C::C];
 #pragma unroll
@@ -538,7 +576,7 @@ __device__ __forceinline__ void promote(const Args &args, const Ctx &c, int half
           const uint32_t dst = map_rank(c.s_red + ((c.rank - 1) * NT * 128 + row) * 4, 0);
 #pragma unroll
           for (int i = 0; i < C::NCH; ++i) {
-            const int col = (2 * i + half) * C::C;
+            const int col = (C::PG * i + half) * C::C;
             if (col < n_mma) {
 #pragma unroll
               for (int j = 0; j < C::C; ++j) st_cluster(dst + (col + j) * 512, acc[i][j]);
@@ -554,7 +592,7 @@ __device__ __forceinline__ void promote(const Args &args, const Ctx &c, int half
         for (int p = 0; p < c.split - 1; ++p) {
 #pragma unroll
           for (int i = 0; i < C::NCH; ++i) {
-            const int col = (2 * i + half) * C::C;
+            const int col = (C::PG * i + half) * C::C;
             if (col < n_mma) {
 #pragma unroll
               for (int j = 0; j < C::C; ++j) {
@@ -572,6 +610,17 @@ __device__ __forceinline__ void promote(const Args &args, const Ctx &c, int half
           for (int p = 1; p < c.split; ++p) arrive_cluster(map_rank(c.red_empty, p));
       }
       const int64_t row0 = static_cast<int64_t>(t.rb) + r0;
+      // Finished values go to shared memory as whole output rows and leave in
+      // 16-byte pieces, a row at a time.  (Stored from the registers, one
+      // column of 32 features per store, a tile took longer than its six
+      // blocks of products; a bulk copy per row, issued lane by lane, too.)
+      const bool staged = args.staged != 0;
+      if (staged) {
+        // The rows of the item before have been read, by every warp.
+        __syncwarp();
+        if (lane == 0) mbar_arrive(c.out_free);
+        if (!wait(c.out_free, out_phase, c.abort)) return;
+      }
       if constexpr (KIND == kGateUp) {
         // Lanes 0-15 hold gate rows, 16-31 the up rows of the same features:
         // of each pair of columns the lower half finishes the first, the upper
@@ -582,47 +631,43 @@ __device__ __forceinline__ void promote(const Args &args, const Ctx &c, int half
         const int last = f < args.n_out ? rows : 0;
 #pragma unroll
         for (int i = 0; i < C::NCH; ++i) {
-          const int col = (2 * i + half) * C::C;
+          const int col = (C::PG * i + half) * C::C;
           if (col < n_mma) {
             auto *out = static_cast<__nv_bfloat16 *>(args.out) + (row0 + col + odd) * args.n_out + f;
+            const uint32_t so = c.s_out + (col + odd) * C::OUT_ROW + (q * 16 + (lane & 15)) * 2;
 #pragma unroll
             for (int j = 0; j < C::C; j += 2) {
               const float other =
                   __shfl_xor_sync(0xffffffffu, up ? acc[i][j] : acc[i][j + 1], 16);
               const float gv = up ? other : acc[i][j];
               const float uv = up ? acc[i][j + 1] : other;
-              if (col + j + odd < last) *out = __float2bfloat16_rn(silu_fast(gv) * uv);
-              out += 2 * static_cast<int64_t>(args.n_out);
+              const __nv_bfloat16 v = __float2bfloat16_rn(silu_fast(gv) * uv);
+              if (staged) {
+                st_shared(so + j * C::OUT_ROW, v);
+              } else {
+                if (col + j + odd < last) *out = v;
+                out += 2 * static_cast<int64_t>(args.n_out);
+              }
             }
           }
         }
       } else if constexpr (KIND == kDown) {
-        const int f = fb * 128 + row;
-        const bool in = f < args.n_out;
+        // Route rows are multiples of 128 bytes: always staged.
 #pragma unroll
         for (int i = 0; i < C::NCH; ++i) {
-          const int col = (2 * i + half) * C::C;
+          const int col = (C::PG * i + half) * C::C;
           if (col < n_mma) {
-            // Lane j knows the route and the weight of column col + j.
-            int32_t route = -1;
+            // Lane j knows the weight of column col + j.
             float weight = 0.f;
             if (lane < C::C && col + lane < rows) {
-              route = args.row_route[row0 + col + lane];
-              if (route < 0 || route >= args.num_routes) {
-                atomicOr(&g_status, kStatusIndex);
-                route = -1;
-              } else {
+              const int32_t route = args.row_route[row0 + col + lane];
+              if (route >= 0 && route < args.num_routes)
                 weight = __bfloat162float(args.route_w[route]);
-              }
             }
 #pragma unroll
-            for (int j = 0; j < C::C; ++j) {
-              const int32_t r = __shfl_sync(0xffffffffu, route, j);
-              const float wgt = __shfl_sync(0xffffffffu, weight, j);
-              if (in && r >= 0)
-                static_cast<float *>(args.out)[static_cast<int64_t>(r) * args.n_out + f] =
-                    acc[i][j] * wgt;
-            }
+            for (int j = 0; j < C::C; ++j)
+              st_shared(c.s_out + (col + j) * C::OUT_ROW + row * 4,
+                        acc[i][j] * __shfl_sync(0xffffffffu, weight, j));
           }
         }
       } else {
@@ -630,14 +675,54 @@ __device__ __forceinline__ void promote(const Args &args, const Ctx &c, int half
         const int last = f < args.n_out ? rows : 0;
 #pragma unroll
         for (int i = 0; i < C::NCH; ++i) {
-          const int col = (2 * i + half) * C::C;
+          const int col = (C::PG * i + half) * C::C;
           if (col < n_mma) {
             auto *out = static_cast<__nv_bfloat16 *>(args.out) + (row0 + col) * args.n_out + f;
+            const uint32_t so = c.s_out + col * C::OUT_ROW + row * 2;
 #pragma unroll
             for (int j = 0; j < C::C; ++j) {
-              if (col + j < last) *out = __float2bfloat16_rn(acc[i][j]);
-              out += args.n_out;
+              const __nv_bfloat16 v = __float2bfloat16_rn(acc[i][j]);
+              if (staged) {
+                st_shared(so + j * C::OUT_ROW, v);
+              } else {
+                if (col + j < last) *out = v;
+                out += args.n_out;
+              }
             }
+          }
+        }
+      }
+      if (staged) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(c.out_full);
+        if (!wait(c.out_full, out_phase, c.abort)) return;
+        out_phase ^= 1;
+        constexpr int PER = KIND == kGateUp ? 64 : 128;  // features of an item
+        constexpr int SIZE = KIND == kDown ? 4 : 2;
+        constexpr int LANES = C::OUT_ROW / 16;  // of a row
+        constexpr int STEP = C::PROMOTERS * (32 / LANES);
+        const int bytes = min(PER, args.n_out - fb * PER) * SIZE;
+        const bool mine = (lane % LANES) * 16 < bytes;
+        char *out = static_cast<char *>(args.out) + static_cast<int64_t>(fb) * (PER * SIZE) +
+                    (lane % LANES) * 16;
+        const int n0 = (half * 4 + q) * (32 / LANES) + lane / LANES;
+#pragma unroll
+        for (int i = 0; i < (NT + STEP - 1) / STEP; ++i) {
+          const int n = n0 + i * STEP;
+          if (n < rows && mine) {
+            int64_t to = row0 + n;
+            if (KIND == kDown) {
+              to = args.row_route[to];
+              if (to < 0 || to >= args.num_routes) {
+                atomicOr(&g_status, kStatusIndex);
+                continue;
+              }
+            }
+            uint4 v;
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                         : "r"(c.s_out + n * C::OUT_ROW + (lane % LANES) * 16));
+            *reinterpret_cast<uint4 *>(out + to * (static_cast<int64_t>(args.n_out) * SIZE)) = v;
           }
         }
       }
@@ -647,10 +732,10 @@ __device__ __forceinline__ void promote(const Args &args, const Ctx &c, int half
 
 // NT: rows of x per tile; GPB: groups per block of 128 k.
 template <int NT, int GPB, int KIND>
-__global__ void __launch_bounds__(Cfg<NT>::THREADS, 1)
+__global__ void __launch_bounds__(Cfg<NT, GPB, KIND>::THREADS, 1)
     w4_gemm_kernel(const __grid_constant__ CUtensorMap tmX,
                    const __grid_constant__ CUtensorMap tmWhole, const __grid_constant__ Args args) {
-  using C = Cfg<NT>;
+  using C = Cfg<NT, GPB, KIND>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                               ~static_cast<uintptr_t>(1023));
@@ -662,7 +747,11 @@ __global__ void __launch_bounds__(Cfg<NT>::THREADS, 1)
   c.zero_off = args.sh.zero_off();
   uint8_t *s_w = smem + C::BS * C::B_BYTES;
   uint8_t *s_red = s_w + args.ws * c.wbytes;  // [split - 1][NT][128] fp32
-  uint64_t *bars = reinterpret_cast<uint64_t *>(s_red + (split - 1) * NT * 512);
+  uint8_t *s_out = s_red + (split - 1) * NT * 512;  // [NT] output rows
+  uint8_t *s_scale = s_out + C::OUT_BYTES;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(s_scale + C::SCALE_BYTES);
+  c.s_scale = smem_u32(s_scale);
+  c.s_out = smem_u32(s_out);
   c.s_b = smem_u32(smem);
   c.s_w = smem_u32(s_w);
   c.s_red = smem_u32(s_red);
@@ -675,8 +764,10 @@ __global__ void __launch_bounds__(Cfg<NT>::THREADS, 1)
   c.d_empty = c.d_full + 8 * C::ND;
   c.red_full = c.d_empty + 8 * C::ND;
   c.red_empty = c.red_full + 8;
+  c.out_free = c.red_empty + 8;
+  c.out_full = c.out_free + 8;
   uint32_t *tmem_holder =
-      reinterpret_cast<uint32_t *>(bars + 2 * MAX_WS + 3 * C::BS + 2 * C::ND + 2);
+      reinterpret_cast<uint32_t *>(bars + 2 * MAX_WS + 3 * C::BS + 2 * C::ND + 4);
   c.abort = reinterpret_cast<volatile int *>(tmem_holder + 1);
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
@@ -688,7 +779,7 @@ __global__ void __launch_bounds__(Cfg<NT>::THREADS, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < args.ws; ++s) {
       mbar_init(c.w_full + 8 * s, 1);
-      mbar_init(c.w_empty + 8 * s, 12);  // four decoding and eight promoting warps
+      mbar_init(c.w_empty + 8 * s, 4);  // a decoding group
     }
     for (int s = 0; s < C::BS; ++s) {
       mbar_init(c.b_full + 8 * s, 1);
@@ -697,10 +788,12 @@ __global__ void __launch_bounds__(Cfg<NT>::THREADS, 1)
     }
     for (int s = 0; s < C::ND; ++s) {
       mbar_init(c.d_full + 8 * s, 1);
-      mbar_init(c.d_empty + 8 * s, 8);
+      mbar_init(c.d_empty + 8 * s, C::PROMOTERS);
     }
-    mbar_init(c.red_full, 8 * (split > 1 ? split - 1 : 1));
-    mbar_init(c.red_empty, 8);
+    mbar_init(c.red_full, C::PROMOTERS * (split > 1 ? split - 1 : 1));
+    mbar_init(c.red_empty, C::PROMOTERS);
+    mbar_init(c.out_free, C::PROMOTERS);
+    mbar_init(c.out_full, C::PROMOTERS);
     *c.abort = 0;
     fence_mbar_init();
   }
@@ -708,7 +801,7 @@ __global__ void __launch_bounds__(Cfg<NT>::THREADS, 1)
     prefetch_tmap(&tmX);
     prefetch_tmap(&tmWhole);
   }
-  if (warp == 3) {
+  if (warp == 2) {
     tmem_alloc(smem_u32(tmem_holder), 512);
     tmem_relinquish();
   }
@@ -732,13 +825,13 @@ __global__ void __launch_bounds__(Cfg<NT>::THREADS, 1)
   if (warp == 0) {
     if (elect_one()) load_codes<NT, KIND>(args, c);
   } else if (warp == 1) {
-    load_rows<NT, KIND>(args, c, &tmX, &tmWhole);
+    load_rows<NT, GPB, KIND>(args, c, &tmX, &tmWhole);
   } else if (warp == 2) {
     if (elect_one()) issue_mma<NT, GPB, KIND>(args, c);
   } else if (warp >= C::PROMOTE0) {
     promote<NT, GPB, KIND>(args, c, (warp - C::PROMOTE0) >> 2, warp & 3);
-  } else if (warp >= 4) {
-    decode<NT, GPB, KIND>(args, c, (warp - 4) >> 2, warp & 3);
+  } else if (warp >= 3) {
+    decode<NT, GPB, KIND>(args, c, (warp - 3) >> 2, warp & 3);
   }
   __syncwarp();
   tc_fence_before();
@@ -751,23 +844,17 @@ __global__ void __launch_bounds__(Cfg<NT>::THREADS, 1)
     __syncthreads();
   }
   if (split > 1) cluster_sync();  // nobody leaves while a peer may write here
-  if (warp == 3) {
+  if (warp == 2) {
     tc_fence_after();
     tmem_dealloc(c.tmem, 512);
   }
 }
 
-template <int NT>
-size_t smem_bytes(const Args &a) {
-  return 1024 + static_cast<size_t>(Cfg<NT>::BS) * Cfg<NT>::B_BYTES +
-         static_cast<size_t>(a.ws) * a.sh.block_bytes() +
-         static_cast<size_t>(a.split - 1) * NT * 512 + TAIL_BYTES;
-}
-
 template <int NT, int GPB, int KIND>
-int launch(const CUtensorMap &mx, const CUtensorMap &mwhole, Args a, double items, cudaStream_t s) {
-  static_assert((2 * MAX_WS + 3 * Cfg<NT>::BS + 2 * Cfg<NT>::ND + 2) * 8 + 16 <=
-                    TAIL_BYTES,
+int launch(const CUtensorMap &mx, const CUtensorMap &mwhole, Args a, double items,
+           cudaStream_t s) {
+  using C = Cfg<NT, GPB, KIND>;
+  static_assert((2 * MAX_WS + 3 * C::BS + 2 * C::ND + 4) * 8 + 16 <= TAIL_BYTES,
                 "shared memory tail");
   static bool done[64] = {false};
   const int dev = current_device();
@@ -792,17 +879,17 @@ int launch(const CUtensorMap &mx, const CUtensorMap &mwhole, Args a, double item
     }
   }
   a.split = best;
-  a.ws = static_cast<int>((SMEM_LIMIT - static_cast<int64_t>(Cfg<NT>::BS) * Cfg<NT>::B_BYTES -
-                           static_cast<int64_t>(a.split - 1) * NT * 512 - TAIL_BYTES) /
-                          a.sh.block_bytes());
-  a.ws = (a.ws > MAX_WS ? MAX_WS : a.ws) & ~1;  // the decoding groups step by two
+  const int64_t fixed = static_cast<int64_t>(C::BS) * C::B_BYTES + C::OUT_BYTES + C::SCALE_BYTES +
+                        static_cast<int64_t>(a.split - 1) * NT * 512 + TAIL_BYTES;
+  a.ws = static_cast<int>((SMEM_LIMIT - fixed) / a.sh.block_bytes());
+  if (a.ws > MAX_WS) a.ws = MAX_WS;
   int clusters = sms / a.split;
   const int64_t most = (KIND == kLinear ? (a.m + NT - 1) / NT : a.max_mtiles) * a.n_blocks;
   if (most < clusters) clusters = static_cast<int>(most < 1 ? 1 : most);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(clusters * a.split);
-  cfg.blockDim = dim3(Cfg<NT>::THREADS);
-  cfg.dynamicSmemBytes = smem_bytes<NT>(a);
+  cfg.blockDim = dim3(C::THREADS);
+  cfg.dynamicSmemBytes = 1024 + static_cast<size_t>(fixed) + static_cast<size_t>(a.ws) * a.sh.block_bytes();
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   int n = 0;
@@ -874,6 +961,7 @@ int w4_linear_tc(const void *x, int64_t m, int n, int k, const void *w, const w4
   a.n_blocks = (n + 127) / 128;
   a.num_kb = static_cast<int>(w4::blocks_of(k));
   a.n_out = n;
+  a.staged = n % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
   a.m = m;
   a.out = out;
   const int nt = tile_rows(m);
@@ -893,6 +981,7 @@ int w4_gate_up_tc(const RowSource &src, int hidden, int inter, const void *w13,
   a.n_blocks = (inter + 63) / 64;
   a.num_kb = static_cast<int>(w4::blocks_of(hidden));
   a.n_out = inter;
+  a.staged = 1;
   a.mtiles = mtiles;
   a.counters = counters;
   a.max_mtiles = max_mtiles;
@@ -919,6 +1008,7 @@ int w4_down_tc(const void *act, int hidden, int inter, const void *w2, const w4:
   a.n_blocks = (hidden + 127) / 128;
   a.num_kb = static_cast<int>(w4::blocks_of(inter));
   a.n_out = hidden;
+  a.staged = 1;
   a.mtiles = mtiles;
   a.counters = counters;
   a.max_mtiles = max_mtiles;
