@@ -340,7 +340,7 @@ int b200moe_w4_experts(const void *x, int64_t tokens, int hidden, int inter,
   // Row tiles to expect when routes fall evenly, and rows of a full one.
   const double mean = static_cast<double>(routes) / num_experts;
   const double tiles = num_experts * (1.0 - exp(-mean)) + static_cast<double>(routes) / 128;
-  const int64_t rows = min64(tokens, static_cast<int64_t>(2.0 * mean + 4.0));
+  const int64_t rows = min64(tokens, static_cast<int64_t>(1.5 * mean + 8.0));
   if (rows <= kStreamRows) {
     rc = w4_gate_up_stream(src, hidden, inter, w13, sh13, b.mtiles, b.max_mtiles, b.counters,
                            tiles, rows, b.act, s);

@@ -76,6 +76,8 @@ struct Cfg {
   // accumulators), so eight places need no barrier of their own.
   static constexpr int SCALES = 8;
   static constexpr int SCALE_BYTES = SCALES * GPB * 512;
+  // Routes and weights of a tile's rows, of two tiles: [2][2][NT].
+  static constexpr int ROUTE_BYTES = KIND == kDown ? 16 * NT : 0;
 };
 
 struct Args {
@@ -115,6 +117,27 @@ __device__ __forceinline__ Tile tile_of(const Args &a, int m) {
   const int32_t *t = a.mtiles + m * B200MOE_MTILE_WORDS;
   return Tile{t[0], t[1], t[2] - t[1]};
 }
+
+// The items of a CTA in order; the record of the next tile is read while the
+// current one is worked off.
+template <int NT, int KIND>
+struct Items {
+  const Args &a;
+  int it, items, step;
+  Tile t, next;
+  __device__ __forceinline__ Items(const Args &args, int first, int count, int by)
+      : a(args), it(first), items(count), step(by), t{0, 0, 0}, next{0, 0, 0} {
+    if (it < items) next = tile_of<NT, KIND>(a, it / a.n_blocks);
+  }
+  // Makes item `it` current; false at the end.
+  __device__ __forceinline__ bool take() {
+    if (it >= items) return false;
+    t = next;
+    if (it + step < items) next = tile_of<NT, KIND>(a, (it + step) / a.n_blocks);
+    return true;
+  }
+  __device__ __forceinline__ int block() const { return it % a.n_blocks; }
+};
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes,
                                           uint32_t bar) {
@@ -283,7 +306,7 @@ struct Ring {
 struct Ctx {
   uint32_t s_b, s_w, s_red;
   uint32_t w_full, w_empty, b_full, a_full, ab_empty, d_full, d_empty, red_full, red_empty;
-  uint32_t s_out, s_scale, out_free, out_full;
+  uint32_t s_out, s_scale, s_route, out_free, out_full;
   uint32_t tmem;
   volatile int *abort;
   int wbytes, qbytes, scale_off, zero_off;
@@ -295,9 +318,9 @@ struct Ctx {
 template <int NT, int KIND>
 __device__ __forceinline__ void load_codes(const Args &args, const Ctx &c) {
   Ring w;
-  for (int it = c.first; it < c.items; it += c.step) {
-    const Tile t = tile_of<NT, KIND>(args, it / args.n_blocks);
-    const uint8_t *src = args.w + (static_cast<int64_t>(t.e) * args.n_blocks + it % args.n_blocks) *
+  for (Items<NT, KIND> item(args, c.first, c.items, c.step); item.take(); item.it += c.step) {
+    const Tile t = item.t;
+    const uint8_t *src = args.w + (static_cast<int64_t>(t.e) * args.n_blocks + item.block()) *
                                       args.num_kb * c.wbytes;
     for (int r0 = 0; r0 < t.rows; r0 += NT)
 #pragma unroll 4
@@ -312,9 +335,10 @@ __device__ __forceinline__ void load_codes(const Args &args, const Ctx &c) {
   }
 }
 
-// Rows of x.  Dense rows and full tiles come as one box of NT rows per 64 k,
-// the rows of other tiles as boxes of 16 (lane b loads the b-th), gathered
-// rows four at a time (lane l loads the l-th four).  A whole warp.
+// Rows of x.  Dense rows and nearly full tiles come as one box of NT rows per
+// 64 k (rows past the tile are multiplied with nothing), those of other tiles as
+// boxes of 16, gathered rows four at a time (lane l loads the l-th four).  A
+// whole warp.
 template <int NT, int GPB, int KIND>
 __device__ __forceinline__ void load_rows(const Args &args, const Ctx &c, const CUtensorMap *tm,
                                           const CUtensorMap *tm_whole) {
@@ -322,13 +346,14 @@ __device__ __forceinline__ void load_rows(const Args &args, const Ctx &c, const 
   const int lane = threadIdx.x & 31;
   const bool gather = KIND == kGateUp && args.gather != 0;
   Ring b;
-  for (int it = c.first; it < c.items; it += c.step) {
-    const Tile t = tile_of<NT, KIND>(args, it / args.n_blocks);
+  for (Items<NT, KIND> item(args, c.first, c.items, c.step); item.take(); item.it += c.step) {
+    const Tile t = item.t;
     for (int r0 = 0; r0 < t.rows; r0 += NT) {
       const int rows = min(NT, t.rows - r0);
       const int nbox = (rows + 15) >> 4;
-      const bool whole = !gather && (nbox * 16 == NT || KIND == kLinear);
-      const bool mine = !whole && lane < (gather ? nbox * 4 : nbox);
+      // One box of NT rows, unless at least half of it would be wasted.
+      const bool whole = !gather && (KIND == kLinear || nbox * 32 > NT);
+      const bool mine = gather && lane < nbox * 4;
       const uint32_t bytes = whole ? C::B_BYTES : nbox * 16 * 256;
       int tok[4] = {0, 0, 0, 0};
       if (gather && mine) {
@@ -348,18 +373,18 @@ __device__ __forceinline__ void load_rows(const Args &args, const Ctx &c, const 
           if (whole) {
             tma_load_2d(dst, tm_whole, bar, c0, t.rb + r0);
             tma_load_2d(dst + NT * 128, tm_whole, bar, c0 + 64, t.rb + r0);
+          } else if (!gather) {
+            for (int i = 0; i < nbox; ++i) {
+              tma_load_2d(dst + i * 2048, tm, bar, c0, t.rb + r0 + i * 16);
+              tma_load_2d(dst + NT * 128 + i * 2048, tm, bar, c0 + 64, t.rb + r0 + i * 16);
+            }
           }
         }
         __syncwarp();
         if (mine) {
-          if (gather) {
-            tma_gather4(dst + lane * 512, tm, bar, c0, tok[0], tok[1], tok[2], tok[3]);
-            tma_gather4(dst + NT * 128 + lane * 512, tm, bar, c0 + 64, tok[0], tok[1], tok[2],
-                        tok[3]);
-          } else {
-            tma_load_2d(dst + lane * 2048, tm, bar, c0, t.rb + r0 + lane * 16);
-            tma_load_2d(dst + NT * 128 + lane * 2048, tm, bar, c0 + 64, t.rb + r0 + lane * 16);
-          }
+          tma_gather4(dst + lane * 512, tm, bar, c0, tok[0], tok[1], tok[2], tok[3]);
+          tma_gather4(dst + NT * 128 + lane * 512, tm, bar, c0 + 64, tok[0], tok[1], tok[2],
+                      tok[3]);
         }
         __syncwarp();
         b.next(C::BS);
@@ -376,8 +401,8 @@ __device__ __forceinline__ void issue_mma(const Args &args, const Ctx &c) {
   Ring b, d;
   // Descriptor of stage 0; the start address field counts 16 bytes.
   const uint64_t desc0 = sw128_kmajor_desc(c.s_b);
-  for (int it = c.first; it < c.items; it += c.step) {
-    const Tile t = tile_of<NT, KIND>(args, it / args.n_blocks);
+  for (Items<NT, KIND> item(args, c.first, c.items, c.step); item.take(); item.it += c.step) {
+    const Tile t = item.t;
     for (int r0 = 0; r0 < t.rows; r0 += NT) {
       const int n_mma = (min(NT, t.rows - r0) + 15) & ~15;
       const uint32_t idesc = idesc_bf16_f32(128, n_mma);
@@ -435,8 +460,8 @@ __device__ __forceinline__ void decode(const Args &args, const Ctx &c, int grp, 
   a.next(C::BS, grp);
   int skip = grp;   // blocks until this group's next one
   int block = grp;  // of all this CTA's blocks
-  for (int it = c.first; it < c.items; it += c.step) {
-    const Tile t = tile_of<NT, KIND>(args, it / args.n_blocks);
+  for (Items<NT, KIND> item(args, c.first, c.items, c.step); item.take(); item.it += c.step) {
+    const Tile t = item.t;
     for (int r0 = 0; r0 < t.rows; r0 += NT) {
       int kb = c.kb0 + skip;
 #pragma unroll C::UNROLL
@@ -511,12 +536,30 @@ __device__ __forceinline__ void promote(const Args &args, const Ctx &c, int half
   Ring d;
   int block = 0;
   uint32_t red_phase = 0, out_phase = 0;
-  for (int it = c.first; it < c.items; it += c.step) {
-    const Tile t = tile_of<NT, KIND>(args, it / args.n_blocks);
-    const int fb = it % args.n_blocks;
+  for (Items<NT, KIND> item(args, c.first, c.items, c.step); item.take(); item.it += c.step) {
+    const Tile t = item.t;
+    const int fb = item.block();
     for (int r0 = 0; r0 < t.rows; r0 += NT) {
       const int rows = min(NT, t.rows - r0);
       const int n_mma = (rows + 15) & ~15;
+      // Routes and weights of the tile's rows are fetched before its products;
+      // the hand-over of the output rows orders them for the other warps.
+      const uint32_t s_route = c.s_route + out_phase * (8 * NT);
+      if (KIND == kDown) {
+        const int n = (half * 4 + q) * 32 + lane;
+        if (n < rows) {
+          int32_t route = args.row_route[t.rb + r0 + n];
+          float weight = 0.f;
+          if (route < 0 || route >= args.num_routes) {
+            atomicOr(&g_status, kStatusIndex);
+            route = -1;
+          } else {
+            weight = __bfloat162float(args.route_w[route]);
+          }
+          asm volatile("st.shared.s32 [%0], %1;" ::"r"(s_route + n * 4), "r"(route) : "memory");
+          st_shared(s_route + (NT + n) * 4, weight);
+        }
+      }
       uint64_t acc2[C::NCH][C::C / 2];  // pairs of neighbouring columns
 #pragma unroll
       for (int i = 0; i < C::NCH; ++i)
@@ -657,17 +700,14 @@ __device__ __forceinline__ void promote(const Args &args, const Ctx &c, int half
         for (int i = 0; i < C::NCH; ++i) {
           const int col = (C::PG * i + half) * C::C;
           if (col < n_mma) {
-            // Lane j knows the weight of column col + j.
-            float weight = 0.f;
-            if (lane < C::C && col + lane < rows) {
-              const int32_t route = args.row_route[row0 + col + lane];
-              if (route >= 0 && route < args.num_routes)
-                weight = __bfloat162float(args.route_w[route]);
-            }
 #pragma unroll
-            for (int j = 0; j < C::C; ++j)
-              st_shared(c.s_out + (col + j) * C::OUT_ROW + row * 4,
-                        acc[i][j] * __shfl_sync(0xffffffffu, weight, j));
+            for (int j = 0; j < C::C; ++j) {
+              float weight;  // of a column past the tile's rows: unused
+              asm volatile("ld.shared.f32 %0, [%1];"
+                           : "=f"(weight)
+                           : "r"(s_route + (NT + col + j) * 4));
+              st_shared(c.s_out + (col + j) * C::OUT_ROW + row * 4, acc[i][j] * weight);
+            }
           }
         }
       } else {
@@ -712,11 +752,10 @@ __device__ __forceinline__ void promote(const Args &args, const Ctx &c, int half
           if (n < rows && mine) {
             int64_t to = row0 + n;
             if (KIND == kDown) {
-              to = args.row_route[to];
-              if (to < 0 || to >= args.num_routes) {
-                atomicOr(&g_status, kStatusIndex);
-                continue;
-              }
+              int32_t route;
+              asm volatile("ld.shared.s32 %0, [%1];" : "=r"(route) : "r"(s_route + n * 4));
+              if (route < 0) continue;
+              to = route;
             }
             uint4 v;
             asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
@@ -749,8 +788,9 @@ __global__ void __launch_bounds__(Cfg<NT, GPB, KIND>::THREADS, 1)
   uint8_t *s_red = s_w + args.ws * c.wbytes;  // [split - 1][NT][128] fp32
   uint8_t *s_out = s_red + (split - 1) * NT * 512;  // [NT] output rows
   uint8_t *s_scale = s_out + C::OUT_BYTES;
-  uint64_t *bars = reinterpret_cast<uint64_t *>(s_scale + C::SCALE_BYTES);
+  uint64_t *bars = reinterpret_cast<uint64_t *>(s_scale + C::SCALE_BYTES + C::ROUTE_BYTES);
   c.s_scale = smem_u32(s_scale);
+  c.s_route = c.s_scale + C::SCALE_BYTES;
   c.s_out = smem_u32(s_out);
   c.s_b = smem_u32(smem);
   c.s_w = smem_u32(s_w);
@@ -879,7 +919,7 @@ int launch(const CUtensorMap &mx, const CUtensorMap &mwhole, Args a, double item
     }
   }
   a.split = best;
-  const int64_t fixed = static_cast<int64_t>(C::BS) * C::B_BYTES + C::OUT_BYTES + C::SCALE_BYTES +
+  const int64_t fixed = static_cast<int64_t>(C::BS) * C::B_BYTES + C::OUT_BYTES + C::SCALE_BYTES + C::ROUTE_BYTES +
                         static_cast<int64_t>(a.split - 1) * NT * 512 + TAIL_BYTES;
   a.ws = static_cast<int>((SMEM_LIMIT - fixed) / a.sh.block_bytes());
   if (a.ws > MAX_WS) a.ws = MAX_WS;
