@@ -536,28 +536,32 @@ __device__ __forceinline__ void promote(const Args &args, const Ctx &c, int half
   Ring d;
   int block = 0;
   uint32_t red_phase = 0, out_phase = 0;
+  const int mine = (half * 4 + q) * 32 + lane;  // of a tile's rows
+  int32_t next_route = -1;
+  bool ahead = false;
   for (Items<NT, KIND> item(args, c.first, c.items, c.step); item.take(); item.it += c.step) {
     const Tile t = item.t;
     const int fb = item.block();
     for (int r0 = 0; r0 < t.rows; r0 += NT) {
       const int rows = min(NT, t.rows - r0);
       const int n_mma = (rows + 15) & ~15;
-      // Routes and weights of the tile's rows are fetched before its products;
-      // the hand-over of the output rows orders them for the other warps.
-      const uint32_t s_route = c.s_route + out_phase * (8 * NT);
+      // Route and weight of row `mine`: the route was asked for one item ago (of
+      // a tile's first rows), the weight is asked for before the products.
+      int32_t route = -1;
+      __nv_bfloat16 weight = __float2bfloat16_rn(0.f);
       if (KIND == kDown) {
-        const int n = (half * 4 + q) * 32 + lane;
-        if (n < rows) {
-          int32_t route = args.row_route[t.rb + r0 + n];
-          float weight = 0.f;
+        if (mine < rows) {
+          route = r0 == 0 && ahead ? next_route : args.row_route[t.rb + r0 + mine];
           if (route < 0 || route >= args.num_routes) {
             atomicOr(&g_status, kStatusIndex);
             route = -1;
           } else {
-            weight = __bfloat162float(args.route_w[route]);
+            weight = args.route_w[route];
           }
-          asm volatile("st.shared.s32 [%0], %1;" ::"r"(s_route + n * 4), "r"(route) : "memory");
-          st_shared(s_route + (NT + n) * 4, weight);
+        }
+        if (r0 == 0) {
+          ahead = item.it + item.step < item.items;
+          if (ahead && mine < item.next.rows) next_route = args.row_route[item.next.rb + mine];
         }
       }
       uint64_t acc2[C::NCH][C::C / 2];  // pairs of neighbouring columns
@@ -658,7 +662,12 @@ __device__ __forceinline__ void promote(const Args &args, const Ctx &c, int half
       // column of 32 features per store, a tile took longer than its six
       // blocks of products; a bulk copy per row, issued lane by lane, too.)
       const bool staged = args.staged != 0;
+      const uint32_t s_route = c.s_route + out_phase * (8 * NT);
       if (staged) {
+        if (KIND == kDown && mine < rows) {
+          asm volatile("st.shared.s32 [%0], %1;" ::"r"(s_route + mine * 4), "r"(route) : "memory");
+          st_shared(s_route + (NT + mine) * 4, __bfloat162float(weight));
+        }
         // The rows of the item before have been read, by every warp.
         __syncwarp();
         if (lane == 0) mbar_arrive(c.out_free);
@@ -701,13 +710,8 @@ __device__ __forceinline__ void promote(const Args &args, const Ctx &c, int half
           const int col = (C::PG * i + half) * C::C;
           if (col < n_mma) {
 #pragma unroll
-            for (int j = 0; j < C::C; ++j) {
-              float weight;  // of a column past the tile's rows: unused
-              asm volatile("ld.shared.f32 %0, [%1];"
-                           : "=f"(weight)
-                           : "r"(s_route + (NT + col + j) * 4));
-              st_shared(c.s_out + (col + j) * C::OUT_ROW + row * 4, acc[i][j] * weight);
-            }
+            for (int j = 0; j < C::C; ++j)
+              st_shared(c.s_out + (col + j) * C::OUT_ROW + row * 4, acc[i][j]);
           }
         }
       } else {
@@ -752,15 +756,23 @@ __device__ __forceinline__ void promote(const Args &args, const Ctx &c, int half
           if (n < rows && mine) {
             int64_t to = row0 + n;
             if (KIND == kDown) {
-              int32_t route;
-              asm volatile("ld.shared.s32 %0, [%1];" : "=r"(route) : "r"(s_route + n * 4));
-              if (route < 0) continue;
-              to = route;
+              int32_t r;
+              asm volatile("ld.shared.s32 %0, [%1];" : "=r"(r) : "r"(s_route + n * 4));
+              if (r < 0) continue;
+              to = r;
             }
             uint4 v;
             asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                          : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                          : "r"(c.s_out + n * C::OUT_ROW + (lane % LANES) * 16));
+            if (KIND == kDown) {
+              float w;
+              asm volatile("ld.shared.f32 %0, [%1];" : "=f"(w) : "r"(s_route + (NT + n) * 4));
+              v.x = __float_as_uint(__uint_as_float(v.x) * w);
+              v.y = __float_as_uint(__uint_as_float(v.y) * w);
+              v.z = __float_as_uint(__uint_as_float(v.z) * w);
+              v.w = __float_as_uint(__uint_as_float(v.w) * w);
+            }
             *reinterpret_cast<uint4 *>(out + to * (static_cast<int64_t>(args.n_out) * SIZE)) = v;
           }
         }
