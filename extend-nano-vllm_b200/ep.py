@@ -135,7 +135,7 @@ def _exchange(layer, x: torch.Tensor) -> torch.Tensor:
     if tokens:
         layer._check_inputs(x)
         logits = layer.gate(x)
-        weights, ids = ops.route_topk(logits, top_k, layer.norm_topk_prob)
+        weights, ids = layer._select(logits)
     else:
         weights = torch.empty((0, top_k), device=device, dtype=torch.bfloat16)
         ids = torch.empty((0, top_k), device=device, dtype=torch.int64)
@@ -258,8 +258,7 @@ class NvlinkExchange:
         k = layer.top_k
         if self.tokens:
             layer._check_inputs(x)
-            self.weights, self.ids = layer._ops.route_topk(layer.gate(x), k,
-                                                           layer.norm_topk_prob)
+            self.weights, self.ids = layer._select(layer.gate(x))
         else:
             self.weights = torch.empty((0, k), device=x.device, dtype=torch.bfloat16)
             self.ids = torch.empty((0, k), device=x.device, dtype=torch.int64)

@@ -18,7 +18,10 @@ Differences from the reference, by design:
   * the unfused grouped-GEMM seam ``_run_grouped_gemm`` does not exist (gate/up
     and SwiGLU are one kernel), nor does the per-expert torch loop
     ``_forward_reference`` (correctness oracles live with the tests);
-  * bf16 activations and weights only.
+  * bf16 activations; weights are bf16, or 4-bit with group scales after
+    ``quantize_w4`` / ``set_w4_weights`` (one EP rank);
+  * optionally, routing by scores with a selection bias and expert groups
+    instead of the plain softmax top-k (``set_scored_routing``).
 """
 
 from __future__ import annotations
@@ -122,8 +125,38 @@ class SharedExpertMLP(nn.Module):
         self.intermediate_size = intermediate_size
         self.gate_up_proj = SharedMergedGate(hidden_size, intermediate_size)
         self.down_proj = ReplicatedGate(intermediate_size, hidden_size)
+        self._w4: tuple[_native_ops.W4Weight, _native_ops.W4Weight] | None = None
+
+    def set_w4_weights(self, gate_up: _native_ops.W4Weight, down: _native_ops.W4Weight) -> None:
+        """Use 4-bit weights (packed in the "rows" layout: [2 I_s, H] with the
+        gate rows first, and [H, I_s]) and release the bf16 ones."""
+        hidden = self.gate_up_proj.input_size
+        for weight, rows, k in ((gate_up, 2 * self.intermediate_size, hidden),
+                                (down, hidden, self.intermediate_size)):
+            if (weight.matrices, weight.rows, weight.k) != (1, rows, k) \
+                    or weight.flags & _lib.W4_GATE_UP:
+                raise ValueError(f"the shared expert needs a [{rows}, {k}] weight in the "
+                                 "\"rows\" layout")
+        self._w4 = (gate_up, down)
+        for linear in (self.gate_up_proj, self.down_proj):
+            linear.weight.data = linear.weight.data.new_empty((0, linear.input_size))
+
+    @torch.no_grad()
+    def quantize_w4(self, group: int = 128, zeros: bool = False) -> None:
+        """Round the weights to 4 bits with group scales (``ops.quantize_w4``)."""
+        self.set_w4_weights(*(_native_ops.pack_w4(*_native_ops.quantize_w4(w, group, zeros))
+                              for w in (self.gate_up_proj.weight, self.down_proj.weight)))
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        for weight in self._w4 or ():
+            weight.data = fn(weight.data)
+        return self
 
     def forward(self, hidden_states: torch.Tensor) -> torch.Tensor:
+        if self._w4 is not None:
+            gate, up = _native_ops.linear_w4(hidden_states, self._w4[0]).chunk(2, dim=-1)
+            return _native_ops.linear_w4(F.silu(gate) * up, self._w4[1])
         gate, up = self.gate_up_proj(hidden_states).chunk(2, dim=-1)
         return self.down_proj(F.silu(gate) * up)
 
@@ -262,6 +295,12 @@ class ExpertParallelMoE(nn.Module):
         # by one unit and with it the routing of that token.
         self.fuse_router_gate = False
 
+        # Scored routing (set_scored_routing) and 4-bit expert weights
+        # (quantize_w4, set_w4_weights); None: softmax top-k, bf16 weights.
+        self._scored: dict | None = None
+        self.register_buffer("route_bias", None, persistent=False)
+        self._w4: tuple[_native_ops.W4Weight, _native_ops.W4Weight] | None = None
+
         # Kernel entry points; tests may substitute an object with the same
         # functions to exercise the host logic without a GPU.
         self._ops = _native_ops
@@ -339,9 +378,104 @@ class ExpertParallelMoE(nn.Module):
         # Device and dtype moves rebuild every parameter separately; put the
         # shared expert back behind the routed experts afterwards.
         super()._apply(fn, recurse)
-        if getattr(self, "_shared_in_store", False):
+        if getattr(self, "_shared_in_store", False) and self._w4 is None:
             self._bind_shared_store()
+        for weight in self._w4 or ():
+            weight.data = fn(weight.data)
+        if self.route_bias is not None and self.route_bias.dtype != torch.float32:
+            self.route_bias = self.route_bias.float()  # scores stay fp32
         return self
+
+    # ------------------------------------------------------------------
+    # Scored routing and 4-bit weights.
+    # ------------------------------------------------------------------
+    def set_scored_routing(self, score: str = "sigmoid", bias: torch.Tensor | None = None,
+                           num_groups: int = 1, topk_groups: int = 1,
+                           group_score: str = "top2", scale: float = 1.0) -> None:
+        """Route by ``ops.route_scored_topk`` instead of the softmax top-k:
+        sigmoid or softmax scores, a selection bias (fp32 [E]), expert groups and
+        a weight scale; ``norm_topk_prob`` says whether the chosen scores are
+        renormalised."""
+        if score not in _lib.SCORE_CODES:
+            raise ValueError(f"unknown score function {score!r}")
+        if group_score not in _lib.GROUP_SCORE_CODES:
+            raise ValueError(f"unknown group score {group_score!r}")
+        if num_groups < 1 or self.num_experts % num_groups:
+            raise ValueError("num_groups must divide the number of experts")
+        if not 1 <= topk_groups <= num_groups:
+            raise ValueError("topk_groups must be between 1 and num_groups")
+        if self.top_k > topk_groups * (self.num_experts // num_groups):
+            raise ValueError("top_k exceeds the experts of topk_groups groups")
+        if bias is not None and bias.shape != (self.num_experts,):
+            raise ValueError("bias must have one value per expert")
+        self.route_bias = (None if bias is None
+                           else bias.detach().to(device=self.gate.weight.device,
+                                                 dtype=torch.float32).clone())
+        self._scored = dict(score=score, num_groups=num_groups, topk_groups=topk_groups,
+                            group_score=group_score, scale=float(scale))
+
+    def set_w4_weights(self, w13: _native_ops.W4Weight, w2: _native_ops.W4Weight) -> None:
+        """Run the experts with 4-bit weights (``ops.pack_w4``: w13 [E, 2 I, H] in
+        the "gate_up" layout, w2 [E, H, I]) and release the bf16 ones.  One EP
+        rank; the layer's weights can no longer be loaded or relocated."""
+        if self.ep_size != 1:
+            raise NotImplementedError("4-bit expert weights need one EP rank")
+        if self.fp64_combine:
+            raise NotImplementedError("4-bit expert weights have no FP64 combine")
+        hidden, inter = self.hidden_size, self.intermediate_size
+        if (w13.matrices, w13.rows, w13.k) != (self.num_experts, 2 * inter, hidden) \
+                or not w13.flags & _lib.W4_GATE_UP:
+            raise ValueError(f"w13 must be {self.num_experts} x [{2 * inter}, {hidden}] in the "
+                             "\"gate_up\" layout")
+        if (w2.matrices, w2.rows, w2.k) != (self.num_experts, hidden, inter) \
+                or w2.flags & _lib.W4_GATE_UP:
+            raise ValueError(f"w2 must be {self.num_experts} x [{hidden}, {inter}] in the "
+                             "\"rows\" layout")
+        self._w4 = (w13, w2)
+        if self._shared_in_store and self.shared_expert._w4 is None:
+            # The shared expert keeps its weights without the routed experts'.
+            shared = self.shared_expert
+            for linear in (shared.gate_up_proj, shared.down_proj):
+                linear.weight.data = linear.weight.data.clone()
+        self.gate_up_proj.data = self.gate_up_proj.data.new_empty((0, 2 * inter, hidden))
+        self.down_proj.data = self.down_proj.data.new_empty((0, hidden, inter))
+
+    @torch.no_grad()
+    def quantize_w4(self, group: int = 128, zeros: bool = False) -> None:
+        """Round the experts' weights, and the shared expert's, to 4 bits with
+        group scales (``ops.quantize_w4``) and release the bf16 ones."""
+        if self.ep_size != 1:
+            raise NotImplementedError("4-bit expert weights need one EP rank")
+        parts = []
+        for param in (self.gate_up_proj, self.down_proj):
+            # One expert at a time: the fp32 intermediate stays small.
+            experts = [_native_ops.quantize_w4(w, group, zeros) for w in param]
+            parts.append([None if t[0] is None else torch.stack(t) for t in zip(*experts)])
+        if self.shared_expert is not None:  # first: it may refuse the group size
+            self.shared_expert.quantize_w4(group, zeros)
+        self.set_w4_weights(_native_ops.pack_w4(*parts[0], layout="gate_up"),
+                            _native_ops.pack_w4(*parts[1]))
+
+    def _select(self, logits: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """Router logits -> (bf16 weights, int64 ids) [T, k]."""
+        if self._scored is not None:
+            return self._ops.route_scored_topk(logits, self.top_k, bias=self.route_bias,
+                                               renormalize=self.norm_topk_prob, **self._scored)
+        return self._ops.route_topk(logits, self.top_k, self.norm_topk_prob)
+
+    def _forward_w4(self, x: torch.Tensor, logits: torch.Tensor) -> torch.Tensor:
+        """Routing, capacity and the experts with 4-bit weights."""
+        weights, ids = self._select(logits)
+        capacity = self._capacity(x.size(0))
+        if capacity is not None:
+            # Packing rewrites dropped routes (id E, weight 0) and counts them.
+            self._pack(ids.view(-1), weights.view(-1), capacity=capacity,
+                       stats=self._device_stats(x.device))
+        elif not _capturing():
+            self._host_counts["dispatch"] += ids.numel()
+            self._host_counts["return"] += ids.numel()
+        self.total_assignment_count += ids.numel()
+        return self._ops.experts_w4(x, ids, weights, *self._w4)
 
     def _shared_store(self) -> tuple[torch.Tensor, torch.Tensor]:
         """[E_loc + 1, 2I, H] and [E_loc + 1, H, I] views over the routed and
@@ -365,7 +499,7 @@ class ExpertParallelMoE(nn.Module):
         it once per rank after the exchange), the native kernels."""
         return (self.shared_expert is not None and getattr(self, "_shared_in_store", False)
                 and self.fuse_shared_expert and self.ep_size == 1 and self._ops is _native_ops and x.is_cuda
-                and self.top_k < 32)
+                and self.top_k < 32 and self._scored is None and self._w4 is None)
 
     # ------------------------------------------------------------------
     # Counters (moe.py:384-393).  Kernels accumulate local assignments and
@@ -427,6 +561,8 @@ class ExpertParallelMoE(nn.Module):
     # ------------------------------------------------------------------
     @property
     def expert_parameter_bytes(self) -> int:
+        if self._w4 is not None:
+            return sum(w.data.numel() for w in self._w4)
         return sum(p.numel() * p.element_size() for p in (self.gate_up_proj, self.down_proj))
 
     def owns_expert(self, expert_id: int) -> bool:
@@ -442,6 +578,8 @@ class ExpertParallelMoE(nn.Module):
                            loaded_weight: torch.Tensor) -> None:
         if not self.owns_expert(expert_id):
             return
+        if self._w4 is not None:
+            raise RuntimeError("the experts hold 4-bit weights (set_w4_weights)")
         local = self._local_id(expert_id)
         if projection == "gate_proj":
             target = self.gate_up_proj[local, : self.intermediate_size]
@@ -465,6 +603,8 @@ class ExpertParallelMoE(nn.Module):
         """
         if not self.dynamic_placement:
             raise RuntimeError("runtime expert placement was not enabled")
+        if self._w4 is not None:
+            raise NotImplementedError("4-bit expert weights are not relocated")
         owners = tuple(expert_owners)
         if (len(owners) != self.num_experts
                 or any(type(o) is not int or not 0 <= o < self.ep_size for o in owners)
@@ -576,7 +716,7 @@ class ExpertParallelMoE(nn.Module):
     def _use_tiny_path(self, num_tokens: int, logits: torch.Tensor) -> bool:
         """Two-launch fused path: tiny buckets, no capacity, plain bf16 combine."""
         return (self.expert_engine == "auto" and self._ops is _native_ops
-                and num_tokens * self.top_k <= _native_ops.TINY_MAX_ROUTES
+                and self._scored is None and num_tokens * self.top_k <= _native_ops.TINY_MAX_ROUTES
                 and self.expert_capacity is None and self.expert_capacity_factor is None
                 and not self.fp64_combine and not self.fp32_reduce
                 and logits.dtype in (torch.float32, torch.bfloat16))
@@ -667,7 +807,7 @@ class ExpertParallelMoE(nn.Module):
     def _route(self, hidden_states: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """Router + capacity (moe.py:870-920) -> (bf16 weights [T,k], int64 ids [T,k])."""
         logits = self.gate(hidden_states)
-        weights, experts = self._ops.route_topk(logits, self.top_k, self.norm_topk_prob)
+        weights, experts = self._select(logits)
         capacity = self._capacity(hidden_states.size(0))
         if capacity is not None:
             packed = self._pack(experts.view(-1), weights.view(-1), capacity=capacity)
@@ -692,6 +832,10 @@ class ExpertParallelMoE(nn.Module):
         num_tokens = hidden_states.size(0)
         top_k = selected_experts.size(1)
         ids = selected_experts.contiguous()
+        if self._w4 is not None:
+            local = (0 if _capturing()
+                     else int(((ids >= 0) & (ids < self.num_experts)).sum()))
+            return self._ops.experts_w4(hidden_states, ids, routing_weights, *self._w4), local
         weights = routing_weights.contiguous().view(-1)
         packed = self._pack(ids.view(-1), None)
         y = self._run_experts(hidden_states.contiguous(), weights, packed, top_k)
@@ -721,6 +865,7 @@ class ExpertParallelMoE(nn.Module):
         if x.size(0) == 0:
             return torch.zeros_like(x)
         if (self.fuse_router_gate and not shared and self._ops is _native_ops and x.is_cuda
+                and self._scored is None and self._w4 is None
                 and x.size(0) <= _native_ops.ROUTE_GATE_MAX_TOKENS
                 and x.dtype == torch.bfloat16 and self.gate.weight.dtype == torch.bfloat16):
             return self._forward_fused_gate(x)
@@ -751,6 +896,8 @@ class ExpertParallelMoE(nn.Module):
         if num_tokens == 0:
             return torch.zeros_like(x)
         self._check_inputs(x)
+        if self._w4 is not None:
+            return self._forward_w4(x, logits)
         stats = self._device_stats(x.device)
         if shared:
             return self._forward_with_shared(x, logits, stats)
@@ -762,7 +909,8 @@ class ExpertParallelMoE(nn.Module):
                 logits, x.contiguous(), self.gate_up_proj, self.down_proj, self.top_k,
                 self.norm_topk_prob, self.num_experts, local_index=local_index,
                 expert_start=max(self.expert_start, 0), stats=stats)
-        if (self._ops is _native_ops and num_tokens <= ROUTE_PACK_MAX_TOKENS
+        if (self._ops is _native_ops and self._scored is None
+                and num_tokens <= ROUTE_PACK_MAX_TOKENS
                 and num_tokens * self.top_k <= _native_ops.ROUTE_PACK_MAX_ROUTES
                 and self.num_experts <= 1024 and self.top_k <= 32):
             # Small batches: router and packing in one launch (same results).
@@ -774,7 +922,7 @@ class ExpertParallelMoE(nn.Module):
                 expert_start=max(self.expert_start, 0), capacity=self._capacity(num_tokens),
                 stats=stats)
         else:
-            weights, ids = self._ops.route_topk(logits, self.top_k, self.norm_topk_prob)
+            weights, ids = self._select(logits)
             packed = self._pack(ids.view(-1), weights.view(-1),
                                 capacity=self._capacity(num_tokens), stats=stats)
         flat_w = weights.view(-1)
