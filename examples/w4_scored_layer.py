@@ -1,4 +1,4 @@
-"""One MoE layer as a DeepSeek-style checkpoint has it, served with 4-bit weights:
+"""One MoE layer with a scored router, served with 4-bit weights:
 sigmoid scores with a balance bias, 8 expert groups of which 4 are on offer,
 top-8, and a shared expert of another width than the routed ones.
 

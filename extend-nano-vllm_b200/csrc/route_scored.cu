@@ -29,6 +29,8 @@ struct ScoredArgs {
   int topk_groups;
   int group_size;   // num_experts / groups
   int group_lanes;  // largest power of two <= 32 / groups
+  uint32_t group_mul;  // expert * group_mul >> 20 is its group
+  int group_pad;    // places between groups in shared memory
   int top2;
   int renormalize;
   float scale;
@@ -46,7 +48,12 @@ __device__ __forceinline__ uint32_t order_key(float v) {
 template <typename T, int VPL>
 __global__ void __launch_bounds__(32 * kWarps) route_scored_kernel(const T *logits,
                                                                    const ScoredArgs a) {
-  extern __shared__ float s_choice[];  // [kWarps][num_experts], only with groups
+  // With groups: [kWarps] choice values, each group group_pad places after the
+  // one before, so that the lanes that look through the groups side by side
+  // meet different banks.
+  extern __shared__ float s_choice[];
+  __shared__ float s_sel[kWarps][32];
+  __shared__ int s_id[kWarps][32];
   pdl_trigger();
   pdl_wait();
   const int lane = threadIdx.x & 31;
@@ -54,15 +61,18 @@ __global__ void __launch_bounds__(32 * kWarps) route_scored_kernel(const T *logi
   const int64_t token = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
   if (token >= a.num_tokens) return;
   const T *row = logits + token * a.num_experts;
-  float s[VPL];
+  float s[VPL], bias[VPL];
   bool live[VPL];
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
     const int e = lane + 32 * i;
     live[i] = e < a.num_experts;
     const float v = live[i] ? to_f32(row[e]) : -INFINITY;
+    bias[i] = live[i] && a.bias ? a.bias[e] : 0.f;
     s[i] = v == v ? v : -INFINITY;
   }
+  const int stretch = a.num_experts + a.groups * a.group_pad;
+  float *choice = s_choice + warp * stretch;
   if (a.sigmoid) {
 #pragma unroll
     for (int i = 0; i < VPL; ++i) s[i] = 1.0f / (1.0f + expf(-s[i]));
@@ -86,10 +96,11 @@ __global__ void __launch_bounds__(32 * kWarps) route_scored_kernel(const T *logi
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
     const int e = lane + 32 * i;
-    float c = live[i] ? s[i] + (a.bias ? a.bias[e] : 0.f) : -INFINITY;
+    float c = live[i] ? s[i] + bias[i] : -INFINITY;
     c = c == c ? c : -INFINITY;
     key[i] = live[i] ? order_key(c) : 0u;
-    if (a.groups > 1 && live[i]) s_choice[warp * a.num_experts + e] = c;
+    if (a.groups > 1 && live[i])
+      choice[e + static_cast<int>((e * a.group_mul) >> 20) * a.group_pad] = c;
   }
   if (a.groups > 1) {
     // group_lanes lanes look through one group, then merge their two largest.
@@ -99,7 +110,7 @@ __global__ void __launch_bounds__(32 * kWarps) route_scored_kernel(const T *logi
     const int size = a.group_size;
     float best = -INFINITY, second = -INFINITY;
     if (group < a.groups) {
-      const float *c = s_choice + warp * a.num_experts + group * size;
+      const float *c = choice + group * (size + a.group_pad);
       for (int i = lane % width; i < size; i += width) {
         const float v = c[i];
         second = fmaxf(second, fminf(best, v));
@@ -125,16 +136,16 @@ __global__ void __launch_bounds__(32 * kWarps) route_scored_kernel(const T *logi
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
       const int e = lane + 32 * i;
-      if (live[i] && !((mask >> (e / size * width)) & 1u)) key[i] = 0u;
+      if (live[i] && !((mask >> (((e * a.group_mul) >> 20) * width)) & 1u)) key[i] = 0u;
     }
   }
-  float sel = 0.f;
-  int sel_id = 0;
-  float total = 0.f;
-  for (int slot = 0; slot < a.top_k; ++slot) {
-    uint32_t bk = 0u;
-    int bi = 0;
-    float bs = 0.f;
+  // top_k rounds: the largest key of the warp; among lanes that hold it, the
+  // lowest expert.  Its lane notes the choice and looks for its next best.
+  uint32_t bk = 0u;
+  int bi = 0;
+  float bs = 0.f;
+  auto best_of_lane = [&]() {
+    bk = 0u;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
       if (key[i] > bk) {
@@ -143,30 +154,43 @@ __global__ void __launch_bounds__(32 * kWarps) route_scored_kernel(const T *logi
         bs = s[i];
       }
     }
+  };
+  best_of_lane();
+  for (int slot = 0; slot < a.top_k; ++slot) {
     const uint32_t kmax = __reduce_max_sync(0xffffffffu, bk);
-    const uint32_t mine = bk == kmax ? static_cast<uint32_t>(lane + 32 * bi) : 0xffffffffu;
-    const uint32_t win = __reduce_min_sync(0xffffffffu, mine);
-    bs = __shfl_sync(0xffffffffu, bs, static_cast<int>(win & 31u));
-#pragma unroll
-    for (int i = 0; i < VPL; ++i)
-      if (lane + 32 * i == static_cast<int>(win)) key[i] = 0u;
-    total += bs;
-    if (lane == slot) {
-      sel = bs;
-      sel_id = static_cast<int>(win);
+    const unsigned who = __ballot_sync(0xffffffffu, bk == kmax);
+    bool mine = bk == kmax;
+    if (who & (who - 1)) {
+      const uint32_t id = mine ? static_cast<uint32_t>(lane + 32 * bi) : 0xffffffffu;
+      mine = __reduce_min_sync(0xffffffffu, id) == static_cast<uint32_t>(lane + 32 * bi) && mine;
     }
+    if (mine) {
+      s_sel[warp][slot] = bs;
+      s_id[warp][slot] = lane + 32 * bi;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        if (i == bi) key[i] = 0u;
+      best_of_lane();
+    }
+    __syncwarp();
   }
+  const float sel = lane < a.top_k ? s_sel[warp][lane] : 0.f;
+  if (lane < a.top_k) {
+    const int64_t at = token * a.top_k + lane;
+    a.ids[at] = s_id[warp][lane];
+  }
+  const float total = warp_sum(sel);
   if (lane < a.top_k) {
     const float w = a.renormalize ? (total > 0.f ? sel / total : 0.f) : sel;
     a.weights[token * a.top_k + lane] = __float2bfloat16_rn(w * a.scale);
-    a.ids[token * a.top_k + lane] = sel_id;
   }
 }
 
 template <typename T>
 int launch_scored(const void *logits, const ScoredArgs &a, cudaStream_t stream) {
   const dim3 grid(static_cast<unsigned>((a.num_tokens + kWarps - 1) / kWarps));
-  const size_t smem = a.groups > 1 ? static_cast<size_t>(kWarps) * a.num_experts * 4 : 0;
+  const size_t smem = a.groups > 1 ? static_cast<size_t>(kWarps) * (a.num_experts + a.groups * a.group_pad) * 4
+                                    : 0;
   const int vpl = (a.num_experts + 31) / 32;
 #define B200_SCORED_CASE(V)                                                                  \
   if (vpl <= V) {                                                                            \
@@ -227,6 +251,9 @@ extern "C" int b200moe_route_scored_topk(const void *logits, int logits_dtype, i
   a.group_size = num_experts / num_groups;
   a.group_lanes = 32;
   while (a.group_lanes * num_groups > 32) a.group_lanes >>= 1;
+  // Exact for e * group_size < 2^20.
+  a.group_mul = (1u << 20) / static_cast<uint32_t>(a.group_size) + 1u;
+  a.group_pad = ((a.group_lanes - a.group_size) % 32 + 32) % 32;
   a.top2 = group_score == B200MOE_GROUP_TOP2;
   a.renormalize = renormalize;
   a.scale = scale;
