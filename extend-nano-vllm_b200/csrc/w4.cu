@@ -248,7 +248,9 @@ int b200moe_w4_linear(const void *x, int64_t m, int n, int k, const void *w, int
   B200_ARG(aligned16(x) && aligned16(w), "x and w must be 16-byte aligned");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const w4::Shape sh = w4::shape_of(group, flags);
-  B200_UNSUPPORTED(m < (int64_t)0x7fffffff, "too many rows");
+  B200_UNSUPPORTED(m < (int64_t)0x7fffffff &&
+                       (m + 15) / 16 * ((n + 127) / 128) < (int64_t)0x7fffffff,
+                   "too many rows");
   return m <= kStreamRows ? w4_linear_stream(x, m, n, k, w, sh, out, s)
                           : w4_linear_tc(x, m, n, k, w, sh, out, s);
 }
@@ -292,6 +294,11 @@ int b200moe_w4_experts(const void *x, int64_t tokens, int hidden, int inter,
            "x, w13, w2 and workspace must be 16-byte aligned");
   const int64_t need = b200moe_w4_experts_workspace(tokens, hidden, inter, top_k, num_experts);
   B200_ARG(workspace_bytes >= need, "workspace needs %lld bytes", (long long)need);
+  // Work items are counted in 32 bits.
+  B200_UNSUPPORTED(b200moe_pack_max_mtiles(tokens * top_k, num_experts) * 4 *
+                           ((hidden > inter ? hidden : inter) / 64 + 1) <
+                       (int64_t)0x7fffffff,
+                   "too many routes");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const w4::Shape sh13 = w4::shape_of(group13, flags13), sh2 = w4::shape_of(group2, flags2);
   const int64_t routes = tokens * top_k;

@@ -21,6 +21,14 @@
 // then decoding (groups of four, alternate blocks), then promoting and epilogue
 // (groups of four, alternate column chunks).
 // Every wait is bounded; on expiry the CTA records a status bit and leaves.
+//
+// What bounds it: instruction issue.  A block of 128 x 128 weights against 128
+// rows takes 590 cycles of matrix instructions (74 each; 37 at 16 rows) but some
+// 540 issue slots of each scheduler for decoding (seven ALU instructions of two
+// cycles per eight codes) and promoting, which do not overlap without gaps.
+// Measured (back to back): 32 rows x [75776, 4096] 52 us = 3.05 TB/s of weights,
+// 64 rows 58 us, 128 rows 83 us; 4096 rows x [4096, 4096] 132 us = 1.04 PFLOP/s
+// (cuBLAS bf16 burst 1.64); groups of 32 with zero points, 64 rows: 91 us.
 #include <cudaTypedefs.h>
 
 #include <type_traits>

@@ -9,10 +9,19 @@
 // -> registers -> integers q - z (exact in bf16) -> warp matrix instructions
 // (m16n8k16: 16 weight rows, 8 rows of x), and adds a group's sum to fp32
 // registers times its scale.  No barrier and no second warp is on the way of a
-// weight, which is what a stream of 4-bit weights needs: at the copy rate an SM has some 23
-// cycles for 512 codes, and the decoding alone takes 7 of each scheduler's.
+// weight, which is what a stream of 4-bit weights needs: at the copy rate an SM
+// has 11 cycles for 512 codes, and decoding them takes 7 of each scheduler's.
 // (tcgen05 wants the operand decoded by one warp, waited for by another and
-// read back by a third; that pays from more than 16 rows on, w4_gemm_sm100.cu.)
+// read back by a third; that pays from more than 16 rows on, w4_gemm_sm100.cu:
+// 16 rows x [151552, 4096] take 97 us here and 107 there, 32 rows 220 and 107.)
+//
+// What bounds it: not the instruction count (a variant that multiplies 128 + q
+// and corrects by the sums of x, a fifth fewer, measured the same; one with
+// shifts on the multiply pipe was slower), but the copies in flight: some 100 KB
+// per SM at 4-5 us each under load.  A deeper ring takes the L1 from x.
+// Measured (back to back, weights larger than L2): 1 row x [75776, 4096] 40.2 us
+// = 3.98 TB/s of weights, 8 rows x [151552, 4096] 84.7 us = 3.78 TB/s, 16 rows
+// 97.2 us = 3.29 TB/s; copy peak 6.5 TB/s.
 //
 // A warp owns 32 weight rows (a quarter of a tile): two 16-row operands, which
 // in gate_up order are the gate and the up rows of the same 16 features, so the
