@@ -66,6 +66,18 @@ def test_linear_shapes(m, n, k, group):
     check_linear(activations((m, k), n), ops.pack_w4(*parts), exact(*parts))
 
 
+@pytest.mark.parametrize("group,zeros", [(128, False), (64, True), (32, True)])
+@pytest.mark.parametrize("m,n,k", [(128, 38016, 128), (200, 19328, 384), (513, 7816, 320),
+                                   (1000, 4744, 1152)])
+def test_linear_many_tiles(m, n, k, group, zeros):
+    # Enough 128-row tiles that two CTAs work on a pair of weight tiles: an odd
+    # number of tiles, ragged rows and features, k inside a block.
+    if k % group:
+        pytest.skip("k is not a multiple of this group size")
+    parts = weight((n, k), group, zeros, seed=n)
+    check_linear(activations((m, k), n), ops.pack_w4(*parts), exact(*parts))
+
+
 @pytest.mark.parametrize("m", [1, 40])
 def test_linear_fp16_scales(m):
     parts = weight((140, 256), 64, True, seed=3, scale_dtype=torch.float16)
@@ -167,6 +179,19 @@ def test_experts_odd_shapes(hidden, inter, experts, top_k, tokens):
     parts13 = weight((experts, 2 * inter, hidden), 32, True, seed=hidden)
     parts2 = weight((experts, hidden, inter), 32, False, seed=inter)
     ids, weights = routed(tokens, experts, top_k, tokens)
+    check_experts(activations((tokens, hidden), 1), ids, weights, parts13, parts2)
+
+
+@pytest.mark.parametrize("group,zeros", [(128, False), (32, True)])
+@pytest.mark.parametrize("hidden,inter,experts,top_k,tokens", [
+    (1152, 640, 4, 2, 1000), (640, 128, 8, 2, 4100), (2048, 384, 6, 3, 1030)])
+def test_experts_prefill(hidden, inter, experts, top_k, tokens, group, zeros):
+    # Hundreds of rows per expert: whole tiles, part tiles, pairs of CTAs, and
+    # (with 4100 tokens and two routes each) the packing of many routes.
+    parts13 = weight((experts, 2 * inter, hidden), group, zeros, seed=hidden)
+    parts2 = weight((experts, hidden, inter), group, False, seed=inter)
+    ids, weights = routed(tokens, experts, top_k, tokens)
+    ids[7] = experts  # a token that was dropped
     check_experts(activations((tokens, hidden), 1), ids, weights, parts13, parts2)
 
 
