@@ -44,6 +44,30 @@ constexpr int64_t kRouteRoutes = 16;
 // instead of reading a packed copy.
 constexpr int64_t kGatherRoutes = 512;
 
+// Rows of the tiles that an expert product is cut into, from the rows to expect
+// of a fuller expert (`rows`: half as many again as the mean, and eight).  A tile
+// that is too small costs passes over the weights, one that is too large costs
+// time only by the hand-over of each group's accumulators, so that large groups
+// want large tiles.  Measured with 128 experts, top-8, the whole call in us with
+// tiles of 16 (streaming) / 32 / 64 / 128 rows:
+//   g 128: 64 tokens 137 / 165 / 177 / 171, 96 164 / 162 / 168 / 160,
+//          256 336 / 207 / 197 / 175, 509 483 / 276 / 225 / 197
+//   g 64:  96 tokens 182 / 161 / 190 / 188, 192 314 / 196 / 199 / 196, 256 374 /
+//          214 / 217 / 203, 509 536 / 288 / 256 / 229
+//   g 32:  96 tokens 189 / 177 / 240 / 281, 384 499 / 282 / 307 / 331, 509 568 /
+//          323 / 317 / 346, 768 796 / 438 / 388 / 377
+// Eight columns (streaming) against sixteen: 64 tokens over 512 experts, top-10
+// (1.25 rows on average) 174 against 185, 64 over 128 149 against 137.
+int64_t tile_rows(int64_t rows, const w4::Shape &sh) {
+  if (rows <= 10) return 8;
+  if (rows <= kStreamRows) return kStreamRows;
+  switch (sh.groups_per_block()) {
+    case 1: return 128;
+    case 2: return rows <= 26 ? 32 : 128;
+    default: return rows <= 50 ? 32 : rows <= 64 ? 64 : 128;
+  }
+}
+
 // Pieces of the workspace, each on a 256-byte boundary.
 struct Workspace {
   int64_t bytes = 0;
@@ -348,19 +372,19 @@ int b200moe_w4_experts(const void *x, int64_t tokens, int hidden, int inter,
   const double mean = static_cast<double>(routes) / num_experts;
   const double tiles = num_experts * (1.0 - exp(-mean)) + static_cast<double>(routes) / 128;
   const int64_t rows = min64(tokens, static_cast<int64_t>(1.5 * mean + 8.0));
-  if (rows <= kStreamRows) {
-    rc = w4_gate_up_stream(src, hidden, inter, w13, sh13, b.mtiles, b.max_mtiles, b.counters,
-                           tiles, rows, b.act, s);
-    if (rc) return rc;
-    rc = w4_down_stream(b.act, hidden, inter, w2, sh2, b.row_route, weights, routes, b.mtiles,
-                        b.max_mtiles, b.counters, tiles, rows, b.y, s);
-  } else {
-    rc = w4_gate_up_tc(src, hidden, inter, w13, sh13, b.row_capacity, b.mtiles, b.max_mtiles,
-                       b.counters, tiles, rows, b.act, s);
-    if (rc) return rc;
-    rc = w4_down_tc(b.act, hidden, inter, w2, sh2, b.row_route, weights, routes, b.row_capacity,
-                    b.mtiles, b.max_mtiles, b.counters, tiles, rows, b.y, s);
-  }
+  const int64_t rows13 = min64(tokens, tile_rows(rows, sh13));
+  const int64_t rows2 = min64(tokens, tile_rows(rows, sh2));
+  rc = rows <= kStreamRows
+           ? w4_gate_up_stream(src, hidden, inter, w13, sh13, b.mtiles, b.max_mtiles, b.counters,
+                               tiles, rows13, b.act, s)
+           : w4_gate_up_tc(src, hidden, inter, w13, sh13, b.row_capacity, b.mtiles, b.max_mtiles,
+                           b.counters, tiles, rows13, b.act, s);
+  if (rc) return rc;
+  rc = rows <= kStreamRows
+           ? w4_down_stream(b.act, hidden, inter, w2, sh2, b.row_route, weights, routes, b.mtiles,
+                            b.max_mtiles, b.counters, tiles, rows2, b.y, s)
+           : w4_down_tc(b.act, hidden, inter, w2, sh2, b.row_route, weights, routes,
+                        b.row_capacity, b.mtiles, b.max_mtiles, b.counters, tiles, rows2, b.y, s);
   if (rc) return rc;
   const int64_t threads = tokens * (hidden / 4);
   B200_LAUNCH_PDL(kPdlCombine, tokens <= 256 ? w4_combine_kernel<8> : w4_combine_kernel<4>,
