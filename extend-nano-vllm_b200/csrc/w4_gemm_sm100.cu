@@ -22,10 +22,13 @@
 // (groups of four, alternate column chunks).
 // Every wait is bounded; on expiry the CTA records a status bit and leaves.
 //
-// What bounds it: instruction issue.  A block of 128 x 128 weights against 128
-// rows takes 590 cycles of matrix instructions (74 each; 37 at 16 rows) but some
-// 540 issue slots of each scheduler for decoding (seven ALU instructions of two
-// cycles per eight codes) and promoting, which do not overlap without gaps.
+// What bounds it: at 128 rows the turns that matrix instructions, promoting and
+// decoding take.  A block of 128 x 128 weights takes 590 cycles of matrix
+// instructions (74 each; 37 at 16 rows) out of some 1050: TMEM holds two
+// accumulators beside the operand stages, and decoding (seven ALU instructions
+// of two cycles per eight codes) and promoting fill half of the issue slots.
+// Neither fewer reads of x (a pair of SMs: slower, its hand-overs cross the
+// pair) nor more decoding warps or fewer, larger promoting warps helped.
 // Measured (back to back): 32 rows x [75776, 4096] 52 us = 3.05 TB/s of weights,
 // 64 rows 58 us, 128 rows 83 us; 4096 rows x [4096, 4096] 132 us = 1.04 PFLOP/s
 // (cuBLAS bf16 burst 1.64); groups of 32 with zero points, 64 rows: 91 us.

@@ -15,10 +15,11 @@
 // read back by a third; that pays from more than 16 rows on, w4_gemm_sm100.cu:
 // 16 rows x [151552, 4096] take 97 us here and 107 there, 32 rows 220 and 107.)
 //
-// What bounds it: not the instruction count (a variant that multiplies 128 + q
-// and corrects by the sums of x, a fifth fewer, measured the same; one with
-// shifts on the multiply pipe was slower), but the copies in flight: some 100 KB
-// per SM at 4-5 us each under load.  A deeper ring takes the L1 from x.
+// What bounds it: the loads of x beside the stream.  Without them it reads 4.7
+// TB/s of weights (8 rows), without the products as well 6.1 with a ring of six.
+// Not the instruction count (a variant that multiplies 128 + q and corrects by
+// the sums of x, a fifth fewer, measured the same; one with shifts on the multiply
+// pipe was slower), nor the depth of the ring (kDepth below).
 // Measured (back to back, weights larger than L2): 1 row x [75776, 4096] 40.2 us
 // = 3.98 TB/s of weights, 8 rows x [151552, 4096] 84.7 us = 3.78 TB/s, 16 rows
 // 97.2 us = 3.29 TB/s; copy peak 6.5 TB/s.
