@@ -9,12 +9,12 @@ int w4_linear_stream(const void *x, int64_t m, int n, int k, const void *w, cons
                      void *out, cudaStream_t s);
 int w4_gate_up_stream(const RowSource &src, int hidden, int inter, const void *w13,
                       const w4::Shape &sh, const int32_t *mtiles, int64_t max_mtiles,
-                      const int32_t *counters, double tiles, int64_t rows, void *act,
+                      const int32_t *counters, double tiles, int cols, void *act,
                       cudaStream_t s);
 int w4_down_stream(const void *act, int hidden, int inter, const void *w2, const w4::Shape &sh,
                    const int32_t *row_route, const void *route_weights, int64_t num_routes,
                    const int32_t *mtiles, int64_t max_mtiles, const int32_t *counters,
-                   double tiles, int64_t rows, float *y, cudaStream_t s);
+                   double tiles, int cols, float *y, cudaStream_t s);
 int w4_route_gate_up(const void *x, int64_t tokens, int hidden, int inter, const int64_t *ids,
                      int top_k, int num_experts, const void *w13, const w4::Shape &sh, void *act,
                      cudaStream_t s);
@@ -35,9 +35,33 @@ int w4_down_tc(const void *act, int hidden, int inter, const void *w2, const w4:
 namespace {
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// Rows of x up to which the weights are streamed (w4_stream.cu); with more,
-// tcgen05 (w4_gemm_sm100.cu).  For experts: rows of a full tile to expect.
+// Rows of x up to which the weights of a dense product are streamed
+// (w4_stream.cuh); with more, tcgen05 (w4_gemm_sm100.cu).
 constexpr int64_t kStreamRows = 16;
+
+// The same for experts, from the rows that an expert has on average.  A streamed
+// expert is passed over once per eight rows (or sixteen, stream_cols), a tile of
+// tcgen05 costs the same for one row as for many.  Small experts with small groups
+// have the dearest passes.  Measured, the whole call in us, streamed against tcgen05:
+//   128 experts of 768 x 2048, top-8, 64 / 80 / 96 / 112 tokens (4 / 5 / 6 / 7 rows):
+//     g 128  115 142 154 175 against 176 154 161 164
+//     g 64   126 157 173 194 against 170 152 160 169
+//     g 32   149 186 208 231 against 181 167 175 186
+//   16 experts of 6400 x 4096, top-4, 24 tokens (6 rows): g 128, 64, 32
+//     213 242 299 against 327 332 358
+bool stream_experts(int64_t tokens, double mean, int inter, const w4::Shape &sh13,
+                    const w4::Shape &sh2) {
+  if (tokens <= kStreamRows) return true;
+  const bool large_groups = sh13.groups_per_block() == 1 && sh2.groups_per_block() == 1;
+  return mean <= (large_groups || inter >= 2048 ? 6.0 : 4.5);
+}
+
+// Rows that a pass over a streamed expert takes.  Measured with 8 and with 16: 64
+// tokens through 128 experts of 768 x 2048 (4 rows) 115 and 118 us, 16 tokens
+// through 16 of 6400 x 4096 (4 rows) 181 and 239, through 8 of 14336 x 4096, top-8
+// (16 rows) 349 and 264.
+int stream_cols(int64_t tokens, double mean) { return tokens <= 8 || mean <= 6.0 ? 8 : 16; }
+
 // Routes up to which the experts run route by route, without packing.
 constexpr int64_t kRouteRoutes = 16;
 // Routes up to which the gate/up product gathers its rows in its own loads
@@ -49,18 +73,14 @@ constexpr int64_t kGatherRoutes = 512;
 // that is too small costs passes over the weights, one that is too large costs
 // time only by the hand-over of each group's accumulators, so that large groups
 // want large tiles.  Measured with 128 experts, top-8, the whole call in us with
-// tiles of 16 (streaming) / 32 / 64 / 128 rows:
-//   g 128: 64 tokens 137 / 165 / 177 / 171, 96 164 / 162 / 168 / 160,
-//          256 336 / 207 / 197 / 175, 509 483 / 276 / 225 / 197
-//   g 64:  96 tokens 182 / 161 / 190 / 188, 192 314 / 196 / 199 / 196, 256 374 /
-//          214 / 217 / 203, 509 536 / 288 / 256 / 229
-//   g 32:  96 tokens 189 / 177 / 240 / 281, 384 499 / 282 / 307 / 331, 509 568 /
-//          323 / 317 / 346, 768 796 / 438 / 388 / 377
-// Eight columns (streaming) against sixteen: 64 tokens over 512 experts, top-10
-// (1.25 rows on average) 174 against 185, 64 over 128 149 against 137.
+// tiles of 32 / 64 / 128 rows:
+//   g 128: 64 tokens 165 / 177 / 171, 96 162 / 168 / 160, 256 207 / 197 / 175,
+//          509 276 / 225 / 197
+//   g 64:  96 tokens 161 / 190 / 188, 192 196 / 199 / 196, 256 214 / 217 / 203,
+//          509 288 / 256 / 229
+//   g 32:  96 tokens 177 / 240 / 281, 384 282 / 307 / 331, 509 323 / 317 / 346,
+//          768 438 / 388 / 377
 int64_t tile_rows(int64_t rows, const w4::Shape &sh) {
-  if (rows <= 10) return 8;
-  if (rows <= kStreamRows) return kStreamRows;
   switch (sh.groups_per_block()) {
     case 1: return 128;
     case 2: return rows <= 26 ? 32 : 128;
@@ -372,19 +392,19 @@ int b200moe_w4_experts(const void *x, int64_t tokens, int hidden, int inter,
   const double mean = static_cast<double>(routes) / num_experts;
   const double tiles = num_experts * (1.0 - exp(-mean)) + static_cast<double>(routes) / 128;
   const int64_t rows = min64(tokens, static_cast<int64_t>(1.5 * mean + 8.0));
-  const int64_t rows13 = min64(tokens, tile_rows(rows, sh13));
-  const int64_t rows2 = min64(tokens, tile_rows(rows, sh2));
-  rc = rows <= kStreamRows
-           ? w4_gate_up_stream(src, hidden, inter, w13, sh13, b.mtiles, b.max_mtiles, b.counters,
-                               tiles, rows13, b.act, s)
-           : w4_gate_up_tc(src, hidden, inter, w13, sh13, b.row_capacity, b.mtiles, b.max_mtiles,
-                           b.counters, tiles, rows13, b.act, s);
+  const bool stream_w = stream_experts(tokens, mean, inter, sh13, sh2);
+  const int cols = stream_cols(tokens, mean);
+  rc = stream_w ? w4_gate_up_stream(src, hidden, inter, w13, sh13, b.mtiles, b.max_mtiles,
+                                    b.counters, tiles, cols, b.act, s)
+                : w4_gate_up_tc(src, hidden, inter, w13, sh13, b.row_capacity, b.mtiles,
+                                b.max_mtiles, b.counters, tiles,
+                                min64(tokens, tile_rows(rows, sh13)), b.act, s);
   if (rc) return rc;
-  rc = rows <= kStreamRows
-           ? w4_down_stream(b.act, hidden, inter, w2, sh2, b.row_route, weights, routes, b.mtiles,
-                            b.max_mtiles, b.counters, tiles, rows2, b.y, s)
-           : w4_down_tc(b.act, hidden, inter, w2, sh2, b.row_route, weights, routes,
-                        b.row_capacity, b.mtiles, b.max_mtiles, b.counters, tiles, rows2, b.y, s);
+  rc = stream_w ? w4_down_stream(b.act, hidden, inter, w2, sh2, b.row_route, weights, routes,
+                                b.mtiles, b.max_mtiles, b.counters, tiles, cols, b.y, s)
+               : w4_down_tc(b.act, hidden, inter, w2, sh2, b.row_route, weights, routes,
+                            b.row_capacity, b.mtiles, b.max_mtiles, b.counters, tiles,
+                            min64(tokens, tile_rows(rows, sh2)), b.y, s);
   if (rc) return rc;
   const int64_t threads = tokens * (hidden / 4);
   B200_LAUNCH_PDL(kPdlCombine, tokens <= 256 ? w4_combine_kernel<8> : w4_combine_kernel<4>,

@@ -5,8 +5,8 @@
 //   D_g[f, r] = sum_{k in group g} (q[f, k] - z[f, g]) * x[r, k]
 //   y[r, f]   = sum_g s[f, g] * D_g[f, r]
 //
-// Each warp streams its own weights (asynchronous copies into a ring of its own)
-// -> registers -> integers q - z (exact in bf16) -> warp matrix instructions
+// Each warp streams its own weights from memory into registers, one block ahead
+// of its products -> integers q - z (exact in bf16) -> warp matrix instructions
 // (m16n8k16: 16 weight rows, 8 rows of x), and adds a group's sum to fp32
 // registers times its scale.  No barrier and no second warp is on the way of a
 // weight, which is what a stream of 4-bit weights needs: at the copy rate an SM
@@ -15,14 +15,16 @@
 // read back by a third; that pays from more than 16 rows on, w4_gemm_sm100.cu:
 // 16 rows x [151552, 4096] take 97 us here and 107 there, 32 rows 220 and 107.)
 //
-// What bounds it: the loads of x beside the stream.  Without them it reads 4.7
-// TB/s of weights (8 rows), without the products as well 6.1 with a ring of six.
-// Not the instruction count (a variant that multiplies 128 + q and corrects by
-// the sums of x, a fifth fewer, measured the same; one with shifts on the multiply
-// pipe was slower), nor the depth of the ring (kDepth below).
-// Measured (back to back, weights larger than L2): 1 row x [75776, 4096] 40.2 us
-// = 3.98 TB/s of weights, 8 rows x [151552, 4096] 84.7 us = 3.78 TB/s, 16 rows
-// 97.2 us = 3.29 TB/s; copy peak 6.5 TB/s.
+// Measured (back to back, weights larger than L2): 1 row x [75776, 4096] 34.2 us
+// = 4.68 TB/s of weights, 8 rows x [151552, 4096] 68 us = 4.71 TB/s, 16 rows 97 us
+// = 3.31 TB/s; 8 rows x [75776, 4096] with groups of 32 and zero points 50.6 us =
+// 3.64 TB/s; copy peak 6.5 TB/s.  What bounds it: L1, 80 % busy with the lines of
+// x beside those of the codes (8 rows, one scale per block; the schedulers issue in
+// 59 % of cycles, 297 instructions per 32 x 128 weights).
+// A ring of asynchronous copies in shared memory per warp, four deep, in place
+// of the registers took 42, 84 and 104 us for the first three: it fetches as far
+// ahead as one likes, but every weight crosses shared memory once more and the
+// ring takes L1 from x.
 //
 // A warp owns 32 weight rows (a quarter of a tile): two 16-row operands, which
 // in gate_up order are the gate and the up rows of the same 16 features, so the
@@ -100,82 +102,59 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Blocks on their way: each warp has a ring of its own in shared memory, filled
-// by bulk copies (one per block and warp), so that six kilobytes per warp are
-// in flight however few registers are left.  Measured at 8 rows x [151552,
-// 4096]: depth 4 with two thread blocks per SM 86 us, depth 6 95, three or four
-// thread blocks (whose rings leave less of the L1 to x) 94-108.
-constexpr int kDepth = 4;
-
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes,
-                                          uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-          dst),
-      "l"(src), "r"(bytes), "r"(bar)
-      : "memory");
-}
-
-// Waits for a copy: bounded, and without a timer on the way of a satisfied wait.
-__device__ __forceinline__ bool wait_copy(uint32_t bar, uint32_t parity) {
-  if (__builtin_expect(mbar_try_wait(bar, parity), 1)) return true;
-  int64_t start = 0;
-  for (uint32_t tries = 1;; ++tries) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((tries & 1023u) == 0) {
-      const int64_t now = clock64();
-      if (start == 0) {
-        start = now;
-      } else if (now - start > 4000000000ll) {
-        atomicOr(&g_status, kStatusTimeout);
-        return false;
-      }
-    }
-  }
-}
-
 // One block's share of a lane: 16 bytes of rows g, g + 8, ... (two per operand
 // of 16 rows), and those rows' scales and zero points.
 template <int GPB, bool ZEROS>
 struct Block {
   uint4 codes[4];
-  uint2 scale[GPB];    // four of 16 bits
-  uint32_t zero[GPB];  // four of 8 bits
+  // Of every group; of four groups that of lane t alone (the neighbours have the
+  // others: fewer loads and registers, 8 rows x [75776, 4096] with groups of 32
+  // and zero points 49.6 us against 54.0; of two groups shuffles cost more, the
+  // experts of 16 tokens over 512 76 us against 70).
+  static constexpr int kHeld = GPB < 4 ? GPB : 1;
+  uint2 scale[kHeld];    // four of 16 bits: rows g, g + 8, g + 16, g + 24
+  uint32_t zero[kHeld];  // four of 8 bits
 
-  __device__ __forceinline__ void read(uint32_t stage, int lane) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(codes[i].x), "=r"(codes[i].y), "=r"(codes[i].z), "=r"(codes[i].w)
-                   : "r"(stage + (lane & 3) * 512 + (lane >> 2) * 16 + i * 128));
+  // q: the quarter's block.
+  __device__ __forceinline__ void load(const uint8_t *q, int lane) {
     const int g = lane >> 2;
 #pragma unroll
-    for (int j = 0; j < GPB; ++j)
-      asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
-                   : "=r"(scale[j].x), "=r"(scale[j].y)
-                   : "r"(stage + w4::kCodeBytes + j * 64 + g * 8));
-    if (ZEROS) {
+    for (int i = 0; i < 4; ++i) codes[i] = load_codes(q + (lane & 3) * 512 + g * 16 + i * 128);
+    q += w4::kCodeBytes;
 #pragma unroll
-      for (int j = 0; j < GPB; ++j)
-        asm volatile("ld.shared.u32 %0, [%1];"
-                     : "=r"(zero[j])
-                     : "r"(stage + w4::kCodeBytes + GPB * 64 + j * 32 + g * 4));
+    for (int h = 0; h < kHeld; ++h) {
+      const int j = kHeld == GPB ? h : lane & 3;
+      asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];"
+                   : "=r"(scale[h].x), "=r"(scale[h].y)
+                   : "l"(q + j * 64 + g * 8));
+      if (ZEROS)
+        asm volatile("ld.global.nc.u32 %0, [%1];"
+                     : "=r"(zero[h])
+                     : "l"(q + GPB * 64 + j * 32 + g * 4));
     }
   }
-  // Scales of rows g, g + 8, g + 16, g + 24.
+  static __device__ __forceinline__ uint32_t from_lane(uint32_t v, int j) {
+    return kHeld == GPB ? v : __shfl_sync(0xffffffffu, v, j, 4);
+  }
+  // Group j's scales of rows g, g + 8, g + 16, g + 24.
   __device__ __forceinline__ void scales(int j, bool half_scale, float (&s)[4]) const {
+    const int h = kHeld == GPB ? j : 0;
+    const uint32_t x = from_lane(scale[h].x, j), y = from_lane(scale[h].y, j);
     if (__builtin_expect(half_scale, 0)) {
-      const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&scale[j].x));
-      const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&scale[j].y));
+      const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&x));
+      const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&y));
       s[0] = a.x, s[1] = a.y, s[2] = b.x, s[3] = b.y;
     } else {
-      s[0] = __uint_as_float(scale[j].x << 16), s[1] = __uint_as_float(scale[j].x & 0xffff0000u);
-      s[2] = __uint_as_float(scale[j].y << 16), s[3] = __uint_as_float(scale[j].y & 0xffff0000u);
+      s[0] = __uint_as_float(x << 16), s[1] = __uint_as_float(x & 0xffff0000u);
+      s[2] = __uint_as_float(y << 16), s[3] = __uint_as_float(y & 0xffff0000u);
     }
   }
-  // Of row g + 8 i: the bytes z and 0x43 twice, 128 + z in both halves.
-  __device__ __forceinline__ uint32_t zpair(int j, int i) const {
-    return ZEROS ? __byte_perm(zero[j], 0x43434343u, 0x4040 | (i << 8) | i) : 0x43084308u;
+  // Per row g + 8 i: the bytes z and 0x43 twice, 128 + z in both halves.
+  __device__ __forceinline__ void zpairs(int j, uint32_t (&z)[4]) const {
+    const uint32_t v = ZEROS ? from_lane(zero[kHeld == GPB ? j : 0], j) : 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      z[i] = ZEROS ? __byte_perm(v, 0x43434343u, 0x4040 | (i << 8) | i) : 0x43084308u;
   }
 };
 
@@ -190,62 +169,95 @@ __device__ __forceinline__ uint4 load_row(const __nv_bfloat16 *p) {
   return v;
 }
 
-// This lane's k of one block of its rows of x.  xp[n]: its eight k of chunk 0
-// of row 8 n + g (of some other row where there are fewer; its sums are not
-// stored).
+// This lane's chunks of one block of its rows of x.  xp[n]: its eight k of chunk
+// 0 of row 8 n + g (of some other row where there are fewer; its sums are not
+// stored).  One column tile has the registers for all four chunks at once, two
+// column tiles for two: 16 rows x [151552, 4096] 92.6 us, with four 96.6, one 157.
 template <int NB>
-__device__ __forceinline__ void read_rows(uint4 (&xv)[4][NB], const __nv_bfloat16 *const (&xp)[NB],
-                                          int k0, int k) {
-  if (__builtin_expect(k0 + w4::kBlockK <= k, 1)) {
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-      for (int n = 0; n < NB; ++n) xv[c][n] = load_row(xp[n] + k0 + 32 * c);
-  } else {
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-      for (int n = 0; n < NB; ++n)
-        xv[c][n] = k0 + 32 * c < k ? load_row(xp[n] + k0 + 32 * c) : make_uint4(0, 0, 0, 0);
-  }
-}
+struct Rows {
+  static constexpr int kAhead = NB == 1 ? 4 : 2;
+  uint4 v[4][NB];
 
-// Adds one block to tot[operand][column tile][4].
+  __device__ __forceinline__ void read(int c, const __nv_bfloat16 *const (&xp)[NB], int k0, int k) {
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+      v[c][n] = k0 + 32 * c < k ? load_row(xp[n] + k0 + 32 * c) : make_uint4(0, 0, 0, 0);
+  }
+};
+
+// Adds one block to tot[operand][column tile][4].  x: its first chunks are read.
 template <int GPB, int NB, bool ZEROS>
-__device__ __forceinline__ void add_block(const Block<GPB, ZEROS> &b, bool half_scale,
-                                          const uint4 (&xv)[4][NB], float (&tot)[2][NB][4]) {
+__device__ __forceinline__ void add_block(const Block<GPB, ZEROS> &b, bool half_scale, Rows<NB> &x,
+                                          const __nv_bfloat16 *const (&xp)[NB], int k0, int k,
+                                          float (&tot)[2][NB][4]) {
   constexpr int CPG = 4 / GPB;  // chunks per group
 #pragma unroll
   for (int j = 0; j < GPB; ++j) {
-    float s[4];
-    b.scales(j, half_scale, s);
+    float acc[2][NB][4];
+    uint32_t z[4];
+    b.zpairs(j, z);
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      float acc[NB][4];
-      const uint32_t z0 = b.zpair(j, 2 * m), z1 = b.zpair(j, 2 * m + 1);
+    for (int cc = 0; cc < CPG; ++cc) {
+      const int c = j * CPG + cc;
+      if (c > 0 && c + x.kAhead - 1 < 4) x.read(c + x.kAhead - 1, xp, k0, k);
 #pragma unroll
-      for (int cc = 0; cc < CPG; ++cc) {
-        const int c = j * CPG + cc;
+      for (int m = 0; m < 2; ++m) {
         uint32_t lo[4], hi[4];
-        w4::decode8(word(b.codes[2 * m], c), z0, lo);
-        w4::decode8(word(b.codes[2 * m + 1], c), z1, hi);
+        w4::decode8(word(b.codes[2 * m], c), z[2 * m], lo);
+        w4::decode8(word(b.codes[2 * m + 1], c), z[2 * m + 1], hi);
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
           if (cc == 0)
-            mma_first(acc[n], lo[0], hi[0], lo[1], hi[1], xv[c][n].x, xv[c][n].y);
+            mma_first(acc[m][n], lo[0], hi[0], lo[1], hi[1], x.v[c][n].x, x.v[c][n].y);
           else
-            mma(acc[n], lo[0], hi[0], lo[1], hi[1], xv[c][n].x, xv[c][n].y);
-          mma(acc[n], lo[2], hi[2], lo[3], hi[3], xv[c][n].z, xv[c][n].w);
+            mma(acc[m][n], lo[0], hi[0], lo[1], hi[1], x.v[c][n].x, x.v[c][n].y);
+          mma(acc[m][n], lo[2], hi[2], lo[3], hi[3], x.v[c][n].z, x.v[c][n].w);
         }
       }
+    }
+    float s[4];
+    b.scales(j, half_scale, s);
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
-        tot[m][n][0] = fmaf(s[2 * m], acc[n][0], tot[m][n][0]);
-        tot[m][n][1] = fmaf(s[2 * m], acc[n][1], tot[m][n][1]);
-        tot[m][n][2] = fmaf(s[2 * m + 1], acc[n][2], tot[m][n][2]);
-        tot[m][n][3] = fmaf(s[2 * m + 1], acc[n][3], tot[m][n][3]);
+        tot[m][n][0] = fmaf(s[2 * m], acc[m][n][0], tot[m][n][0]);
+        tot[m][n][1] = fmaf(s[2 * m], acc[m][n][1], tot[m][n][1]);
+        tot[m][n][2] = fmaf(s[2 * m + 1], acc[m][n][2], tot[m][n][2]);
+        tot[m][n][3] = fmaf(s[2 * m + 1], acc[m][n][3], tot[m][n][3]);
       }
-    }
+  }
+}
+
+// Adds an item's share of a warp, the blocks part, part + wk, ... of the quarter
+// at w.  The block after the one at work is on its way meanwhile; the first is
+// asked for before the wait for x.  (Asking for the next item's first block too
+// costs more in the loop than it gains: 8 rows 78 us against 68, 64 tokens
+// through 128 experts 126 against 118.)
+template <int GPB, int NB, bool ZEROS>
+__device__ __forceinline__ void add_item(const Args &a, const uint8_t *w, int part,
+                                         const __nv_bfloat16 *const (&xp)[NB], int lane,
+                                         bool wait_x, float (&tot)[2][NB][4]) {
+  const bool half_scale = a.sh.half_scale != 0;
+  const int wk = a.wk;
+  constexpr int kBlock = 4 * (w4::kCodeBytes + GPB * (ZEROS ? 96 : 64));
+  w += static_cast<int64_t>(part) * kBlock;
+  const int64_t hop = static_cast<int64_t>(wk) * kBlock;
+  Block<GPB, ZEROS> even, odd;
+  even.load(w, lane);
+  if (wait_x) pdl_wait();
+  auto step = [&](int kb, const Block<GPB, ZEROS> &now, Block<GPB, ZEROS> &next) {
+    Rows<NB> x;
+#pragma unroll
+    for (int c = 0; c < x.kAhead; ++c) x.read(c, xp, kb * w4::kBlockK, a.k);
+    w += hop;
+    if (kb + wk < a.num_kb) next.load(w, lane);
+    add_block<GPB, NB, ZEROS>(now, half_scale, x, xp, kb * w4::kBlockK, a.k, tot);
+  };
+#pragma unroll 1
+  for (int kb = part; kb < a.num_kb; kb += 2 * wk) {
+    step(kb, even, odd);
+    if (kb + wk < a.num_kb) step(kb + wk, odd, even);
   }
 }
 
@@ -323,10 +335,7 @@ __device__ __forceinline__ void store(const Args &a, const Item &it, int r0, int
 template <int GPB, int KIND, int NB, bool ZEROS>
 __global__ void __launch_bounds__(32 * kWarps, 2) w4_stream_kernel(
     const __grid_constant__ Args a) {
-  extern __shared__ __align__(16) uint8_t ring_smem[];  // [kWarps][kDepth] quarter blocks
   __shared__ float red[kWarps][2 * NB * 4][32];
-  constexpr int kStage = w4::kCodeBytes + GPB * (ZEROS ? 96 : 64);
-  __shared__ uint64_t bars[kWarps][kDepth];
   // Route by route, the next kernel reads the routes before it waits for this
   // one, so it may start only when they are there.
   const bool by_route = KIND == kGateUp && a.ids != nullptr;
@@ -337,14 +346,6 @@ __global__ void __launch_bounds__(32 * kWarps, 2) w4_stream_kernel(
   const int wk = a.wk;
   const int wr = kWarps / wk;  // items of a thread block at a time
   const int part = warp / wr;
-  const bool half_scale = a.sh.half_scale != 0;
-  const uint32_t ring = smem_u32(ring_smem) + warp * (kDepth * kStage);
-  const uint32_t full = smem_u32(bars[warp]);
-  if (lane == 0) {
-    for (int i = 0; i < kDepth; ++i) mbar_init(full + 8 * i, 1);
-    fence_mbar_init();
-  }
-  __syncwarp();
   if (KIND != kLinear) pdl_wait();
   if (by_route) pdl_trigger();
   const int mt = KIND == kLinear ? 1
@@ -355,36 +356,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) w4_stream_kernel(
   const int stride = gridDim.x * wr;
   const int begin = blockIdx.x * wr + warp % wr;
 
-  // Where the copies are: they run kDepth - 1 blocks ahead of the products,
-  // into the next items too.
-  const uint8_t *src = nullptr, *src_next = nullptr;
-  int src_item = begin, src_kb = a.num_kb, src_left = 0, src_stage = 0;
-  auto copy_next = [&]() {
-    if (__builtin_expect(src_kb >= a.num_kb, 0)) {  // the next pass over the item, or the next item
-      while (src_left == 0 && src_item < items) {
-        const Item n = item_of<KIND>(a, src_item);
-        src_item += stride;
-        src = n.w + static_cast<int64_t>(part) * (4 * kStage);
-        src_left = (n.rows + 8 * NB - 1) / (8 * NB);
-      }
-      if (src_left == 0) return;
-      --src_left;
-      src_kb = part;
-      src_next = src;
-    }
-    if (lane == 0) {
-      mbar_arrive_expect_tx(full + 8 * src_stage, kStage);
-      bulk_load(ring + src_stage * kStage, src_next, kStage, full + 8 * src_stage);
-    }
-    src_next += static_cast<int64_t>(wk) * (4 * kStage);
-    src_kb += wk;
-    src_stage = (src_stage + 1) % kDepth;
-  };
-#pragma unroll 1
-  for (int i = 0; i < kDepth - 1; ++i) copy_next();
-  if (KIND == kLinear) pdl_wait();  // codes are constant, x is not
-  int stage = 0;
-  uint32_t phase = 0;
+  bool wait_x = KIND == kLinear;  // codes are constant, x is not
 
   // All warps of a block take the same number of turns (they meet when k is
   // shared); a turn past the end does nothing.
@@ -413,30 +385,8 @@ __global__ void __launch_bounds__(32 * kWarps, 2) w4_stream_kernel(
                                                   a.top_k, a.num_routes, a.x_rows);
           xp[n] = static_cast<const __nv_bfloat16 *>(a.x) + row * a.k + 8 * t;
         }
-        // The rows of x come from L1 or L2 and are asked for one block ahead;
-        // with two column tiles there is no room for that.
-        uint4 xv[NB == 1 ? 2 : 1][4][NB];
-        if (NB == 1) read_rows(xv[0], xp, part * w4::kBlockK, a.k);
-        auto step = [&](int kb, uint4 (&now)[4][NB], uint4 (&next)[4][NB]) {
-          const bool arrived = wait_copy(full + 8 * stage, phase);
-          Block<GPB, ZEROS> b;
-          b.read(ring + stage * kStage, lane);
-          __syncwarp();  // every lane is done with the stage before, which is filled next
-          copy_next();
-          if (NB == 1) {
-            if (kb + wk < a.num_kb) read_rows(next, xp, (kb + wk) * w4::kBlockK, a.k);
-          } else {
-            read_rows(now, xp, kb * w4::kBlockK, a.k);
-          }
-          stage = (stage + 1) % kDepth;
-          phase ^= stage == 0 ? 1u : 0u;
-          if (arrived) add_block<GPB, NB, ZEROS>(b, half_scale, now, tot);
-        };
-#pragma unroll 1
-        for (int kb = part; kb < a.num_kb; kb += 2 * wk) {
-          step(kb, xv[0], xv[NB == 1 ? 1 : 0]);
-          if (kb + wk < a.num_kb) step(kb + wk, xv[NB == 1 ? 1 : 0], xv[0]);
-        }
+        add_item<GPB, NB, ZEROS>(a, it.w, part, xp, lane, wait_x, tot);
+        wait_x = false;
       }
       if (wk == 1) {
         if (rows > 0) {
@@ -475,16 +425,8 @@ __global__ void __launch_bounds__(32 * kWarps, 2) w4_stream_kernel(
 
 template <int GPB, int KIND, int NB, bool ZEROS>
 int launch(const Args &a, int64_t blocks, cudaStream_t s) {
-  constexpr int smem = kWarps * kDepth * (w4::kCodeBytes + GPB * (ZEROS ? 96 : 64));
-  static bool done[64] = {false};
-  const int dev = current_device();
-  if (!(dev >= 0 && dev < 64 && done[dev])) {
-    B200_CUDA(cudaFuncSetAttribute(w4_stream_kernel<GPB, KIND, NB, ZEROS>,
-                                   cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    if (dev >= 0 && dev < 64) done[dev] = true;
-  }
   B200_LAUNCH_PDL(kPdlStream, w4_stream_kernel<GPB, KIND, NB, ZEROS>, dim3(static_cast<unsigned>(blocks)),
-                  dim3(32 * kWarps), smem, s, a);
+                  dim3(32 * kWarps), 0, s, a);
   B200_LAUNCHED();
   return B200MOE_OK;
 }
@@ -502,9 +444,9 @@ int launch_tile(const Args &a, int64_t blocks, cudaStream_t s) {
 }
 
 // items: warp items (quarters of tiles) that the call is expected to work off;
-// most: an upper bound.  rows: of a row tile.
+// most: an upper bound.  cols: rows of x of a pass, 8 or 16.
 template <int KIND>
-int run(Args a, double items, int64_t most, int64_t rows, cudaStream_t s) {
+int run(Args a, double items, int64_t most, int cols, cudaStream_t s) {
   const int64_t slots = static_cast<int64_t>(sm_count()) * 2;  // resident blocks
   // Warps per item: as many as the machine has room for while there are few
   // items; else shared by two where a warp keeps at least eight blocks, so that
@@ -530,7 +472,7 @@ int run(Args a, double items, int64_t most, int64_t rows, cudaStream_t s) {
   int64_t blocks = (most + wr - 1) / wr;
   if (blocks > slots) blocks = slots;
   if (blocks < 1) blocks = 1;
-  return rows <= 8 ? launch_tile<KIND, 1>(a, blocks, s) : launch_tile<KIND, 2>(a, blocks, s);
+  return cols <= 8 ? launch_tile<KIND, 1>(a, blocks, s) : launch_tile<KIND, 2>(a, blocks, s);
 }
 
 }  // namespace w4s

@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(32 * kWarps) w4_down_slots_kernel(
 int w4_down_stream(const void *act, int hidden, int inter, const void *w2, const w4::Shape &sh,
                    const int32_t *row_route, const void *route_weights, int64_t num_routes,
                    const int32_t *mtiles, int64_t max_mtiles, const int32_t *counters,
-                   double tiles, int64_t rows, float *y, cudaStream_t s) {
+                   double tiles, int cols, float *y, cudaStream_t s) {
   using namespace w4s;
   Args a = {};
   a.w = static_cast<const uint8_t *>(w2);
@@ -124,7 +124,7 @@ int w4_down_stream(const void *act, int hidden, int inter, const void *w2, const
   a.route_w = static_cast<const __nv_bfloat16 *>(route_weights);
   a.num_routes = num_routes;
   a.out = y;
-  return run<kDown>(a, 4.0 * tiles * a.n_blocks, 4 * max_mtiles * a.n_blocks, rows, s);
+  return run<kDown>(a, 4.0 * tiles * a.n_blocks, 4 * max_mtiles * a.n_blocks, cols, s);
 }
 
 // Few routes: down projection of act [tokens * top_k, inter] and the sum over a

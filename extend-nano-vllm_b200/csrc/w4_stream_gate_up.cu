@@ -5,7 +5,7 @@ namespace b200moe {
 
 int w4_gate_up_stream(const RowSource &src, int hidden, int inter, const void *w13,
                       const w4::Shape &sh, const int32_t *mtiles, int64_t max_mtiles,
-                      const int32_t *counters, double tiles, int64_t rows, void *act,
+                      const int32_t *counters, double tiles, int cols, void *act,
                       cudaStream_t s) {
   using namespace w4s;
   Args a = {};
@@ -25,7 +25,7 @@ int w4_gate_up_stream(const RowSource &src, int hidden, int inter, const void *w
   a.num_routes = src.num_routes;
   a.top_k = src.top_k;
   a.out = act;
-  return run<kGateUp>(a, 4.0 * tiles * a.n_blocks, 4 * max_mtiles * a.n_blocks, rows, s);
+  return run<kGateUp>(a, 4.0 * tiles * a.n_blocks, 4 * max_mtiles * a.n_blocks, cols, s);
 }
 
 // Route by route, without packing: act[r] for route r = (t, s), expert ids[r].
@@ -49,7 +49,7 @@ int w4_route_gate_up(const void *x, int64_t tokens, int hidden, int inter, const
   a.num_experts = num_experts;
   a.out = act;
   const int64_t items = 4 * a.num_routes * a.n_blocks;
-  return run<kGateUp>(a, static_cast<double>(items), items, 1, s);
+  return run<kGateUp>(a, static_cast<double>(items), items, 8, s);
 }
 
 }  // namespace b200moe

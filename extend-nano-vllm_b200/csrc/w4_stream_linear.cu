@@ -17,7 +17,7 @@ int w4_linear_stream(const void *x, int64_t m, int n, int k, const void *w, cons
   a.x = x;
   a.x_rows = m;
   a.out = out;
-  return run<kLinear>(a, 4.0 * a.n_blocks, 4ll * a.n_blocks, m, s);
+  return run<kLinear>(a, 4.0 * a.n_blocks, 4ll * a.n_blocks, m <= 8 ? 8 : 16, s);
 }
 
 }  // namespace b200moe

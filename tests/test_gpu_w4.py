@@ -195,6 +195,24 @@ def test_experts_prefill(hidden, inter, experts, top_k, tokens, group, zeros):
     check_experts(activations((tokens, hidden), 1), ids, weights, parts13, parts2)
 
 
+@pytest.mark.parametrize("group,zeros", [(128, False), (64, True), (32, True)])
+@pytest.mark.parametrize("hidden,inter,experts,top_k,tokens", [
+    (640, 256, 4, 4, 9), (384, 1280, 3, 2, 16),       # few experts, passes of 16 rows
+    (384, 256, 32, 4, 40), (384, 256, 32, 4, 48),     # five and six rows on average
+    (256, 2304, 16, 4, 24), (256, 384, 64, 2, 130)])  # long rows; four rows on average
+def test_experts_of_few_rows(hidden, inter, experts, top_k, tokens, group, zeros):
+    parts13 = weight((experts, 2 * inter, hidden), group, zeros, seed=hidden)
+    parts2 = weight((experts, hidden, inter), group, not zeros, seed=inter)
+    packed = ops.pack_w4(*parts13, layout="gate_up"), ops.pack_w4(*parts2)
+    ids, weights = routed(tokens, experts, top_k, tokens)
+    x = activations((tokens, hidden), 1)
+    check_experts(x, ids, weights, parts13, parts2, packed)
+    ids[:, 0], ids[:, 1] = 1, 2  # two experts with every token: passes over them
+    for s in range(2, top_k):
+        ids[:, s] = experts
+    check_experts(x, ids, weights, parts13, parts2, packed)
+
+
 @pytest.mark.parametrize("tokens", [2, 90])
 def test_experts_dropped_routes_and_one_full_expert(tokens):
     hidden, inter, experts, top_k = 128, 128, 8, 2
