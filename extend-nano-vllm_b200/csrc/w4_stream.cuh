@@ -450,11 +450,12 @@ int run(Args a, double items, int64_t most, int cols, cudaStream_t s) {
   const int64_t slots = static_cast<int64_t>(sm_count()) * 2;  // resident blocks
   // Warps per item: as many as the machine has room for while there are few
   // items; else shared by two where a warp keeps at least eight blocks, so that
-  // the warps of a block read one tile and the same rows of x.  Measured: 64
-  // tokens through 128 experts, gate/up (16 blocks of k) 148 / 137 / 137 / 149 us
-  // of the call with 1 / 2 / 4 / 8 warps, down (6 blocks) 148 / 152 / 160 with
-  // 1 / 2 / 4.  The cost is rounds of items, each as long as its blocks and some
-  // to begin and end.
+  // the warps of a block read one tile and the same rows of x.  Measured, us of the
+  // call with 1 / 2 / 4 / 8 warps: 64 tokens through 128 experts, gate/up (16 blocks
+  // of k) 123 / 115 / 113 / 120, down (6 blocks) 115 / 118 / 131; down of 16 tokens
+  // through 16 experts (50 blocks) 191 / 180 / 180 / 179; two rows x [8192, 4096]
+  // 21 / 12 / 9.2 / 5.9, x [37888, 4096] 24.0 / 17.8 / 19.0 / 20.7.  The cost is
+  // rounds of items, each as long as its blocks and some to begin and end.
   double best = 1e30;
   a.wk = 1;
   for (int wk = 1; wk <= kWarps && wk <= a.num_kb; wk *= 2) {
