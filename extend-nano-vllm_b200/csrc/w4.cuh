@@ -7,9 +7,11 @@
 // A matrix [rows, k] is laid out once as tiles of 128 rows; a tile is a run of
 // blocks of 128 k, a block four quarters of 32 rows, and a quarter one
 // contiguous piece of memory (what one copy brings):
-//   codes  4 units x 32 rows x 16 bytes: word c of unit u holds the eight k
-//          32 c + 8 u .. + 7 of a row.  A thread that owns a row reads four
-//          units; in a warp matrix instruction lane t of a row reads unit t;
+//   codes  32 rows x 4 units x 16 bytes: word c of unit u holds the eight k
+//          32 c + 8 u .. + 7 of a row.  In a warp matrix instruction lane t of a
+//          row reads unit t, so that eight lanes read one line; a thread that
+//          owns a row reads its four units in turn, and their exchange within the
+//          row (code_place) spreads eight such threads over all banks;
 //   scales [128 / g][32] of 16 bits (bf16 or fp16), row r at place
 //          4 (r % 8) + r / 8 (scale_place): the four rows r, r + 8, r + 16,
 //          r + 24 that one lane needs are neighbours;
@@ -53,6 +55,11 @@ inline Shape shape_of(int group, int flags) {
 }
 inline bool group_ok(int group) { return group == 32 || group == 64 || group == 128; }
 __host__ __device__ inline int64_t blocks_of(int64_t k) { return (k + kBlockK - 1) / kBlockK; }
+
+// Place of unit u of a quarter's row among its codes, in bytes.
+__host__ __device__ __forceinline__ int code_place(int row, int u) {
+  return row * 64 + ((u ^ ((row >> 1) & 3)) << 4);
+}
 
 // Place of a quarter's row among its scales.
 __host__ __device__ __forceinline__ int scale_place(int row) {

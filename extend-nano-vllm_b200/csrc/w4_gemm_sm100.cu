@@ -485,7 +485,7 @@ __device__ __forceinline__ void decode(const Args &args, const Ctx &c, int grp, 
           asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                        : "=r"(code[4 * i]), "=r"(code[4 * i + 1]), "=r"(code[4 * i + 2]),
                          "=r"(code[4 * i + 3])
-                       : "r"(st + i * 512 + lane * 16));
+                       : "r"(st + w4::code_place(lane, i)));
         uint32_t zp[GPB];
 #pragma unroll
         for (int g = 0; g < GPB; ++g) {

@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(w4::kTileRows) w4_pack_kernel(
   }
 #pragma unroll
   for (int u = 0; u < 4; ++u)
-    *reinterpret_cast<uint4 *>(quarter + u * 512 + (row & 31) * 16) =
+    *reinterpret_cast<uint4 *>(quarter + w4::code_place(row & 31, u)) =
         make_uint4(word[u][0], word[u][1], word[u][2], word[u][3]);
   for (int g = 0; g < sh.groups_per_block(); ++g) {
     const int64_t gi = kb * sh.groups_per_block() + g;

@@ -119,7 +119,7 @@ struct Block {
   __device__ __forceinline__ void load(const uint8_t *q, int lane) {
     const int g = lane >> 2;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) codes[i] = load_codes(q + (lane & 3) * 512 + g * 16 + i * 128);
+    for (int i = 0; i < 4; ++i) codes[i] = load_codes(q + w4::code_place(g, lane & 3) + i * 512);
     q += w4::kCodeBytes;
 #pragma unroll
     for (int h = 0; h < kHeld; ++h) {

@@ -41,9 +41,9 @@ __global__ void __launch_bounds__(32 * kWarps) w4_down_slots_kernel(
         for (int b = 0; b < BATCH; ++b)
           if (kb0 + b < num_kb) {
             const uint8_t *block = w + static_cast<int64_t>(kb0 + b) * bytes;
-            const uint8_t *c = block + t * 512 + (op * 16 + g) * 16;
+            const uint8_t *c = block + w4::code_place(op * 16 + g, t);
             codes[b][0] = load_codes(c);
-            codes[b][1] = load_codes(c + 128);
+            codes[b][1] = load_codes(c + 512);
             const uint8_t *sc = block + w4::kCodeBytes + (4 * g + 2 * op) * 2;
 #pragma unroll
             for (int j = 0; j < GPB; ++j) {
