@@ -44,11 +44,11 @@ constexpr int64_t kStreamRows = 16;
 // tcgen05 costs the same for one row as for many.  Small experts with small groups
 // have the dearest passes.  Measured, the whole call in us, streamed against tcgen05:
 //   128 experts of 768 x 2048, top-8, 64 / 80 / 96 / 112 tokens (4 / 5 / 6 / 7 rows):
-//     g 128  115 142 154 175 against 176 154 161 164
-//     g 64   126 157 173 194 against 170 152 160 169
-//     g 32   149 186 208 231 against 181 167 175 186
+//     g 128  110 142 154 175 against 176 154 161 164
+//     g 64   121 157 173 194 against 170 152 160 169
+//     g 32   144 186 208 231 against 181 167 175 186
 //   16 experts of 6400 x 4096, top-4, 24 tokens (6 rows): g 128, 64, 32
-//     213 242 299 against 327 332 358
+//     202 232 287 against 327 332 358
 bool stream_experts(int64_t tokens, double mean, int inter, const w4::Shape &sh13,
                     const w4::Shape &sh2) {
   if (tokens <= kStreamRows) return true;

@@ -13,14 +13,16 @@
 // has 11 cycles for 512 codes, and decoding them takes 7 of each scheduler's.
 // (tcgen05 wants the operand decoded by one warp, waited for by another and
 // read back by a third; that pays from more than 16 rows on, w4_gemm_sm100.cu:
-// 16 rows x [151552, 4096] take 97 us here and 107 there, 32 rows 220 and 107.)
+// 16 rows x [151552, 4096] take 92 us here and 107 there, 32 rows 220 and 107.)
 //
-// Measured (back to back, weights larger than L2): 1 row x [75776, 4096] 34.2 us
-// = 4.68 TB/s of weights, 8 rows x [151552, 4096] 68 us = 4.71 TB/s, 16 rows 97 us
-// = 3.31 TB/s; 8 rows x [75776, 4096] with groups of 32 and zero points 50.6 us =
-// 3.64 TB/s; copy peak 6.5 TB/s.  What bounds it: L1, 80 % busy with the lines of
-// x beside those of the codes (8 rows, one scale per block; the schedulers issue in
-// 59 % of cycles, 297 instructions per 32 x 128 weights).
+// Measured (back to back, weights larger than L2): 1 row x [75776, 4096] 33.6 us
+// = 4.76 TB/s of weights, 8 rows x [151552, 4096] 65.7 us = 4.87 TB/s, 16 rows
+// 91.5 us = 3.50 TB/s; 8 rows x [75776, 4096] with groups of 32 and zero points
+// 48.4 us = 3.81 TB/s; copy peak 6.5 TB/s.  What bounds it: no one unit.  With 8
+// rows the schedulers issue in 59 % of cycles (297 instructions per 32 x 128
+// weights) and wait for loads and for the decoding's integer pipe in turn; 16 warps
+// with a block in flight each are what the registers hold.  A row's four units lie
+// side by side (w4.cuh): 512 bytes apart they took 34.2, 68, 97 and 50.6 us.
 // A ring of asynchronous copies in shared memory per warp, four deep, in place
 // of the registers took 42, 84 and 104 us for the first three: it fetches as far
 // ahead as one likes, but every weight crosses shared memory once more and the
