@@ -90,6 +90,7 @@ SIGNATURES: dict[str, tuple] = {
                                        ctypes.c_float, _P, _P, _P]),
     "b200moe_w4_bytes": (_L, [_L, _L, _L, _I, _I]),
     "b200moe_w4_pack": (_I, [_P, _P, _P, _L, _L, _L, _I, _I, _P, _P]),
+    "b200moe_w4_ring_stages": (_I, [_I, _I, _I, _I, _I, _P, _P]),
     "b200moe_w4_linear": (_I, [_P, _L, _I, _I, _P, _I, _I, _P, _P]),
     "b200moe_w4_experts_workspace": (_L, [_L, _I, _I, _I, _I]),
     "b200moe_w4_experts_launches": (_I, [_L, _I, _I]),
@@ -137,7 +138,7 @@ PACK_SINGLE_LAUNCH_ROUTES = 1024
 # kernel per projection, the tiny decode path two).
 CALL_COUNTS: dict[str, int] = {}
 LAUNCH_COUNTS: dict[str, int] = {}
-_NO_KERNEL = ("b200moe_device_status", "b200moe_ipc_handle", "b200moe_ipc_open",
+_NO_KERNEL = ("b200moe_device_status", "b200moe_w4_ring_stages", "b200moe_ipc_handle", "b200moe_ipc_open",
               "b200moe_ipc_close")
 
 

@@ -54,6 +54,15 @@ constexpr int MAX_WS = 16;
 constexpr int SMEM_LIMIT = 226 * 1024;
 constexpr int TAIL_BYTES = 1024;  // barriers
 
+// Operand stages; the down projection's largest tile leaves one to the staging
+// of its fp32 rows.
+constexpr int operand_stages_of(int kind, int nt) { return kind == kDown && nt == 128 ? 3 : 4; }
+
+// Whether the first CTA of a cluster has room for the others' sums of nt rows.
+constexpr bool split_ok(int split, int nt) {
+  return split >= 1 && split <= 8 && (split & (split - 1)) == 0 && (split - 1) * nt <= 112;
+}
+
 // NT: rows of x per tile (the N side); GPB: groups per block of 128 k.
 template <int NT, int GPB, int KIND>
 struct Cfg {
@@ -66,9 +75,7 @@ struct Cfg {
   static constexpr int U = GPB < 128 / NT ? GPB : 128 / NT;
   static constexpr int UPB = GPB / U;                               // units per block
   static constexpr int ND = 256 / (U * NT) < 4 ? 256 / (U * NT) : 4;  // units in TMEM
-  // Operand stages; the down projection's largest tile leaves one to the
-  // staging of its fp32 rows.
-  static constexpr int BS = KIND == kDown && NT == 128 ? 3 : 4;
+  static constexpr int BS = operand_stages_of(KIND, NT);
   static constexpr bool LOCKSTEP = UPB == 1 && ND == BS;  // the two rings are one
   static constexpr int B_BYTES = NT * 256;                // 128 k of NT rows
   static constexpr int C = NT == 16 || NT == 128 ? 8 : 16;  // columns per chunk
@@ -89,6 +96,23 @@ struct Cfg {
   static constexpr int SCALE_BYTES = SCALES * GPB * 512;
   // Routes and weights of a tile's rows, of two tiles: [2][2][NT].
   static constexpr int ROUTE_BYTES = KIND == kDown ? 16 * NT : 0;
+  // Shared memory beside the stages of codes.
+  __host__ __device__ static constexpr int fixed_bytes(int split) {
+    return BS * B_BYTES + OUT_BYTES + SCALE_BYTES + ROUTE_BYTES + (split - 1) * NT * 512 +
+           TAIL_BYTES;
+  }
+  // Stages of codes: as many as there is room for.  The decoding groups take
+  // alternate blocks, and a wait goes by the parity of a stage's use: the group
+  // that asks for use u has to know that use u - 1 has landed.  With DG | stages
+  // that was a block of its own; else it knows of the blocks up to b - DG - BS,
+  // whose products ended before it took the operand stage of block b - DG, and use
+  // u - 1 is among them with BS + DG stages or more.  Five stages of codes beside
+  // four of operands become four.
+  __host__ __device__ static constexpr int code_stages(int block_bytes, int split) {
+    const int room = (SMEM_LIMIT - fixed_bytes(split)) / block_bytes;
+    const int ws = room > MAX_WS ? MAX_WS : room;
+    return ws < BS + DG ? ws / DG * DG : ws;
+  }
 };
 
 struct Args {
@@ -932,7 +956,7 @@ int launch(const CUtensorMap &mx, const CUtensorMap &mwhole, Args a, double item
   int best = 1;
   double best_time = 1e30;
   for (int sp = 1; sp <= 8 && sp <= a.num_kb; sp *= 2) {
-    if ((sp - 1) * NT > 112) break;
+    if (!split_ok(sp, NT)) break;
     const double rounds = static_cast<double>(
         static_cast<int64_t>((items + sms / sp - 1) / (sms / sp)));
     const double time = rounds * ((a.num_kb + sp - 1) / sp + 2.0 + (sp > 1 ? 1.0 : 0.0));
@@ -942,17 +966,15 @@ int launch(const CUtensorMap &mx, const CUtensorMap &mwhole, Args a, double item
     }
   }
   a.split = best;
-  const int64_t fixed = static_cast<int64_t>(C::BS) * C::B_BYTES + C::OUT_BYTES + C::SCALE_BYTES + C::ROUTE_BYTES +
-                        static_cast<int64_t>(a.split - 1) * NT * 512 + TAIL_BYTES;
-  a.ws = static_cast<int>((SMEM_LIMIT - fixed) / a.sh.block_bytes());
-  if (a.ws > MAX_WS) a.ws = MAX_WS;
+  a.ws = C::code_stages(a.sh.block_bytes(), a.split);
   int clusters = sms / a.split;
   const int64_t most = (KIND == kLinear ? (a.m + NT - 1) / NT : a.max_mtiles) * a.n_blocks;
   if (most < clusters) clusters = static_cast<int>(most < 1 ? 1 : most);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(clusters * a.split);
   cfg.blockDim = dim3(C::THREADS);
-  cfg.dynamicSmemBytes = 1024 + static_cast<size_t>(fixed) + static_cast<size_t>(a.ws) * a.sh.block_bytes();
+  cfg.dynamicSmemBytes =
+      1024 + static_cast<size_t>(C::fixed_bytes(a.split)) + static_cast<size_t>(a.ws) * a.sh.block_bytes();
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   int n = 0;
@@ -990,6 +1012,27 @@ int rows_map(CUtensorMap *map, const void *base, int64_t rows, int k, int box_ro
   const uint64_t strides[1] = {static_cast<uint64_t>(k) * 2};
   const uint32_t box[2] = {64, static_cast<uint32_t>(box_rows)};
   return tcg::make_map(map, base, 2, dims, strides, box);
+}
+
+template <int KIND>
+int stages_of(int nt, const Shape &sh, int split) {
+  auto of = [&](auto rows, auto gpb) {
+    return Cfg<decltype(rows)::value, decltype(gpb)::value, KIND>::code_stages(sh.block_bytes(),
+                                                                               split);
+  };
+  auto by_group = [&](auto rows) {
+    switch (sh.groups_per_block()) {
+      case 1: return of(rows, std::integral_constant<int, 1>{});
+      case 2: return of(rows, std::integral_constant<int, 2>{});
+      default: return of(rows, std::integral_constant<int, 4>{});
+    }
+  };
+  switch (nt) {
+    case 16: return by_group(std::integral_constant<int, 16>{});
+    case 32: return by_group(std::integral_constant<int, 32>{});
+    case 64: return by_group(std::integral_constant<int, 64>{});
+    default: return by_group(std::integral_constant<int, 128>{});
+  }
 }
 
 // The smallest tile that holds `rows` rows.
@@ -1083,3 +1126,21 @@ int w4_down_tc(const void *act, int hidden, int inter, const void *w2, const w4:
 }
 
 }  // namespace b200moe
+
+extern "C" int b200moe_w4_ring_stages(int product, int tile_rows, int group, int flags, int split,
+                                      int *code_stages, int *operand_stages) {
+  using namespace b200moe;
+  using namespace b200moe::w4g;
+  B200_ARG(product >= kLinear && product <= kDown, "unknown product code %d", product);
+  B200_ARG(tile_rows == 16 || tile_rows == 32 || tile_rows == 64 || tile_rows == 128,
+           "no tile of %d rows", tile_rows);
+  B200_ARG(w4::group_ok(group), "group size %d must be 32, 64 or 128", group);
+  B200_ARG(split_ok(split, tile_rows), "no clusters of %d CTAs with %d rows", split, tile_rows);
+  B200_ARG(code_stages && operand_stages, "null pointer argument");
+  const w4::Shape sh = w4::shape_of(group, flags);
+  *code_stages = product == kLinear   ? stages_of<kLinear>(tile_rows, sh, split)
+                 : product == kGateUp ? stages_of<kGateUp>(tile_rows, sh, split)
+                                      : stages_of<kDown>(tile_rows, sh, split);
+  *operand_stages = operand_stages_of(product, tile_rows);
+  return B200MOE_OK;
+}

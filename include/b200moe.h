@@ -639,6 +639,14 @@ B200MOE_API int b200moe_w4_pack(const uint8_t *codes, const void *scales, const 
                                 void *out, void *stream);
 
 /*
+ * Stages of shared memory that the tcgen05 product with 4-bit weights cycles
+ * through: of packed codes and of operands.  product: 0 dense, 1 gate/up, 2
+ * down; tile_rows: rows of x per tile; split: CTAs per cluster.
+ */
+B200MOE_API int b200moe_w4_ring_stages(int product, int tile_rows, int group, int flags, int split,
+                                       int *code_stages, int *operand_stages);
+
+/*
  * Dense product out[m, n] = sum_k x[m, k] W[n, k], fp32 sums, bf16 out.
  *   x [m, k] bf16, w one laid-out matrix [n, k], out [m, n] bf16; 16-byte aligned.
  */
