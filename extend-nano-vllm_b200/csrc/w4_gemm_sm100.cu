@@ -897,9 +897,9 @@ __global__ void __launch_bounds__(Cfg<NT, GPB, KIND>::THREADS, 1)
   tc_fence_after();
   if (split > 1) cluster_sync();  // the peers' barriers are ready
   c.tmem = *tmem_holder;
-  // Codes are constant; a dense call's items are known too, so its first
-  // blocks are fetched while the previous kernel still runs.
-  if (!(KIND == kLinear && warp == 0)) pdl_wait();
+  // Every role, that of the codes too: the kernel before may be the one that packs
+  // or updates them, and only this wait promises that its writes are seen.
+  pdl_wait();
   const int mt = KIND == kLinear
                      ? static_cast<int>((args.m + NT - 1) / NT)
                      : static_cast<int>(min64(args.counters[B200MOE_CNT_MTILES], args.max_mtiles));

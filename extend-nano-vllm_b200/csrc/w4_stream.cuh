@@ -15,10 +15,10 @@
 // read back by a third; that pays from more than 16 rows on, w4_gemm_sm100.cu:
 // 16 rows x [151552, 4096] take 92 us here and 107 there, 32 rows 220 and 107.)
 //
-// Measured (back to back, weights larger than L2): 1 row x [75776, 4096] 33.6 us
-// = 4.76 TB/s of weights, 8 rows x [151552, 4096] 65.7 us = 4.87 TB/s, 16 rows
-// 91.5 us = 3.50 TB/s; 8 rows x [75776, 4096] with groups of 32 and zero points
-// 48.4 us = 3.81 TB/s; copy peak 6.5 TB/s.  What bounds it: no one unit.  With 8
+// Measured (back to back, weights larger than L2): 1 row x [75776, 4096] 34.4 us
+// = 4.65 TB/s of weights, 8 rows x [151552, 4096] 67.0 us = 4.78 TB/s, 16 rows
+// 92.1 us = 3.48 TB/s; 8 rows x [75776, 4096] with groups of 32 and zero points
+// 49.3 us = 3.74 TB/s; copy peak 6.5 TB/s.  What bounds it: no one unit.  With 8
 // rows the schedulers issue in 59 % of cycles (297 instructions per 32 x 128
 // weights) and wait for loads and for the decoding's integer pipe in turn; 16 warps
 // with a block in flight each are what the registers hold.  A row's four units lie
@@ -232,14 +232,13 @@ __device__ __forceinline__ void add_block(const Block<GPB, ZEROS> &b, bool half_
 }
 
 // Adds an item's share of a warp, the blocks part, part + wk, ... of the quarter
-// at w.  The block after the one at work is on its way meanwhile; the first is
-// asked for before the wait for x.  (Asking for the next item's first block too
-// costs more in the loop than it gains: 8 rows 78 us against 68, 64 tokens
-// through 128 experts 126 against 118.)
+// at w.  The block after the one at work is on its way meanwhile.  (Asking for the
+// next item's first block too costs more in the loop than it gains: 8 rows 78 us
+// against 68, 64 tokens through 128 experts 126 against 118.)
 template <int GPB, int NB, bool ZEROS>
 __device__ __forceinline__ void add_item(const Args &a, const uint8_t *w, int part,
                                          const __nv_bfloat16 *const (&xp)[NB], int lane,
-                                         bool wait_x, float (&tot)[2][NB][4]) {
+                                         float (&tot)[2][NB][4]) {
   const bool half_scale = a.sh.half_scale != 0;
   const int wk = a.wk;
   constexpr int kBlock = 4 * (w4::kCodeBytes + GPB * (ZEROS ? 96 : 64));
@@ -247,7 +246,6 @@ __device__ __forceinline__ void add_item(const Args &a, const uint8_t *w, int pa
   const int64_t hop = static_cast<int64_t>(wk) * kBlock;
   Block<GPB, ZEROS> even, odd;
   even.load(w, lane);
-  if (wait_x) pdl_wait();
   auto step = [&](int kb, const Block<GPB, ZEROS> &now, Block<GPB, ZEROS> &next) {
     Rows<NB> x;
 #pragma unroll
@@ -348,7 +346,9 @@ __global__ void __launch_bounds__(32 * kWarps, 2) w4_stream_kernel(
   const int wk = a.wk;
   const int wr = kWarps / wk;  // items of a thread block at a time
   const int part = warp / wr;
-  if (KIND != kLinear) pdl_wait();
+  // Before the codes too: the kernel before may be the one that packs or updates
+  // them, and only this wait promises that its writes are seen.
+  pdl_wait();
   if (by_route) pdl_trigger();
   const int mt = KIND == kLinear ? 1
                  : KIND == kGateUp && a.ids != nullptr
@@ -357,8 +357,6 @@ __global__ void __launch_bounds__(32 * kWarps, 2) w4_stream_kernel(
   const int items = mt * 4 * a.n_blocks;
   const int stride = gridDim.x * wr;
   const int begin = blockIdx.x * wr + warp % wr;
-
-  bool wait_x = KIND == kLinear;  // codes are constant, x is not
 
   // All warps of a block take the same number of turns (they meet when k is
   // shared); a turn past the end does nothing.
@@ -387,8 +385,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) w4_stream_kernel(
                                                   a.top_k, a.num_routes, a.x_rows);
           xp[n] = static_cast<const __nv_bfloat16 *>(a.x) + row * a.k + 8 * t;
         }
-        add_item<GPB, NB, ZEROS>(a, it.w, part, xp, lane, wait_x, tot);
-        wait_x = false;
+        add_item<GPB, NB, ZEROS>(a, it.w, part, xp, lane, tot);
       }
       if (wk == 1) {
         if (rows > 0) {

@@ -21,9 +21,10 @@ __global__ void __launch_bounds__(32 * kWarps) w4_down_slots_kernel(
   const int64_t token = blockIdx.y;
   const bool zeros = sh.has_zero != 0;
   const int bytes = sh.block_bytes();
-  // The gate/up kernel before this one lets it start only after its own wait,
-  // so the routes are there: the first blocks of codes are fetched while that
-  // kernel still computes act.
+  // Only w4_route_gate_up comes before this kernel, and each of its blocks lets it
+  // start after its own wait: every kernel before that one has ended and its writes
+  // are seen, so the routes and the codes are there, and the first blocks are
+  // fetched while gate/up still computes act.
   bool act_ready = false;
   for (int s = warp; s < top_k; s += kWarps) {
     const int64_t route = token * top_k + s;
