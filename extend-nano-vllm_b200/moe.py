@@ -65,6 +65,12 @@ def _capturing() -> bool:
     return torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
 
 
+def _moved(fn, tensor: torch.Tensor) -> torch.Tensor:
+    """What ``nn.Module._apply``'s ``fn`` makes of a tensor whose type stays."""
+    out = fn(tensor)
+    return out if out.dtype == tensor.dtype else tensor.to(out.device)
+
+
 def reduce_fp64_to_bf16(local_output: torch.Tensor, group, output_dtype=torch.bfloat16
                         ) -> torch.Tensor:
     """fp64 reduce-scatter then all-gather in ``output_dtype`` (moe.py:41-58)."""
@@ -150,7 +156,7 @@ class SharedExpertMLP(nn.Module):
     def _apply(self, fn, recurse=True):
         super()._apply(fn, recurse)
         for weight in self._w4 or ():
-            weight.data = fn(weight.data)
+            weight.data = _moved(fn, weight.data)
         return self
 
     def forward(self, hidden_states: torch.Tensor) -> torch.Tensor:
@@ -376,14 +382,20 @@ class ExpertParallelMoE(nn.Module):
 
     def _apply(self, fn, recurse=True):
         # Device and dtype moves rebuild every parameter separately; put the
-        # shared expert back behind the routed experts afterwards.
-        super()._apply(fn, recurse)
+        # shared expert back behind the routed experts afterwards.  The selection
+        # bias moves by itself: it stays fp32, with its values.
+        bias, self.route_bias = self.route_bias, None
+        try:
+            super()._apply(fn, recurse)
+            moved = None if bias is None else _moved(fn, bias)
+        except BaseException:
+            self.route_bias = bias
+            raise
+        self.route_bias = moved
         if getattr(self, "_shared_in_store", False) and self._w4 is None:
             self._bind_shared_store()
         for weight in self._w4 or ():
-            weight.data = fn(weight.data)
-        if self.route_bias is not None and self.route_bias.dtype != torch.float32:
-            self.route_bias = self.route_bias.float()  # scores stay fp32
+            weight.data = _moved(fn, weight.data)
         return self
 
     # ------------------------------------------------------------------
