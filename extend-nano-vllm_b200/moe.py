@@ -349,6 +349,12 @@ class ExpertParallelMoE(nn.Module):
     # ------------------------------------------------------------------
     # Shared expert storage.
     # ------------------------------------------------------------------
+    def _shared_stored(self) -> bool:
+        """Whether the shared expert's bf16 weights belong behind the routed
+        experts': same width, and neither of them holds 4-bit weights."""
+        return (getattr(self, "_shared_in_store", False) and self._w4 is None
+                and self.shared_expert._w4 is None)
+
     def _shared_pairs(self):
         return ((self.gate_up_proj, self.shared_expert.gate_up_proj.weight),
                 (self.down_proj, self.shared_expert.down_proj.weight))
@@ -392,7 +398,7 @@ class ExpertParallelMoE(nn.Module):
             self.route_bias = bias
             raise
         self.route_bias = moved
-        if getattr(self, "_shared_in_store", False) and self._w4 is None:
+        if self._shared_stored():
             self._bind_shared_store()
         for weight in self._w4 or ():
             weight.data = _moved(fn, weight.data)
@@ -509,9 +515,9 @@ class ExpertParallelMoE(nn.Module):
         """The shared expert runs inside the grouped expert path: same width
         as the routed experts, one EP rank (with several, the reference adds
         it once per rank after the exchange), the native kernels."""
-        return (self.shared_expert is not None and getattr(self, "_shared_in_store", False)
+        return (self._shared_stored()
                 and self.fuse_shared_expert and self.ep_size == 1 and self._ops is _native_ops and x.is_cuda
-                and self.top_k < 32 and self._scored is None and self._w4 is None)
+                and self.top_k < 32 and self._scored is None)
 
     # ------------------------------------------------------------------
     # Counters (moe.py:384-393).  Kernels accumulate local assignments and

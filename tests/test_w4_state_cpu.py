@@ -5,6 +5,7 @@ replaced by a stand-in that keeps the shapes; nothing is computed."""
 import pytest
 import torch
 
+from extend_nano_vllm_b200 import _lib, ops
 from extend_nano_vllm_b200.moe import ExpertParallelMoE
 
 
@@ -30,3 +31,37 @@ def test_the_selection_bias_follows_the_device():
     layer.to("meta", torch.bfloat16)
     assert layer.route_bias.device.type == "meta" and layer.route_bias.dtype == torch.float32
     assert ExpertParallelMoE(64, 32, 8, 2, True).to(torch.bfloat16).route_bias is None
+
+
+@pytest.fixture
+def packed_by_shape(monkeypatch):
+    """ops.pack_w4 without a GPU: the shapes and flags of a packed weight."""
+    def pack(codes, scales, zeros=None, *, layout="rows"):
+        rows, k = codes.shape[-2:]
+        flags = ((_lib.W4_ZEROS if zeros is not None else 0)
+                 | (_lib.W4_GATE_UP if layout == "gate_up" else 0))
+        matrices = codes.size(0) if codes.dim() == 3 else 1
+        group = k // scales.size(-1)
+        size = _lib.LIB.b200moe_w4_bytes(matrices, rows, k, group, flags)
+        return ops.W4Weight(torch.zeros(size, dtype=torch.uint8), matrices, rows, k, group, flags)
+    monkeypatch.setattr(ops, "pack_w4", pack)
+
+
+def layer_of(shared=None, **kw):
+    layer = ExpertParallelMoE(64, 32, 8, 2, True, shared_expert_intermediate_size=shared, **kw)
+    with torch.no_grad():
+        for p in layer.parameters():
+            p.normal_(0.0, 0.02, generator=torch.Generator().manual_seed(p.numel()))
+    return layer.bfloat16()
+
+
+@pytest.mark.parametrize("shared", [32, 64])
+def test_a_shared_expert_with_4_bits_alone(packed_by_shape, shared):
+    layer = layer_of(shared)
+    before = layer.gate_up_proj.detach().clone(), layer.down_proj.detach().clone()
+    layer.shared_expert.quantize_w4(32)
+    x = torch.empty(3, 64, dtype=torch.bfloat16)
+    x_on_gpu = type("OnGpu", (), {"is_cuda": True})()
+    assert not layer._fused_shared(x) and not layer._fused_shared(x_on_gpu)
+    moved = layer.to(torch.bfloat16).float().bfloat16()
+    assert torch.equal(moved.gate_up_proj, before[0]) and torch.equal(moved.down_proj, before[1])
