@@ -148,10 +148,19 @@ class SharedExpertMLP(nn.Module):
             linear.weight.data = linear.weight.data.new_empty((0, linear.input_size))
 
     @torch.no_grad()
+    def pack_w4(self, group: int = 128, zeros: bool = False
+                ) -> tuple[_native_ops.W4Weight, _native_ops.W4Weight]:
+        """The bf16 weights rounded to 4 bits and packed (``set_w4_weights``)."""
+        if self._w4 is not None:
+            raise RuntimeError("the shared expert holds 4-bit weights already")
+        gate_up, down = (
+            _native_ops.pack_w4(*_native_ops.quantize_w4(w, group, zeros))
+            for w in (self.gate_up_proj.weight, self.down_proj.weight))
+        return gate_up, down
+
     def quantize_w4(self, group: int = 128, zeros: bool = False) -> None:
         """Round the weights to 4 bits with group scales (``ops.quantize_w4``)."""
-        self.set_w4_weights(*(_native_ops.pack_w4(*_native_ops.quantize_w4(w, group, zeros))
-                              for w in (self.gate_up_proj.weight, self.down_proj.weight)))
+        self.set_w4_weights(*self.pack_w4(group, zeros))
 
     def _apply(self, fn, recurse=True):
         super()._apply(fn, recurse)
@@ -432,14 +441,18 @@ class ExpertParallelMoE(nn.Module):
         self._scored = dict(score=score, num_groups=num_groups, topk_groups=topk_groups,
                             group_score=group_score, scale=float(scale))
 
-    def set_w4_weights(self, w13: _native_ops.W4Weight, w2: _native_ops.W4Weight) -> None:
-        """Run the experts with 4-bit weights (``ops.pack_w4``: w13 [E, 2 I, H] in
-        the "gate_up" layout, w2 [E, H, I]) and release the bf16 ones.  One EP
-        rank; the layer's weights can no longer be loaded or relocated."""
+    def _check_w4_supported(self) -> None:
         if self.ep_size != 1:
             raise NotImplementedError("4-bit expert weights need one EP rank")
         if self.fp64_combine:
             raise NotImplementedError("4-bit expert weights have no FP64 combine")
+
+    def set_w4_weights(self, w13: _native_ops.W4Weight, w2: _native_ops.W4Weight) -> None:
+        """Run the experts with 4-bit weights (``ops.pack_w4``: w13 [E, 2 I, H] in
+        the "gate_up" layout, w2 [E, H, I]) and release the bf16 ones.  One EP
+        rank; the layer's weights can no longer be loaded or relocated.  A call
+        that raises leaves the layer as it was."""
+        self._check_w4_supported()
         hidden, inter = self.hidden_size, self.intermediate_size
         if (w13.matrices, w13.rows, w13.k) != (self.num_experts, 2 * inter, hidden) \
                 or not w13.flags & _lib.W4_GATE_UP:
@@ -449,30 +462,35 @@ class ExpertParallelMoE(nn.Module):
                 or w2.flags & _lib.W4_GATE_UP:
             raise ValueError(f"w2 must be {self.num_experts} x [{hidden}, {inter}] in the "
                              "\"rows\" layout")
-        self._w4 = (w13, w2)
-        if self._shared_in_store and self.shared_expert._w4 is None:
+        if self._shared_stored():
             # The shared expert keeps its weights without the routed experts'.
-            shared = self.shared_expert
-            for linear in (shared.gate_up_proj, shared.down_proj):
-                linear.weight.data = linear.weight.data.clone()
+            linears = self.shared_expert.gate_up_proj, self.shared_expert.down_proj
+            copies = [linear.weight.data.clone() for linear in linears]
+            for linear, copy in zip(linears, copies):
+                linear.weight.data = copy
+        self._w4 = (w13, w2)
         self.gate_up_proj.data = self.gate_up_proj.data.new_empty((0, 2 * inter, hidden))
         self.down_proj.data = self.down_proj.data.new_empty((0, hidden, inter))
 
     @torch.no_grad()
     def quantize_w4(self, group: int = 128, zeros: bool = False) -> None:
-        """Round the experts' weights, and the shared expert's, to 4 bits with
-        group scales (``ops.quantize_w4``) and release the bf16 ones."""
-        if self.ep_size != 1:
-            raise NotImplementedError("4-bit expert weights need one EP rank")
+        """Round the experts' weights, and those of a bf16 shared expert, to 4 bits
+        with group scales (``ops.quantize_w4``) and release the bf16 ones.  A call
+        that raises leaves the layer as it was."""
+        self._check_w4_supported()
+        if self._w4 is not None:
+            raise RuntimeError("the experts hold 4-bit weights already")
         parts = []
         for param in (self.gate_up_proj, self.down_proj):
             # One expert at a time: the fp32 intermediate stays small.
             experts = [_native_ops.quantize_w4(w, group, zeros) for w in param]
             parts.append([None if t[0] is None else torch.stack(t) for t in zip(*experts)])
-        if self.shared_expert is not None:  # first: it may refuse the group size
-            self.shared_expert.quantize_w4(group, zeros)
-        self.set_w4_weights(_native_ops.pack_w4(*parts[0], layout="gate_up"),
-                            _native_ops.pack_w4(*parts[1]))
+        # Everything is packed before anything is swapped in.
+        packed = (_native_ops.pack_w4(*parts[0], layout="gate_up"),
+                  _native_ops.pack_w4(*parts[1]))
+        if self.shared_expert is not None and self.shared_expert._w4 is None:
+            self.shared_expert.set_w4_weights(*self.shared_expert.pack_w4(group, zeros))
+        self.set_w4_weights(*packed)
 
     def _select(self, logits: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """Router logits -> (bf16 weights, int64 ids) [T, k]."""

@@ -54,3 +54,17 @@ def test_routed_experts_with_4_bits_beside_a_bf16_shared_expert(tokens):
         assert torch.equal(layer(x), want)
         assert torch.equal(layer.to("cpu").to(DEV)(x), want)
     assert device_status() == 0
+
+
+def test_rounding_in_two_steps_is_rounding_in_one():
+    x = torch.randn((40, 256), generator=torch.Generator(device=DEV).manual_seed(2),
+                    device=DEV).bfloat16()
+    with torch.no_grad():
+        one, two = make(128), make(128)
+        one.quantize_w4(64)
+        two.shared_expert.quantize_w4(64)
+        two.quantize_w4(64)
+        assert torch.equal(one(x), two(x))
+        with pytest.raises(RuntimeError, match="4-bit weights already"):
+            two.quantize_w4(64)
+        assert torch.equal(one(x), two(x))

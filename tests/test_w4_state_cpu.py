@@ -65,3 +65,61 @@ def test_a_shared_expert_with_4_bits_alone(packed_by_shape, shared):
     assert not layer._fused_shared(x) and not layer._fused_shared(x_on_gpu)
     moved = layer.to(torch.bfloat16).float().bfloat16()
     assert torch.equal(moved.gate_up_proj, before[0]) and torch.equal(moved.down_proj, before[1])
+
+
+def state(layer):
+    shared = layer.shared_expert
+    return ({n: p.detach().clone() for n, p in layer.named_parameters()}, layer._w4,
+            shared and shared._w4)
+
+
+def same(a, b):
+    return (a[0].keys() == b[0].keys() and all(torch.equal(v, b[0][n]) for n, v in a[0].items())
+            and a[1:] == b[1:])
+
+
+@pytest.mark.parametrize("shared", [None, 32, 64])
+def test_a_refused_rounding_leaves_the_layer_as_it_was(packed_by_shape, shared):
+    layer = layer_of(shared)
+    layer.fp64_combine = True
+    before = state(layer)
+    with pytest.raises(NotImplementedError, match="FP64"):
+        layer.quantize_w4(32)
+    assert same(state(layer), before)
+    layer.fp64_combine = False
+    with pytest.raises(ValueError, match="multiple of the group size"):
+        layer.quantize_w4(64)  # the routed experts' 32 k
+    assert same(state(layer), before)
+    layer.quantize_w4(32)
+    assert layer._w4 is not None and (shared is None or layer.shared_expert._w4 is not None)
+
+
+@pytest.mark.parametrize("fails", range(4))
+def test_a_packing_that_fails_leaves_the_layer_as_it_was(packed_by_shape, monkeypatch, fails):
+    layer, pack, calls = layer_of(64), ops.pack_w4, []
+
+    def failing(*args, **kw):
+        calls.append(args)
+        if len(calls) == fails + 1:
+            raise torch.OutOfMemoryError("no memory")
+        return pack(*args, **kw)
+
+    monkeypatch.setattr(ops, "pack_w4", failing)
+    before = state(layer)
+    with pytest.raises(torch.OutOfMemoryError):
+        layer.quantize_w4(32)
+    assert same(state(layer), before)
+
+
+@pytest.mark.parametrize("shared", [32, 64])
+def test_rounding_one_part_after_the_other_and_twice(packed_by_shape, shared):
+    layer = layer_of(shared)
+    layer.shared_expert.quantize_w4(32)
+    held = layer.shared_expert._w4
+    layer.quantize_w4(32)
+    assert layer._w4 is not None and layer.shared_expert._w4 is held
+    before = state(layer)
+    for again in (layer, layer.shared_expert):
+        with pytest.raises(RuntimeError, match="4-bit weights already"):
+            again.quantize_w4(32)
+    assert same(state(layer), before)
