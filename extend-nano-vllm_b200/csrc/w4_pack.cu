@@ -6,7 +6,9 @@
 namespace b200moe {
 namespace {
 
-// One block of the layout per thread block, one row per thread.
+// One block of the layout per thread block, one row per thread.  A code or zero
+// point above 15 has no place in the layout: its low four bits are taken, and the
+// status word says that it was there.
 __global__ void __launch_bounds__(w4::kTileRows) w4_pack_kernel(
     const uint8_t *codes, const uint16_t *scales, const uint8_t *zeros, int64_t rows, int64_t k,
     w4::Shape sh, int gate_up, uint8_t *out) {
@@ -29,6 +31,7 @@ __global__ void __launch_bounds__(w4::kTileRows) w4_pack_kernel(
   uint8_t *quarter = block + (row >> 5) * sh.quarter_bytes();
   const uint8_t *crow = codes + (mat * rows + src) * k;
   uint32_t word[4][4];  // [unit][chunk of 32 k]
+  uint32_t high = 0;    // bits of codes and zero points above the lowest four
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
 #pragma unroll
@@ -38,6 +41,8 @@ __global__ void __launch_bounds__(w4::kTileRows) w4_pack_kernel(
       uint32_t in[8];
       *reinterpret_cast<uint4 *>(in) = *reinterpret_cast<const uint4 *>(crow + k0);
       *reinterpret_cast<uint4 *>(in + 4) = *reinterpret_cast<const uint4 *>(crow + k0 + 16);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) high |= in[i] & 0xf0f0f0f0u;
 #pragma unroll
       for (int u = 0; u < 4; ++u)
 #pragma unroll
@@ -57,10 +62,13 @@ __global__ void __launch_bounds__(w4::kTileRows) w4_pack_kernel(
     const int64_t at = (mat * rows + src) * groups + gi;
     reinterpret_cast<uint16_t *>(quarter + sh.scale_off())[g * 32 + place] =
         in ? scales[at] : static_cast<uint16_t>(0);
-    if (sh.has_zero)
-      quarter[sh.zero_off() + g * 32 + place] =
-          in ? static_cast<uint8_t>(zeros[at] & 15) : static_cast<uint8_t>(0);
+    if (sh.has_zero) {
+      const uint32_t z = in ? zeros[at] : 0u;
+      high |= z & 0xf0u;
+      quarter[sh.zero_off() + g * 32 + place] = static_cast<uint8_t>(z & 15u);
+    }
   }
+  if (high) atomicOr(&g_status, kStatusIndex);
 }
 
 }  // namespace

@@ -588,9 +588,11 @@ def quantize_w4(weight: torch.Tensor, group: int = 128, zeros: bool = False
 def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None, *,
             layout: str = "rows") -> W4Weight:
     """Lay codes [rows, k] or [matrices, rows, k] (uint8 0..15), scales (bf16 or
-    fp16) and optional zero points (uint8) [..., rows, k / group] out for the
+    fp16) and optional zero points (uint8 0..15) [..., rows, k / group] out for the
     kernels, once.  ``layout="gate_up"``: the rows are a SwiGLU pair [2 I, k],
-    gate rows first (the first weight of ``experts_w4``)."""
+    gate rows first (the first weight of ``experts_w4``).  The codes and zero
+    points are looked through for values above 15, which synchronises (under
+    stream capture only the device status word tells)."""
     _require_cuda(codes, scales, zeros)
     if layout not in ("rows", "gate_up"):
         raise ValueError(f"unknown layout {layout!r}")
@@ -615,6 +617,10 @@ def pack_w4(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | Non
     if size < 0:
         raise ValueError(f"no 4-bit layout for {matrices} x [{rows}, {k}] in groups of {group} "
                          "(32, 64 or 128; a gate_up weight has an even number of rows)")
+    if not torch.cuda.is_current_stream_capturing():
+        for name, t in (("codes", codes), ("zeros", zeros)):
+            if t is not None and int(t.max()) > 15:
+                raise ValueError(f"{name} must be 0..15, got {int(t.max())}")
     codes, scales = _aligned(codes), scales.contiguous()
     zeros = None if zeros is None else zeros.contiguous()
     data = torch.empty(size, device=codes.device, dtype=torch.uint8)

@@ -631,6 +631,8 @@ B200MOE_API int b200moe_route_scored_topk(const void *logits, int logits_dtype,
  *   codes  [matrices, rows, k] uint8, one code per byte (16-byte aligned)
  *   scales [matrices, rows, k / group] bf16 or fp16 (B200MOE_W4_F16_SCALES)
  *   zeros  [matrices, rows, k / group] uint8, with B200MOE_W4_ZEROS
+ * A code or zero point above 15 cannot be laid out: its low four bits are, and
+ * bit 1 of the device status word is set (b200moe_device_status).
  */
 B200MOE_API int64_t b200moe_w4_bytes(int64_t matrices, int64_t rows, int64_t k, int group,
                                      int flags);
