@@ -3,8 +3,9 @@
 //
 //   s_e = 1 / (1 + exp(-l_e))  or  exp(l_e - max l) / sum exp(l - max l)
 //   c_e = s_e + b_e                                    (what the choice goes by)
-//   v_g = max or sum of the two largest c of group g; the topk_groups groups
-//         with the largest v stay (lowest index first among equals)
+//   v_g = max or sum of the two largest c of group g (+inf where the largest is
+//         +inf, whatever the other); the topk_groups groups with the largest v
+//         stay (lowest index first among equals)
 //   ids = the top_k experts with the largest c in them (lowest id first)
 //   w   = s_ids / sum(s_ids) * scale                   (the bias is not in it)
 //
@@ -123,7 +124,9 @@ __global__ void __launch_bounds__(32 * kWarps) route_scored_kernel(const T *logi
       second = fmaxf(fminf(best, b), fmaxf(second, d));
       best = fmaxf(best, b);
     }
-    const float value = a.top2 && size > 1 ? best + second : best;
+    // A choice of +inf (a forced expert) beside others of -inf has no sum: its
+    // group counts as +inf.
+    const float value = a.top2 && size > 1 && best < INFINITY ? best + second : best;
     // Rank of each group: how many come before it.
     const uint32_t mine = group < a.groups ? order_key(value) : 0u;
     int before = 0;

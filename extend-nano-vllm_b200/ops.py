@@ -508,7 +508,8 @@ def route_scored_topk(logits: torch.Tensor, top_k: int, *, score: str = "softmax
     by ``scale``.  With ``num_groups`` > 1 the experts form that many equal
     groups and only the ``topk_groups`` best ones are on offer; a group's
     score is its largest biased score ("max") or the sum of its two largest
-    ("top2").  Equal values go to the lowest index."""
+    ("top2"; +inf where the largest is +inf).  Equal values go to the lowest
+    index."""
     if not logits.is_cuda:
         _require_cuda(logits)
     dtype = _LOGIT_DTYPES.get(logits.dtype)

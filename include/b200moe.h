@@ -600,7 +600,8 @@ B200MOE_API int b200moe_nvl_wait_return(int rank, int ep_size, const uint64_t *p
  * Scored routing, for layers whose router is not a plain softmax top-k:
  *   s_e = sigmoid(l_e) or softmax(l)_e,  c_e = s_e + bias_e,
  *   the topk_groups of num_groups equal expert groups with the largest group
- *   score (largest c, or sum of the two largest c) stay on offer, the top_k
+ *   score (largest c, or sum of the two largest c; +inf where the largest is
+ *   +inf) stay on offer, the top_k
  *   experts with the largest c among them are chosen (equal values: lowest
  *   index first), and
  *   weight = s_id [/ sum of the chosen s] * scale, rounded to bf16.
