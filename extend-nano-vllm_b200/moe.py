@@ -120,11 +120,62 @@ class SharedMergedGate(ReplicatedGate):
                           self.intermediate_size).copy_(loaded_weight)
 
 
-class SharedExpertMLP(nn.Module):
+class _W4Holder(nn.Module):
+    """A module that may hold two 4-bit weights (``_w4``, ``set_w4_weights``) in
+    place of bf16 parameters: its state dict carries them, each as the packed
+    bytes and their layout [matrices, rows, k, group, flags]."""
+
+    _w4_names: tuple[str, str]
+    _w4: tuple[_native_ops.W4Weight, _native_ops.W4Weight] | None
+
+    def _save_to_state_dict(self, destination, prefix, keep_vars):
+        super()._save_to_state_dict(destination, prefix, keep_vars)
+        for name, weight in zip(self._w4_names, self._w4 or ()):
+            destination[f"{prefix}{name}"] = weight.data
+            destination[f"{prefix}{name}_layout"] = torch.tensor(weight.layout)
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys,
+                              unexpected_keys, error_msgs):
+        names = [f"{prefix}{name}{end}" for name in self._w4_names for end in ("", "_layout")]
+        saved = [state_dict.get(name) for name in names]
+        if all(t is not None for t in saved):
+            try:
+                # Before the bf16 parameters, which are empty beside 4-bit weights.
+                self._load_w4(names, saved)
+            except (ValueError, NotImplementedError) as exc:
+                error_msgs.append(str(exc))
+        elif strict and (self._w4 is not None or any(t is not None for t in saved)):
+            missing_keys += [name for name, t in zip(names, saved) if t is None]
+        super()._load_from_state_dict({k: v for k, v in state_dict.items() if k not in names},
+                                      prefix, local_metadata, strict, missing_keys,
+                                      unexpected_keys, error_msgs)
+
+    def _load_w4(self, names: list[str], saved: list[torch.Tensor]) -> None:
+        weights = []
+        for name, data, layout in zip(names[::2], saved[::2], saved[1::2]):
+            layout = [int(v) for v in layout.flatten()]
+            size = int(_lib.LIB.b200moe_w4_bytes(*layout)) if len(layout) == 5 else -1
+            if data.dtype != torch.uint8 or data.dim() != 1 or data.numel() != size:
+                raise ValueError(f"{name} does not hold a 4-bit weight of layout {layout}")
+            weights.append(_native_ops.W4Weight(data, *layout))
+        if self._w4 is not None and all(new.layout == old.layout
+                                        for new, old in zip(weights, self._w4)):
+            for new, old in zip(weights, self._w4):  # in place: captured graphs stay valid
+                old.data.copy_(new.data)
+            return
+        device = next(self.parameters()).device
+        for weight in weights:
+            weight.data = weight.data.to(device, copy=True)
+        self.set_w4_weights(*weights)
+
+
+class SharedExpertMLP(_W4Holder):
     """Dense shared expert (moe.py:212-234), replicated.  With one EP rank and
     the routed experts' width the layer runs it inside the grouped expert
     kernels; otherwise it is computed as the reference does, after the
     routed output."""
+
+    _w4_names = ("w4_gate_up", "w4_down")
 
     def __init__(self, hidden_size: int, intermediate_size: int) -> None:
         super().__init__()
@@ -176,8 +227,10 @@ class SharedExpertMLP(nn.Module):
         return self.down_proj(F.silu(gate) * up)
 
 
-class ExpertParallelMoE(nn.Module):
+class ExpertParallelMoE(_W4Holder):
     """Qwen3-MoE sparse block with the reference's constructor and seams."""
+
+    _w4_names = ("w4_w13", "w4_w2")
 
     def __init__(
         self,

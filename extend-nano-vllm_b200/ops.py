@@ -559,6 +559,10 @@ class W4Weight:
     def device(self) -> torch.device:
         return self.data.device
 
+    @property
+    def layout(self) -> list[int]:
+        return [self.matrices, self.rows, self.k, self.group, self.flags]
+
 
 def quantize_w4(weight: torch.Tensor, group: int = 128, zeros: bool = False
                 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:

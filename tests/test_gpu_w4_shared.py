@@ -68,3 +68,25 @@ def test_rounding_in_two_steps_is_rounding_in_one():
         with pytest.raises(RuntimeError, match="4-bit weights already"):
             two.quantize_w4(64)
         assert torch.equal(one(x), two(x))
+
+
+@pytest.mark.parametrize("shared", [128, 96])
+def test_a_saved_layer_computes_the_same(shared, tmp_path):
+    x = torch.randn((40, 256), generator=torch.Generator(device=DEV).manual_seed(3),
+                    device=DEV).bfloat16()
+    with torch.no_grad():
+        layer = make(shared)
+        layer.quantize_w4(32, zeros=True)
+        want = layer(x)
+        torch.save(layer.state_dict(), tmp_path / "layer.pt")
+        saved = torch.load(tmp_path / "layer.pt", map_location="cpu")
+        fresh = ExpertParallelMoE(256, 128, 16, 4, True, shared_expert_intermediate_size=shared)
+        fresh = fresh.to(device=DEV, dtype=torch.bfloat16)
+        fresh.load_state_dict(saved)
+        assert torch.equal(fresh(x), want)
+        again = make(shared)
+        again.quantize_w4(32, zeros=True)
+        for weight in (*again._w4, *again.shared_expert._w4):
+            weight.data.zero_()
+        again.load_state_dict(saved)
+        assert torch.equal(again(x), want)

@@ -123,3 +123,71 @@ def test_rounding_one_part_after_the_other_and_twice(packed_by_shape, shared):
         with pytest.raises(RuntimeError, match="4-bit weights already"):
             again.quantize_w4(32)
     assert same(state(layer), before)
+
+
+def filled(layer, seed):
+    g = torch.Generator().manual_seed(seed)
+    for holder in (layer, layer.shared_expert):
+        for weight in (holder and holder._w4) or ():
+            weight.data.copy_(torch.randint(0, 256, weight.data.shape, generator=g))
+    return layer
+
+
+def packed_of(layer):
+    return [w for holder in (layer, layer.shared_expert) for w in (holder and holder._w4) or ()]
+
+
+@pytest.mark.parametrize("shared", [None, 32, 64])
+@pytest.mark.parametrize("into_rounded", [False, True])
+def test_saved_and_loaded(packed_by_shape, tmp_path, shared, into_rounded):
+    layer = layer_of(shared)
+    layer.quantize_w4(32)
+    filled(layer, 1)
+    torch.save(torch.nn.ModuleDict({"mlp": layer}).state_dict(), tmp_path / "layer.pt")
+    other = layer_of(shared)
+    if into_rounded:
+        other.quantize_w4(32)
+        filled(other, 2)
+        kept = [w.data.data_ptr() for w in packed_of(other)]
+    with torch.no_grad():
+        other.gate.weight.zero_()
+    torch.nn.ModuleDict({"mlp": other}).load_state_dict(torch.load(tmp_path / "layer.pt"))
+    assert torch.equal(other.gate.weight, layer.gate.weight)
+    assert len(packed_of(other)) == (2 if shared is None else 4)
+    for a, b in zip(packed_of(layer), packed_of(other)):
+        assert torch.equal(a.data, b.data) and a.data.data_ptr() != b.data.data_ptr()
+        assert (a.matrices, a.rows, a.k, a.group, a.flags) == (b.matrices, b.rows, b.k, b.group,
+                                                              b.flags)
+    if into_rounded:  # in place, so that captured graphs keep their pointers
+        assert [w.data.data_ptr() for w in packed_of(other)] == kept
+    assert other.gate_up_proj.numel() == 0
+    other.to(torch.bfloat16)
+
+
+def test_loading_what_does_not_fit_raises(packed_by_shape):
+    rounded, plain = layer_of(32), layer_of(32)
+    saved = plain.state_dict()
+    assert not any("w4" in name for name in saved)
+    plain.load_state_dict(saved)
+    rounded.quantize_w4(32)
+    with pytest.raises(RuntimeError, match="size mismatch"):
+        rounded.load_state_dict(saved)  # bf16 weights into a rounded layer
+    packed = rounded.state_dict()
+    wider = ExpertParallelMoE(64, 64, 8, 2, True, shared_expert_intermediate_size=32)
+    with torch.no_grad():
+        wider.gate_up_proj.fill_(1.0)
+    before = state(wider)
+    with pytest.raises(RuntimeError, match="w13 must be"):
+        wider.load_state_dict(packed)
+    assert wider._w4 is None and torch.equal(before[0]["gate_up_proj"], wider.gate_up_proj)
+    missing = {n: t for n, t in packed.items() if n != "w4_w2"}
+    with pytest.raises(RuntimeError, match="w4_w2"):
+        rounded.load_state_dict(missing)
+    with pytest.raises(RuntimeError, match="w4_w13"):
+        layer = layer_of(32)
+        layer.quantize_w4(32)
+        layer.load_state_dict({n: t for n, t in packed.items() if "w4" not in n})
+    short = dict(packed)
+    short["w4_w2"] = short["w4_w2"][:-1]
+    with pytest.raises(RuntimeError, match="w4_w2"):
+        rounded.load_state_dict(short)
