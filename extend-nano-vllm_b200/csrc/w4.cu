@@ -33,7 +33,10 @@ int w4_down_tc(const void *act, int hidden, int inter, const void *w2, const w4:
                const int32_t *counters, double tiles, int64_t rows, float *y, cudaStream_t s);
 
 namespace {
-bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool aligned(const void *p, int bytes) {
+  return (reinterpret_cast<uintptr_t>(p) & static_cast<uintptr_t>(bytes - 1)) == 0;
+}
+bool aligned16(const void *p) { return aligned(p, 16); }
 
 // Rows of x up to which the weights of a dense product are streamed
 // (w4_stream.cuh); with more, tcgen05 (w4_gemm_sm100.cu).
@@ -290,6 +293,7 @@ int b200moe_w4_linear(const void *x, int64_t m, int n, int k, const void *w, int
   if (m == 0) return B200MOE_OK;
   B200_ARG(x && w && out, "null pointer argument");
   B200_ARG(aligned16(x) && aligned16(w), "x and w must be 16-byte aligned");
+  B200_ARG(aligned(out, 2), "out must be aligned to its type");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const w4::Shape sh = w4::shape_of(group, flags);
   B200_UNSUPPORTED(m < (int64_t)0x7fffffff &&
@@ -334,8 +338,11 @@ int b200moe_w4_experts(const void *x, int64_t tokens, int hidden, int inter,
   B200_ARG(tokens < (int64_t)0x7fffffff / top_k, "too many routes");
   if (tokens == 0) return B200MOE_OK;
   B200_ARG(x && expert_ids && weights && w13 && w2 && workspace && out, "null pointer argument");
-  B200_ARG(aligned16(x) && aligned16(w13) && aligned16(w2) && aligned16(workspace),
-           "x, w13, w2 and workspace must be 16-byte aligned");
+  B200_ARG(aligned16(x) && aligned16(w13) && aligned16(w2) && aligned16(workspace) &&
+               aligned16(out),
+           "x, w13, w2, workspace and out must be 16-byte aligned");
+  B200_ARG(aligned(expert_ids, 8) && aligned(weights, 2),
+           "expert_ids and weights must be aligned to their types");
   const int64_t need = b200moe_w4_experts_workspace(tokens, hidden, inter, top_k, num_experts);
   B200_ARG(workspace_bytes >= need, "workspace needs %lld bytes", (long long)need);
   // Work items are counted in 32 bits.

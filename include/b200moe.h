@@ -651,7 +651,8 @@ B200MOE_API int b200moe_w4_ring_stages(int product, int tile_rows, int group, in
 
 /*
  * Dense product out[m, n] = sum_k x[m, k] W[n, k], fp32 sums, bf16 out.
- *   x [m, k] bf16, w one laid-out matrix [n, k], out [m, n] bf16; 16-byte aligned.
+ *   x [m, k] bf16, w one laid-out matrix [n, k], out [m, n] bf16; x and w 16-byte
+ *   aligned (with out and n * 2 too, rows are stored in 16-byte pieces).
  */
 B200MOE_API int b200moe_w4_linear(const void *x, int64_t m, int n, int k, const void *w, int group,
                                   int flags, void *out, void *stream);
@@ -665,8 +666,8 @@ B200MOE_API int b200moe_w4_linear(const void *x, int64_t m, int n, int k, const 
  *   x [tokens, hidden] bf16, expert_ids [tokens, top_k] int64, weights
  *   [tokens, top_k] bf16, w13 [num_experts] laid-out SwiGLU pairs [2 inter,
  *   hidden] (B200MOE_W4_GATE_UP), w2 [num_experts] matrices [hidden, inter],
- *   out [tokens, hidden] bf16; pointers 16-byte aligned.
- *   workspace: b200moe_w4_experts_workspace bytes, 256-byte aligned.
+ *   out [tokens, hidden] bf16; all but the routes' pointers 16-byte aligned.
+ *   workspace: b200moe_w4_experts_workspace bytes, 16-byte aligned.
  * b200moe_w4_experts_launches: kernels that a call launches.
  */
 B200MOE_API int64_t b200moe_w4_experts_workspace(int64_t tokens, int hidden, int inter, int top_k,
