@@ -154,11 +154,11 @@ constexpr int kPackThreads = 1024;
 __global__ void __launch_bounds__(kPackThreads) w4_pack_routes_kernel(
     const int64_t *ids, int num_routes, int num_experts, int32_t *row_route, int32_t *mtiles,
     int32_t *counters) {
-  extern __shared__ int32_t pack_smem[];  // count[E], first row[E], first tile[E]
+  extern __shared__ int32_t pack_smem[];  // count[E], first row[E]
   __shared__ int32_t warp_rows[32], warp_tiles[32];
   pdl_trigger();
   pdl_wait();
-  int32_t *count = pack_smem, *row0 = count + num_experts, *tile0 = row0 + num_experts;
+  int32_t *count = pack_smem, *row0 = count + num_experts;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   for (int e = tid; e < num_experts; e += kPackThreads) count[e] = 0;
   __syncthreads();
@@ -365,11 +365,7 @@ int b200moe_w4_experts(const void *x, int64_t tokens, int hidden, int inter,
                               num_experts, w2, sh2, out, s);
   }
   if (b.scratch == nullptr) {
-    const size_t smem = static_cast<size_t>(num_experts) * 12;
-    if (smem > 46 * 1024)
-      B200_CUDA(cudaFuncSetAttribute(w4_pack_routes_kernel,
-                                     cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     kPackExperts * 12));
+    const size_t smem = static_cast<size_t>(num_experts) * 8;  // 32 KB at most
     B200_LAUNCH_PDL(kPdlPack, w4_pack_routes_kernel, dim3(1), dim3(kPackThreads), smem, s,
                     expert_ids, static_cast<int>(routes), num_experts, b.row_route, b.mtiles,
                     b.counters);

@@ -1,6 +1,6 @@
 // Products with 4-bit weights on tcgen05: the dense product and the experts'
-// gate/up (+ SwiGLU) and down projections, for more rows than the CUDA-core
-// kernels (w4_gemv.cu) take.
+// gate/up (+ SwiGLU) and down projections, for more rows than the streaming
+// kernels (w4_stream.cuh) take.
 //
 //   D_g[f, r] = sum_{k in group g} (q[f, k] - z[f, g]) * x[r, k]
 //   y[r, f]   = sum_g s[f, g] * D_g[f, r]
@@ -60,7 +60,7 @@ constexpr int operand_stages_of(int kind, int nt) { return kind == kDown && nt =
 
 // Whether the first CTA of a cluster has room for the others' sums of nt rows.
 constexpr bool split_ok(int split, int nt) {
-  return split >= 1 && split <= 8 && (split & (split - 1)) == 0 && (split - 1) * nt <= 112;
+  return split >= 1 && (split & (split - 1)) == 0 && (split - 1) * nt <= 112;
 }
 
 // NT: rows of x per tile (the N side); GPB: groups per block of 128 k.
@@ -78,7 +78,7 @@ struct Cfg {
   static constexpr int BS = operand_stages_of(KIND, NT);
   static constexpr bool LOCKSTEP = UPB == 1 && ND == BS;  // the two rings are one
   static constexpr int B_BYTES = NT * 256;                // 128 k of NT rows
-  static constexpr int C = NT == 16 || NT == 128 ? 8 : 16;  // columns per chunk
+  static constexpr int C = NT == 128 ? 8 : 16;              // columns per chunk
   static constexpr int DG = 2;                              // decoding groups
   static constexpr int PG = NT == 128 ? 4 : 2;              // promoting groups
   static constexpr int NCH = NT / C / PG;                   // chunks per promoting group
@@ -955,8 +955,7 @@ int launch(const CUtensorMap &mx, const CUtensorMap &mwhole, Args a, double item
   const int sms = sm_count();
   int best = 1;
   double best_time = 1e30;
-  for (int sp = 1; sp <= 8 && sp <= a.num_kb; sp *= 2) {
-    if (!split_ok(sp, NT)) break;
+  for (int sp = 1; split_ok(sp, NT) && sp <= a.num_kb; sp *= 2) {
     const double rounds = static_cast<double>(
         static_cast<int64_t>((items + sms / sp - 1) / (sms / sp)));
     const double time = rounds * ((a.num_kb + sp - 1) / sp + 2.0 + (sp > 1 ? 1.0 : 0.0));
@@ -1028,15 +1027,15 @@ int stages_of(int nt, const Shape &sh, int split) {
     }
   };
   switch (nt) {
-    case 16: return by_group(std::integral_constant<int, 16>{});
     case 32: return by_group(std::integral_constant<int, 32>{});
     case 64: return by_group(std::integral_constant<int, 64>{});
     default: return by_group(std::integral_constant<int, 128>{});
   }
 }
 
-// The smallest tile that holds `rows` rows.
-int tile_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+// The smallest tile that holds `rows` rows, or the largest.  Sixteen rows and fewer
+// are streamed (w4_stream.cuh).
+int tile_of_rows(int64_t rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 
 // x: [rows, k]; gathered four rows at a time, or in boxes of 16 and nt rows.
 template <int KIND>
@@ -1049,7 +1048,6 @@ int launch_any(const void *x, int64_t rows, int k, const Args &a, int nt, double
   if (rc) return rc;
   if (a.gather) mwhole = mx;
   switch (nt) {
-    case 16: return launch_nt<16, KIND>(mx, mwhole, a, items, s);
     case 32: return launch_nt<32, KIND>(mx, mwhole, a, items, s);
     case 64: return launch_nt<64, KIND>(mx, mwhole, a, items, s);
     default: return launch_nt<128, KIND>(mx, mwhole, a, items, s);
@@ -1070,7 +1068,7 @@ int w4_linear_tc(const void *x, int64_t m, int n, int k, const void *w, const w4
   a.staged = n % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
   a.m = m;
   a.out = out;
-  const int nt = tile_rows(m);
+  const int nt = tile_of_rows(m);
   return launch_any<kLinear>(x, m, k, a, nt, static_cast<double>((m + nt - 1) / nt) * a.n_blocks, s);
 }
 
@@ -1098,8 +1096,8 @@ int w4_gate_up_tc(const RowSource &src, int hidden, int inter, const void *w13,
   a.x_rows = src.x_rows;
   a.out = act;
   return a.gather
-             ? launch_any<kGateUp>(src.x, src.x_rows, hidden, a, tile_rows(rows), tiles * a.n_blocks, s)
-             : launch_any<kGateUp>(src.x_packed, row_capacity, hidden, a, tile_rows(rows),
+             ? launch_any<kGateUp>(src.x, src.x_rows, hidden, a, tile_of_rows(rows), tiles * a.n_blocks, s)
+             : launch_any<kGateUp>(src.x_packed, row_capacity, hidden, a, tile_of_rows(rows),
                           tiles * a.n_blocks, s);
 }
 
@@ -1122,7 +1120,7 @@ int w4_down_tc(const void *act, int hidden, int inter, const void *w2, const w4:
   a.route_w = static_cast<const __nv_bfloat16 *>(route_weights);
   a.num_routes = num_routes;
   a.out = y;
-  return launch_any<kDown>(act, row_capacity, inter, a, tile_rows(rows), tiles * a.n_blocks, s);
+  return launch_any<kDown>(act, row_capacity, inter, a, tile_of_rows(rows), tiles * a.n_blocks, s);
 }
 
 }  // namespace b200moe
@@ -1132,7 +1130,7 @@ extern "C" int b200moe_w4_ring_stages(int product, int tile_rows, int group, int
   using namespace b200moe;
   using namespace b200moe::w4g;
   B200_ARG(product >= kLinear && product <= kDown, "unknown product code %d", product);
-  B200_ARG(tile_rows == 16 || tile_rows == 32 || tile_rows == 64 || tile_rows == 128,
+  B200_ARG(tile_rows == 32 || tile_rows == 64 || tile_rows == 128,
            "no tile of %d rows", tile_rows);
   B200_ARG(w4::group_ok(group), "group size %d must be 32, 64 or 128", group);
   B200_ARG(split_ok(split, tile_rows), "no clusters of %d CTAs with %d rows", split, tile_rows);
