@@ -36,3 +36,11 @@ def test_linear(x, w, out):
     at = [ctypes.c_void_p((1 << 20) + off) for off in (x, w, out)]
     with pytest.raises(ValueError, match="aligned"):
         _lib.call("b200moe_w4_linear", at[0], 1, 8, 64, at[1], 64, 0, at[2], None)
+
+
+def test_more_experts_than_a_packing_takes():
+    size = _lib.LIB.b200moe_w4_experts_workspace(3, 64, 64, 8, 4097)
+    at = ctypes.c_void_p(1 << 20)
+    with pytest.raises(ValueError, match="4096"):
+        _lib.call("b200moe_w4_experts", at, 3, 64, 64, at, at, 8, 4097, at, 64, _lib.W4_GATE_UP,
+                  at, 64, 0, at, size, at, None)
