@@ -13,6 +13,14 @@
 // at the end, because the expert kernels take bf16 route weights.  A NaN logit
 // counts as -inf, a NaN choice likewise; a row without a finite score has
 // weights 0.
+//
+// One warp a token, because the choice is a chain of top_k rounds and a token's
+// scores fit one warp's registers; no two warps ever meet.  What bounds it: at few
+// tokens that chain (1 token of 256 experts, 8 groups: 4.6 us on the GPU, 64 of
+// 128: 3.2); at many the issue of its instructions.  8192 tokens of 256 experts
+// take 16-17 us, of which 1570 instructions a token are 11 us of all schedulers'
+// issue (profiled: 70 % of the cycles issue, the integer pipe 73 %); their 8.4 MB
+// would take 1.4.
 #include "common.cuh"
 
 namespace b200moe {

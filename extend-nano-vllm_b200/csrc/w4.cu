@@ -113,8 +113,14 @@ struct ExpertBuffers {
           *tile_expert = nullptr, *offsets = nullptr, *counts = nullptr, *mtiles = nullptr,
           *counters = nullptr, *scratch = nullptr;
   __nv_bfloat16 *x_packed = nullptr;  // above kGatherRoutes routes
-  __nv_bfloat16 *act = nullptr;       // [row_capacity, inter], packed order (few routes: route order)
-  float *y = nullptr;                 // [routes, hidden], route order
+  // [row_capacity, inter], packed order (few routes: route order).  bf16, the type
+  // of the down product's operand: the call's error against 64 bits is 0.0023 of
+  // the result with it and would be 0.0017 (the last store's) without; the bf16
+  // experts round here too.
+  __nv_bfloat16 *act = nullptr;
+  // [routes, hidden], route order.  fp32: in bf16 the rows would be half of the
+  // traffic (8192 tokens, top-8, 2048 wide: 537 MB written and read) and the error 0.0029.
+  float *y = nullptr;
 };
 
 ExpertBuffers expert_buffers(Workspace &ws, int64_t tokens, int hidden, int inter, int top_k,

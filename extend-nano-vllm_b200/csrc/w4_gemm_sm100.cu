@@ -23,15 +23,18 @@
 // Every wait is bounded; on expiry the CTA records a status bit and leaves.
 //
 // What bounds it: at 128 rows the turns that matrix instructions, promoting and
-// decoding take.  A block of 128 x 128 weights takes 590 cycles of matrix
-// instructions (74 each; 37 at 16 rows) out of some 1050: TMEM holds two
-// accumulators beside the operand stages, and decoding (seven ALU instructions
-// of two cycles per eight codes) and promoting fill half of the issue slots.
+// decoding take.  A block of 128 x 128 weights takes some 1050 cycles (profiled,
+// 4096 rows x [4096, 4096]), the tensor pipe works in 49 % of them: TMEM holds two
+// accumulators beside the operand stages.  Decoding and promoting take 64 % of the
+// issue slots (the integer pipe 51 %) and wait for TMEM most.  With groups of 32 a
+// block takes some 1940 cycles, the tensor pipe 26 %: four accumulators to promote
+// instead of one.
 // Neither fewer reads of x (a pair of SMs: slower, its hand-overs cross the
 // pair) nor more decoding warps or fewer, larger promoting warps helped.
-// Measured (back to back): 32 rows x [75776, 4096] 52 us = 3.05 TB/s of weights,
-// 64 rows 58 us, 128 rows 83 us; 4096 rows x [4096, 4096] 132 us = 1.04 PFLOP/s
-// (cuBLAS bf16 burst 1.64); groups of 32 with zero points, 64 rows: 91 us.
+// Measured (back to back): 32 rows x [75776, 4096] 54 us = 2.95 TB/s of weights,
+// 64 rows 60 us, 128 rows 84 us; 4096 rows x [4096, 4096] 133 us = 1.03 PFLOP/s
+// (cuBLAS bf16 burst 1.64).  Groups of 32 with zero points: 64 rows 93 us, 128 rows
+// 141 us; 4096 rows x [4096, 4096] 240 us, groups of 64 157 us.
 #include <cudaTypedefs.h>
 
 #include <type_traits>
@@ -311,8 +314,8 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int
 }
 
 // One lane of the warp, in a form that tells the compiler so: matrix
-// instructions issued under it take uniform registers (37 cycles each at
-// N = 16); under a test of the lane number they took 128.
+// instructions issued under it take uniform registers (37 cycles each, measured at
+// N = 16, against 128 under a test of the lane number).
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
   asm volatile(

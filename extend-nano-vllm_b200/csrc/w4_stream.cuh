@@ -13,15 +13,18 @@
 // has 11 cycles for 512 codes, and decoding them takes 7 of each scheduler's.
 // (tcgen05 wants the operand decoded by one warp, waited for by another and
 // read back by a third; that pays from more than 16 rows on, w4_gemm_sm100.cu:
-// 16 rows x [151552, 4096] take 92 us here and 107 there, 32 rows 220 and 107.)
+// x [151552, 4096], 16 rows take 92 us here, in a tcgen05 tile of their own they
+// took 107; 32 rows 220 here in passes of 32 and 100 there.)
 //
 // Measured (back to back, weights larger than L2): 1 row x [75776, 4096] 34.4 us
 // = 4.65 TB/s of weights, 8 rows x [151552, 4096] 67.0 us = 4.78 TB/s, 16 rows
 // 92.1 us = 3.48 TB/s; 8 rows x [75776, 4096] with groups of 32 and zero points
 // 49.3 us = 3.74 TB/s; copy peak 6.5 TB/s.  What bounds it: no one unit.  With 8
-// rows the schedulers issue in 59 % of cycles (297 instructions per 32 x 128
-// weights) and wait for loads and for the decoding's integer pipe in turn; 16 warps
-// with a block in flight each are what the registers hold.  A row's four units lie
+// rows (profiled on 75776 x 4096) the integer pipe works in 67 % of cycles and the
+// schedulers issue in 60 % (297 instructions per 32 x 128 weights); warps wait for
+// fixed latencies, for that pipe and for loads in turn (1.5, 1.2 and 1.0 of them an
+// issue), at half of the DRAM's rate.  16 warps with a block in flight each are
+// what the registers hold.  A row's four units lie
 // side by side (w4.cuh): 512 bytes apart they took 34.2, 68, 97 and 50.6 us.
 // A ring of asynchronous copies in shared memory per warp, four deep, in place
 // of the registers took 42, 84 and 104 us for the first three: it fetches as far
@@ -453,7 +456,7 @@ int run(Args a, double items, int64_t most, int cols, cudaStream_t s) {
   // call with 1 / 2 / 4 / 8 warps: 64 tokens through 128 experts, gate/up (16 blocks
   // of k) 123 / 115 / 113 / 120, down (6 blocks) 115 / 118 / 131; down of 16 tokens
   // through 16 experts (50 blocks) 191 / 180 / 180 / 179; two rows x [8192, 4096]
-  // 21 / 12 / 9.2 / 5.9, x [37888, 4096] 24.0 / 17.8 / 19.0 / 20.7.  The cost is
+  // 19.6 / 12.0 / 9.6 / 6.5, x [37888, 4096] 23.0 / 18.8 / 19.3 / 20.9.  The cost is
   // rounds of items, each as long as its blocks and some to begin and end.
   double best = 1e30;
   a.wk = 1;
