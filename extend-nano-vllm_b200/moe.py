@@ -503,7 +503,7 @@ class ExpertParallelMoE(_W4Holder):
     def set_w4_weights(self, w13: _native_ops.W4Weight, w2: _native_ops.W4Weight) -> None:
         """Run the experts with 4-bit weights (``ops.pack_w4``: w13 [E, 2 I, H] in
         the "gate_up" layout, w2 [E, H, I]) and release the bf16 ones.  One EP
-        rank; the layer's weights can no longer be loaded or relocated.  A call
+        rank; bf16 expert weights can no longer be loaded or relocated.  A call
         that raises leaves the layer as it was."""
         self._check_w4_supported()
         hidden, inter = self.hidden_size, self.intermediate_size
