@@ -141,16 +141,18 @@ class _W4Holder(nn.Module):
         if all(t is not None for t in saved):
             try:
                 # Before the bf16 parameters, which are empty beside 4-bit weights.
-                self._load_w4(names, saved)
+                self._load_w4(names, saved,
+                              local_metadata.get("assign_to_params_buffers", False))
             except (ValueError, NotImplementedError) as exc:
                 error_msgs.append(str(exc))
         elif strict and (self._w4 is not None or any(t is not None for t in saved)):
             missing_keys += [name for name, t in zip(names, saved) if t is None]
-        super()._load_from_state_dict({k: v for k, v in state_dict.items() if k not in names},
-                                      prefix, local_metadata, strict, missing_keys,
+        for name in names:
+            state_dict.pop(name, None)
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys,
                                       unexpected_keys, error_msgs)
 
-    def _load_w4(self, names: list[str], saved: list[torch.Tensor]) -> None:
+    def _load_w4(self, names: list[str], saved: list[torch.Tensor], assign: bool) -> None:
         weights = []
         for name, data, layout in zip(names[::2], saved[::2], saved[1::2]):
             layout = [int(v) for v in layout.flatten()]
@@ -158,14 +160,15 @@ class _W4Holder(nn.Module):
             if data.dtype != torch.uint8 or data.dim() != 1 or data.numel() != size:
                 raise ValueError(f"{name} does not hold a 4-bit weight of layout {layout}")
             weights.append(_native_ops.W4Weight(data, *layout))
-        if self._w4 is not None and all(new.layout == old.layout
-                                        for new, old in zip(weights, self._w4)):
-            for new, old in zip(weights, self._w4):  # in place: captured graphs stay valid
-                old.data.copy_(new.data)
-            return
-        device = next(self.parameters()).device
-        for weight in weights:
-            weight.data = weight.data.to(device, copy=True)
+        if not assign:
+            if self._w4 is not None and all(new.layout == old.layout
+                                            for new, old in zip(weights, self._w4)):
+                for new, old in zip(weights, self._w4):  # in place: captured graphs stay valid
+                    old.data.copy_(new.data)
+                return
+            device = next(self.parameters()).device
+            for weight in weights:
+                weight.data = weight.data.to(device, copy=True)
         self.set_w4_weights(*weights)
 
 

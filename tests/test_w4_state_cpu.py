@@ -191,3 +191,39 @@ def test_loading_what_does_not_fit_raises(packed_by_shape):
     short["w4_w2"] = short["w4_w2"][:-1]
     with pytest.raises(RuntimeError, match="w4_w2"):
         rounded.load_state_dict(short)
+
+
+def test_loading_into_a_layer_on_meta(packed_by_shape):
+    layer = layer_of(64)
+    layer.quantize_w4(32)
+    saved = filled(layer, 3).state_dict()
+    with torch.device("meta"):
+        fresh = ExpertParallelMoE(64, 32, 8, 2, True, shared_expert_intermediate_size=64)
+    torch.nn.ModuleDict({"mlp": fresh}).load_state_dict(
+        {f"mlp.{n}": t for n, t in saved.items()}, assign=True)
+    for a, b in zip(packed_of(layer), packed_of(fresh)):
+        assert b.data.device.type == "cpu" and torch.equal(a.data, b.data)
+    other = filled(layer_of(64), 4)
+    other.quantize_w4(32)
+    other.load_state_dict(saved, assign=True)
+    assert all(torch.equal(a.data, b.data) for a, b in zip(packed_of(layer), packed_of(other)))
+
+
+def test_hooks_see_and_change_the_state_dict_that_is_loaded(packed_by_shape):
+    # A hook of the layer that renames what an older version saved for a part of it.
+    for rounded in (False, True):
+        layer, other = layer_of(64), layer_of(64)
+        if rounded:
+            layer.quantize_w4(32)
+        saved = layer.state_dict()
+        saved["shared_expert_gate.old"] = saved.pop("shared_expert_gate.weight")
+
+        def rename(module, state_dict, prefix, *rest):
+            state_dict[f"{prefix}shared_expert_gate.weight"] = state_dict.pop(
+                f"{prefix}shared_expert_gate.old")
+
+        other.register_load_state_dict_pre_hook(rename)
+        with torch.no_grad():
+            other.shared_expert_gate.weight.zero_()
+        other.load_state_dict(saved)
+        assert torch.equal(other.shared_expert_gate.weight, layer.shared_expert_gate.weight)
